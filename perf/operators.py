@@ -28,6 +28,11 @@ def ceil(a, b):
     return -(-a // b)
 
 
+def _over_448(m):
+    """m / 448 (e4m3's largest value), one rounding: torch divides by a plain number through its reciprocal."""
+    return m / torch.full_like(m, 448.0)
+
+
 # ---- the cases -------------------------------------------------------------------------
 
 def listed():
@@ -104,7 +109,7 @@ def _weights(shape, type_, g):
     p = torch.zeros((*lead, Ob * G, Kb * G), device="cuda")
     p[..., :O, :K] = w
     p = p.view(*lead, Ob, G, Kb, G)
-    s = p.abs().amax(dim=(-3, -1)) / 448
+    s = _over_448(p.abs().amax(dim=(-3, -1)))
     s = torch.where(s == 0, torch.ones_like(s), s)
     q = (p / s[..., :, None, :, None]).clamp(-448, 448).view(*lead, Ob * G, Kb * G)[..., :O, :K].to(E4M3)
     return q.contiguous(), s
@@ -164,7 +169,7 @@ def _encode(x):
     p = torch.zeros((n, Kb * G), device=x.device)
     p[:, :d] = x.float()
     p = p.view(n, Kb, G)
-    s = p.abs().amax(dim=2) / 448
+    s = _over_448(p.abs().amax(dim=2))
     s = torch.where(s == 0, torch.ones_like(s), s)
     q = (p / s[:, :, None]).clamp(-448, 448).view(n, Kb * G)[:, :d].to(E4M3)
     return q.contiguous(), s.t().contiguous().t()
