@@ -1,0 +1,33 @@
+// Shared by the float experts' kernels: element types, scales and rounding.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "mb_common.cuh"
+
+constexpr int kScaleBlock = MB_SCALE_BLOCK;
+
+// The scale of a group whose largest magnitude is m: m / 448, and 1 where that is 0 (a group of zeros, or of values so
+// small that the quotient underflows), as mb_encode_rows does for int8.
+__device__ __forceinline__ float e4m3_scale(float m)
+{
+    const float s = __fdiv_rn(m, 448.0f);
+    return s == 0.0f ? 1.0f : s;
+}
+
+// Nearest e4m3 (ties to even).  Saturation matters only where s is subnormal: x / s may then round to above 448.
+__device__ __forceinline__ uint8_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+
+// out[i] = v, rounded once (to nearest even) to the type; not e4m3.
+template <int TYPE>
+__device__ __forceinline__ void store_out(void* out, int64_t i, float v)
+{
+    if (TYPE == MB_T_F32)
+        reinterpret_cast<float*>(out)[i] = v;
+    else if (TYPE == MB_T_BF16)
+        reinterpret_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+    else
+        reinterpret_cast<__half*>(out)[i] = __float2half_rn(v);
+}

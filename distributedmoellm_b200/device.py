@@ -329,6 +329,230 @@ def matmul_t(w_tiles: torch.Tensor, fmt: int, O: int, K: int, x: torch.Tensor, y
     return y
 
 
+# ---- float experts: e4m3 with block scales, bf16, f16 -----------------------------------
+
+SCALE_BLOCK = 128
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
+OPERAND_TYPES = (torch.float8_e4m3fn, torch.bfloat16, torch.float16)
+RESULT_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // SCALE_BLOCK)
+
+
+def _want(t, name, shape, dtypes):
+    if t is None:
+        raise ValueError(f"{name} is missing")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} is {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
+
+
+def _rows_of(t, name):
+    """Elements between the rows of t (..., rows, columns), whose columns must be adjacent."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"the columns of {name} must be adjacent (strides {t.stride()})")
+    return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], t.stride(-2))
+
+
+def _row_stride(t, name):
+    """As :func:`_rows_of`; a single row's distance is rounded up to 16 bytes, since nothing lies behind it."""
+    ld = _rows_of(t, name)
+    if t.shape[-2] <= 1:
+        step = 16 // t.element_size()
+        ld = -(-max(ld, t.shape[-1]) // step) * step
+    return ld
+
+
+def _one_device(*ts):
+    """The device all of ts are on."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("expected CUDA tensors")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices ({dev}, {t.device})")
+        dev = t.device
+    return dev
+
+
+def _status_word(status):
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise ValueError("status must be one int32")
+
+
+def _new_scales(n: int, groups: int, device):
+    """Scales (n, groups), stored group after group: the products read one group of many rows at a time."""
+    return torch.empty((groups, n), dtype=torch.float32, device=device).t()
+
+
+def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                 scales: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """Rows of x (T, d) f32 / bf16 / f16 in the form the grouped products take:
+    x[rows] (all of x when rows is None; rows int32, as Routing.sorted_rows)
+    rounded to ``dtype``.  torch.float8_e4m3fn: each group of 128 columns over
+    its scale max|x| / 448.  Returns (q (n, d), scales (n, ceil(d / 128)) f32
+    or None); rows of q and the scales may have any strides, columns of x and q
+    must be adjacent.  An index outside x sets bit 2 of ``status`` and gives a row
+    of zeros."""
+    if x.dim() != 2 or x.dtype not in RESULT_TYPES:
+        raise ValueError(f"operand_rows takes (rows, columns) of f32, bf16 or f16, got {tuple(x.shape)} {x.dtype}")
+    if dtype not in OPERAND_TYPES:
+        raise ValueError(f"operand type {dtype}, expected one of {', '.join(str(d) for d in OPERAND_TYPES)}")
+    if rows is not None and (rows.dim() != 1 or rows.dtype != torch.int32 or not rows.is_contiguous()):
+        raise ValueError("rows must be a contiguous vector of int32")
+    T, d = x.shape
+    n = T if rows is None else rows.numel()
+    e4m3 = dtype == torch.float8_e4m3fn
+    if q is not None:
+        _want(q, "q", (n, d), (dtype,))
+        _rows_of(q, "q")
+    if scales is not None:
+        if not e4m3:
+            raise ValueError(f"{dtype} rows have no scales")
+        _want(scales, "scales", (n, _blocks(d)), (torch.float32,))
+    _rows_of(x, "x")
+    _status_word(status)
+    dev = _one_device(x, rows, q, scales, status)
+    with torch.cuda.device(dev):
+        q = torch.empty((n, d), dtype=dtype, device=dev) if q is None else q
+        if e4m3 and scales is None:
+            scales = _new_scales(n, _blocks(d), dev)
+        sr, sg = scales.stride() if e4m3 else (0, 0)
+        check(lib().mb_operand_rows(_p(x), _TYPES[x.dtype], _rows_of(x, "x"), T, _p(rows), n, d, _TYPES[dtype],
+                                    _p(q), _rows_of(q, "q"), _p(scales), sr, sg, _p(status), _stream()),
+              "mb_operand_rows")
+    return q, scales
+
+
+def _operands(x, w, xs, ws, ws_shape):
+    """Checks of a product's rows x (P, K) and matrices w (..., O, K) with their scales."""
+    if x.dim() != 2 or x.dtype not in OPERAND_TYPES:
+        raise ValueError(f"rows must be (P, K) of e4m3, bf16 or f16, got {tuple(x.shape)} {x.dtype}")
+    if w.dtype != x.dtype:
+        raise ValueError(f"rows of {x.dtype} with weights of {w.dtype}")
+    if w.shape[-1] != x.shape[1]:
+        raise ValueError(f"rows of {x.shape[1]} columns with weights of {w.shape[-1]}")
+    if x.dtype == torch.float8_e4m3fn:
+        _want(xs, "xs", (x.shape[0], _blocks(x.shape[1])), (torch.float32,))
+        _want(ws, "ws", ws_shape, (torch.float32,))
+        if not ws.is_contiguous():
+            raise ValueError("ws must be contiguous")
+        return xs.stride()
+    if xs is not None or ws is not None:
+        raise ValueError(f"{x.dtype} operands have no scales")
+    return 0, 0
+
+
+def _groups(w, offsets):
+    if w.dim() != 3:
+        raise ValueError(f"weights must be (E, O, K), got {tuple(w.shape)}")
+    _want(offsets, "offsets", (w.shape[0] + 1,), (torch.int32,))
+    if not offsets.is_contiguous():
+        raise ValueError("offsets must be contiguous")
+
+
+def matmul_t_e4m3(x: torch.Tensor, xs: torch.Tensor, w: torch.Tensor, ws: torch.Tensor, y: torch.Tensor | None = None,
+                  dtype: torch.dtype | None = None, status: torch.Tensor | None = None):
+    """x @ w.T of e4m3 rows x (n, K) with scales xs (n, ceil(K/128)), as
+    operand_rows makes them, and an e4m3 matrix w (O, K) with one f32 scale per
+    block of 128 x 128, ws (ceil(O/128), ceil(K/128)).  y (n, O) of ``dtype``
+    (f32 unless said otherwise, bf16 or f16); f32 sums.  Rows of x and w must lie
+    a multiple of 16 bytes apart."""
+    if w.dim() != 2:
+        raise ValueError(f"w must be (O, K), got {tuple(w.shape)}")
+    if x.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"matmul_t_e4m3 takes rows of e4m3, got {x.dtype}")
+    xr, xg = _operands(x, w, xs, ws, (_blocks(w.shape[0]), _blocks(w.shape[1])))
+    n, O = x.shape[0], w.shape[0]
+    dtype = (torch.float32 if y is None else y.dtype) if dtype is None else dtype
+    if dtype not in RESULT_TYPES:
+        raise ValueError(f"result type {dtype}")
+    if y is not None:
+        _want(y, "y", (n, O), (dtype,))
+        _rows_of(y, "y")
+    ldx, ldw = _row_stride(x, "x"), _row_stride(w, "w")
+    _status_word(status)
+    dev = _one_device(x, xs, w, ws, y, status)
+    with torch.cuda.device(dev):
+        y = torch.empty((n, O), dtype=dtype, device=dev) if y is None else y
+        check(lib().mb_matmul_t_e4m3(_p(x), ldx, _p(xs), xr, xg, n, _p(w), ldw, _p(ws), O, x.shape[1], _p(y),
+                                     _TYPES[dtype], _rows_of(y, "y"), _p(status), _stream()), "mb_matmul_t_e4m3")
+    return y
+
+
+def grouped_matmul_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs: torch.Tensor | None = None,
+                     ws: torch.Tensor | None = None, y: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+                     status: torch.Tensor | None = None):
+    """y[p] = x[p] @ w[e].T for the rows offsets[e] <= p < offsets[e+1] of every
+    expert (offsets: Routing.offsets).  x (P, K) and w (E, O, K) both bf16,
+    both f16, or both e4m3 with xs (P, ceil(K/128)) and ws (E, ceil(O/128),
+    ceil(K/128)).  y (P, O) of ``dtype`` (f32 unless said otherwise, bf16 or
+    f16); f32 sums.  Rows of y outside every expert's range are not written.
+    Rows and matrices of x and w must lie a multiple of 16 bytes apart.
+    Offsets that decrease or pass P set bit 2 of ``status``."""
+    _groups(w, offsets)
+    E, O, K = w.shape
+    xr, xg = _operands(x, w, xs, ws, (E, _blocks(O), _blocks(K)))
+    P = x.shape[0]
+    dtype = (torch.float32 if y is None else y.dtype) if dtype is None else dtype
+    if dtype not in RESULT_TYPES:
+        raise ValueError(f"result type {dtype}")
+    if y is not None:
+        _want(y, "y", (P, O), (dtype,))
+        _rows_of(y, "y")
+    ldx, ldw = _row_stride(x, "x"), _row_stride(w, "w")
+    _status_word(status)
+    dev = _one_device(x, w, offsets, xs, ws, y, status)
+    with torch.cuda.device(dev):
+        y = torch.empty((P, O), dtype=dtype, device=dev) if y is None else y
+        check(lib().mb_grouped_matmul_t(_p(x), _TYPES[x.dtype], ldx, _p(xs), xr, xg, P, _p(w), w.stride(0), ldw,
+                                        _p(ws), E, O, K, _p(offsets), _p(y), _TYPES[dtype], _rows_of(y, "y"),
+                                        _p(status), _stream()), "mb_grouped_matmul_t")
+    return y
+
+
+def grouped_swiglu_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs: torch.Tensor | None = None,
+                     ws: torch.Tensor | None = None, q: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                     status: torch.Tensor | None = None):
+    """The grouped product with gate|up matrices w (E, 2I, K) (I gate rows, then
+    I up rows; ws (E, 2, ceil(I/128), ceil(K/128)) for e4m3), SiLU(gate) * up
+    in f32, and its rows in operand form of x's type: returns (q (P, I), scales
+    (P, ceil(I/128)) or None), what the down product takes.  Otherwise as
+    grouped_matmul_t."""
+    _groups(w, offsets)
+    E, I2, K = w.shape
+    if I2 % 2:
+        raise ValueError(f"a gate|up matrix has an even number of rows, got {I2}")
+    I = I2 // 2
+    e4m3 = x.dtype == torch.float8_e4m3fn
+    xr, xg = _operands(x, w, xs, ws, (E, 2, _blocks(I), _blocks(K)))
+    P = x.shape[0]
+    if q is not None:
+        _want(q, "q", (P, I), (x.dtype,))
+        _rows_of(q, "q")
+    if scales is not None:
+        if not e4m3:
+            raise ValueError(f"{x.dtype} rows have no scales")
+        _want(scales, "scales", (P, _blocks(I)), (torch.float32,))
+    ldx, ldw = _row_stride(x, "x"), _row_stride(w, "w")
+    _status_word(status)
+    dev = _one_device(x, w, offsets, xs, ws, q, scales, status)
+    with torch.cuda.device(dev):
+        q = torch.empty((P, I), dtype=x.dtype, device=dev) if q is None else q
+        if e4m3 and scales is None:
+            scales = _new_scales(P, _blocks(I), dev)
+        sr, sg = scales.stride() if e4m3 else (0, 0)
+        check(lib().mb_grouped_swiglu_t(_p(x), _TYPES[x.dtype], ldx, _p(xs), xr, xg, P, _p(w), w.stride(0), ldw,
+                                        _p(ws), E, I, K, _p(offsets), _p(q), _rows_of(q, "q"), _p(scales), sr, sg,
+                                        _p(status), _stream()), "mb_grouped_swiglu_t")
+    return q, scales
+
+
 __all__ = [n for n in dir() if not n.startswith("_")] + ["_lib"]
 
 

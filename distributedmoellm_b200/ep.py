@@ -42,6 +42,7 @@ import torch.distributed as dist
 from . import device as D
 from .layout import FMT_Q4K_F32
 from .layer import GEMM_MIN_ROWS, run_experts
+from .store import FloatExperts
 
 
 def local_plan(recv_ec: np.ndarray):
@@ -379,6 +380,8 @@ class EPPeerLayer:
         self.rank = dist.get_rank(group)
         if E % self.world or experts.E != E // self.world:
             raise ValueError(f"E={E} experts do not split into {self.world} slices of {experts.E}")
+        if isinstance(experts, FloatExperts):
+            raise ValueError("EPPeerLayer dispatches rows in the packed experts' f16 form; use EPLayer or EPGatherLayer")
         if experts.fmt_gu == FMT_Q4K_F32:
             raise ValueError("EPPeerLayer: Q4_K experts need the precise gate|up form over f32 rows; use EPLayer")
         self.E_local = E // self.world

@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import device as D
-from .store import LayerExperts
+from .store import FloatExperts, LayerExperts
 
 # average picks per expert from which a layer's experts run as grouped GEMMs (see kernel_plan)
 GEMM_MIN_ROWS = 12
@@ -31,7 +31,9 @@ def uses_gemm(experts: LayerExperts, P: int, gemm_min_rows: int) -> bool:
 
 
 def kernel_plan(experts, P: int, gemm_min_rows: int) -> list:
-    """Which kernels run for P picks over these experts: ("gemm", 1), every
+    """Which kernels run for P picks over these experts: ("float", 0), the
+    grouped products of float experts, whatever P; for packed experts
+    ("gemm", 1), every
     expert as a grouped GEMM, or ("decode", 0), every expert on the decode
     mat-vecs.  Timed on B200 at the Qwen3-30B shape (expert kernels, graph
     replays): 128 experts at 1024 / 2048 / 4096 picks take 170 / 172 / 180 us
@@ -42,7 +44,42 @@ def kernel_plan(experts, P: int, gemm_min_rows: int) -> list:
     expert: the GEMM from 12 picks per expert on average (at 8 the two are
     even on one GPU and the decode kernel measured ahead in a 2-GPU
     expert-parallel step, where each rank's 64 experts get 8 picks)."""
+    if isinstance(experts, FloatExperts):
+        return [("float", 0)]
     return [("gemm", 1)] if uses_gemm(experts, P, gemm_min_rows) else [("decode", 0)]
+
+
+def _float_buffers(ex: FloatExperts, P: int, workspace):
+    """(x rows, their scales, activation rows, their scales) for P picks, cut from one workspace buffer."""
+    sz = ex.dtype.itemsize
+    e4m3 = ex.dtype == torch.float8_e4m3fn
+    parts, at = [], 0
+    for cols in (ex.H, ex.I):
+        ld = -(-cols * sz // 16) * 16                     # bytes between operand rows
+        groups = -(-cols // D.SCALE_BLOCK) if e4m3 else 0
+        parts.append((at, ld, cols, groups, at + -(-P * ld // 256) * 256))
+        at = parts[-1][4] + -(-P * groups * 4 // 256) * 256
+    buf = workspace("float", max(at, 256))
+    out = []
+    for q0, ld, cols, groups, s0 in parts:
+        out.append(buf[q0:q0 + P * ld].view(P, ld).view(ex.dtype)[:, :cols])
+        out.append(buf[s0:s0 + P * groups * 4].view(torch.float32).view(groups, P).t() if e4m3 else None)
+    return out
+
+
+def run_float_experts(ex: FloatExperts, x: torch.Tensor, routing, y: torch.Tensor, workspace,
+                      status: torch.Tensor) -> None:
+    """Every expert's picks through its float matrices into y (one row per
+    pick, in routing order): the picks' rows in operand form, the grouped
+    gate|up product with SiLU(gate) * up back in operand form, the grouped down
+    product with f32 results."""
+    P = routing.P
+    if P == 0:
+        return
+    q, qs, a, as_ = _float_buffers(ex, P, workspace)
+    D.operand_rows(x, ex.dtype, routing.sorted_rows[:P], q, qs, status)
+    D.grouped_swiglu_t(q, ex.gu, routing.offsets, qs, ex.gu_s, a, as_, status)
+    D.grouped_matmul_t(a, ex.down, routing.offsets, as_, ex.dn_s, y[:P], status=status)
 
 
 def run_experts(experts: LayerExperts, x: torch.Tensor, row_exp: torch.Tensor, routing, y: torch.Tensor,
@@ -53,6 +90,8 @@ def run_experts(experts: LayerExperts, x: torch.Tensor, row_exp: torch.Tensor, r
     nbytes that stays the same between calls of the same size.  ``picks``:
     the picks these experts get (default routing.P; smaller when routing
     covers other ranks' experts too), for the choice of kernels."""
+    if isinstance(experts, FloatExperts):
+        return run_float_experts(experts, x, routing, y, workspace, status)
     ex, P = experts, routing.P
     plan = kernel_plan(ex, P if picks is None else picks, gemm_min_rows)
     for kind, rows in plan:
@@ -66,7 +105,7 @@ def run_experts(experts: LayerExperts, x: torch.Tensor, row_exp: torch.Tensor, r
 
 
 class _Buffers:
-    def __init__(self, T: int, E: int, k: int, H: int, I: int, dev):
+    def __init__(self, T: int, E: int, k: int, H: int, I: int, dev, packed: bool = True):
         P = T * k
         self.logits = torch.empty((T, E), dtype=torch.float32, device=dev)
         self.row_exp = torch.empty(T, dtype=torch.int32, device=dev)
@@ -74,24 +113,26 @@ class _Buffers:
         self.w = torch.empty((T, k), dtype=torch.float32, device=dev)
         self.routing = D.Routing(T, k, E, dev)
         self.y = torch.empty((max(P, 1), H), dtype=torch.float32, device=dev)
-        self.ws = torch.empty(D.decode_workspace_bytes(P, I), dtype=torch.uint8, device=dev)
+        self.ws = torch.empty(D.decode_workspace_bytes(P, I) if packed else 0, dtype=torch.uint8, device=dev)
         self.rws = torch.empty(D.router_workspace_bytes(T, H, E), dtype=torch.uint8, device=dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self.out = torch.empty((T, H), dtype=torch.float32, device=dev)
-        self.pws = None     # grouped-GEMM workspace, made on first use
+        self.pws = None     # grouped-GEMM workspace (float experts: operand rows), made on first use
 
 
 class MoELayer:
-    """``router`` (E, H) f32 on the device; ``experts`` the layer's packed experts.
+    """``router`` (E, H) f32 on the device; ``experts`` the layer's packed experts
+    (LayerExperts) or float experts (FloatExperts).
 
     Once the layer's picks average ``gemm_min_rows`` per expert (prefill-sized
     batches) every expert runs as a grouped GEMM on the tensor cores (f16
     operands, f32 accumulation; the reference's dense path for 8 or more
     rows, experts.py:148-151, 216-219), below that through the f32-exact
     decode mat-vecs (see kernel_plan); ``gemm_min_rows=0`` keeps every expert
-    on the decode kernels."""
+    on the decode kernels.  Float experts run as grouped products at every
+    size."""
 
-    def __init__(self, router: torch.Tensor, experts: LayerExperts, top_k: int, normalize: bool = True,
+    def __init__(self, router: torch.Tensor, experts: LayerExperts | FloatExperts, top_k: int, normalize: bool = True,
                  gemm_min_rows: int = GEMM_MIN_ROWS):
         self.router = router.contiguous()
         self.experts = experts
@@ -111,7 +152,8 @@ class MoELayer:
     def buffers(self, T: int) -> _Buffers:
         b = self._bufs.get(T)
         if b is None:
-            b = self._bufs[T] = _Buffers(T, self.E, self.k, self.H, self.I, self.router.device)
+            b = self._bufs[T] = _Buffers(T, self.E, self.k, self.H, self.I, self.router.device,
+                                          not isinstance(self.experts, FloatExperts))
         return b
 
     def route(self, x: torch.Tensor) -> _Buffers:

@@ -141,3 +141,65 @@ class LayerExperts:
     @property
     def nbytes(self) -> int:
         return self.buf.numel()
+
+
+def _float_up(a, dtype, dev) -> torch.Tensor:
+    """A host array or tensor of the stored type as a contiguous tensor on dev; e4m3 bytes may come as uint8 and bf16
+    bits as uint16 (numpy has neither type)."""
+    t = a if isinstance(a, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(a))
+    bits = {torch.float8_e4m3fn: torch.uint8, torch.bfloat16: torch.uint16}.get(dtype)
+    if t.dtype == bits:
+        t = t.contiguous().view(dtype)
+    if t.dtype != dtype:
+        raise ValueError(f"matrix of {t.dtype} for experts of {dtype}")
+    return t.to(dev).contiguous()
+
+
+class FloatExperts:
+    """One MoE layer's experts as floating-point matrices on a device: torch
+    dtype float8_e4m3fn (with one f32 scale per block of 128 x 128 weights),
+    bfloat16 or float16.  gu (E, 2I, H): each expert's gate rows, then its up
+    rows; down (E, H, I); for e4m3 gu_s (E, 2, ceil(I/128), ceil(H/128)) and
+    dn_s (E, ceil(H/128), ceil(I/128)).  moelan keeps such experts dense in
+    host memory (moelan/experts.py:72-122)."""
+
+    def __init__(self, E: int, H: int, I: int, dtype: torch.dtype, device):
+        from . import device as D
+        if dtype not in D.OPERAND_TYPES:
+            raise ValueError(f"float experts are e4m3, bf16 or f16, not {dtype}")
+        self.E, self.H, self.I, self.dtype = E, H, I, dtype
+        self.device = torch.device(device)
+
+        def mats(rows, cols):          # rows a multiple of 16 bytes apart, as the products need them
+            step = 16 // dtype.itemsize
+            return torch.zeros((E, rows, -(-cols // step) * step), dtype=dtype, device=self.device)[..., :cols]
+        self.gu, self.down = mats(2 * I, H), mats(H, I)
+        self.gu_s = self.dn_s = None
+        if dtype == torch.float8_e4m3fn:
+            Hb, Ib = -(-H // D.SCALE_BLOCK), -(-I // D.SCALE_BLOCK)
+            self.gu_s = torch.ones((E, 2, Ib, Hb), dtype=torch.float32, device=self.device)
+            self.dn_s = torch.ones((E, Hb, Ib), dtype=torch.float32, device=self.device)
+        self.present: set[int] = set()
+
+    def put(self, e: int, gu, down, gu_s=None, dn_s=None) -> None:
+        """Store expert ``e``: gu (2I, H), down (H, I) and, for e4m3, the block
+        scales of the gate and of the up rows gu_s (2, ceil(I/128), ceil(H/128))
+        and dn_s (ceil(H/128), ceil(I/128))."""
+        if not 0 <= e < self.E:
+            raise KeyError(f"expert {e} of {self.E}")
+        if (gu_s is None) != (self.gu_s is None) or (dn_s is None) != (self.dn_s is None):
+            raise ValueError(f"{self.dtype} experts " + ("need block scales" if gu_s is None else "have no scales"))
+        todo = [(self.gu[e], _float_up(gu, self.dtype, self.device)),
+                (self.down[e], _float_up(down, self.dtype, self.device))]
+        if gu_s is not None:
+            todo += [(d[e], _up(s, self.device).to(torch.float32)) for d, s in ((self.gu_s, gu_s), (self.dn_s, dn_s))]
+        for dst, src in todo:
+            if dst.shape != src.shape:
+                raise ValueError(f"expert {e}: {tuple(src.shape)} does not match {tuple(dst.shape)}")
+        for dst, src in todo:
+            dst.copy_(src)
+        self.present.add(e)
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.untyped_storage().nbytes() for t in (self.gu, self.down, self.gu_s, self.dn_s) if t is not None)

@@ -353,6 +353,76 @@ int64_t mb_matmul_t_workspace_bytes(int64_t n);
 int mb_matmul_t(const void *w_tiles, int fmt, int O, int K, const float *x, int64_t n, float *y, void *workspace,
                 int64_t workspace_bytes, unsigned *status, void *stream);
 
+/* ---- float experts: e4m3 with block scales, bf16, f16 -----------------------------
+ *
+ * Experts whose weights are floating-point numbers instead of group-scaled
+ * integers: float8 e4m3 with one f32 scale per block of 128 x 128 weights
+ * (multiplied by rows of e4m3 with one scale per 128 columns), or plain bf16
+ * / f16.  moelan keeps such experts dense (moelan/experts.py:72-122 F32Matrix,
+ * Half16: x @ W.T per expert); the e4m3 form has no counterpart there.  One
+ * layer: mb_router_route, mb_permute, mb_operand_rows (rows = sorted_rows),
+ * mb_grouped_swiglu_t, mb_grouped_matmul_t, mb_unpermute_combine.
+ * None of these entries needs a workspace. */
+
+/* Element types. */
+enum { MB_T_F32 = 0, MB_T_BF16 = 1, MB_T_F16 = 2, MB_T_E4M3 = 3 };
+
+/* Columns (and weight rows) that share one e4m3 scale. */
+#define MB_SCALE_BLOCK 128
+
+/* Rows of x (n_src, d) in the form the products below take (in place of
+ * moelan/experts.py:707-727's x[rows] gather): row p of the result is
+ * x[rows[p]] (x[p] when rows is NULL, which needs n <= n_src), 0 <= p < n.
+ *   type MB_T_BF16 / MB_T_F16: rounded to nearest even; scales unused.
+ *   type MB_T_E4M3: for each group g of 128 columns (the last may be shorter)
+ *     scales[p, g] = max|x| / 448 (1 when that is 0), q = e4m3(x / scale) with
+ *     both divisions and the final rounding to nearest even.  A NaN stays a
+ *     NaN; a group that holds an infinity gets an infinite scale.
+ * x_type: MB_T_F32, MB_T_BF16 or MB_T_F16.  Rows of x and q are ldx / ldq
+ * elements apart; scales[p, g] is at scales[p * s_row + g * s_group].  An
+ * index outside x sets MB_STATUS_BADARG (2) in *status (when not NULL) and its
+ * row becomes zeros with scales 1. */
+int mb_operand_rows(const void *x, int x_type, int64_t ldx, int64_t n_src, const int32_t *rows, int64_t n, int d,
+                    int type, void *q, int64_t ldq, float *scales, int64_t s_row, int64_t s_group, unsigned *status,
+                    void *stream);
+
+/* y[p] = x[p] @ w[e].T for the rows offsets[e] <= p < offsets[e + 1] of each
+ * expert e (ragged; an expert may have no rows), f32 sums, rounded once to
+ * y_type (MB_T_F32, MB_T_BF16 or MB_T_F16).  offsets (E + 1) int32 on the
+ * device, non-decreasing within 0 .. P (else MB_STATUS_BADARG is set and the
+ * offending experts' rows are left); rows of y before offsets[0] and from
+ * offsets[E] on are left as they are.
+ *   x (P, K) and w (E, O, K) of one type: MB_T_E4M3, MB_T_BF16 or MB_T_F16.
+ *   ldx, ldw: elements between rows; w_expert: between experts' matrices.  x,
+ *   w and these distances in bytes must be multiples of 16.  y rows are ldy
+ *   elements apart (no alignment beyond the element's).
+ *   MB_T_E4M3: xs[p, g] at xs[p * xs_row + g * xs_group], ws (E, ceil(O/128),
+ *   ceil(K/128)) contiguous:
+ *     y[p, o] = sum_g xs[p, g] * ws[e, o/128, g] * sum_{k in g} x[p, k] w[e, o, k].
+ * 1 <= E <= 1024, P < 2^31. */
+int mb_grouped_matmul_t(const void *x, int type, int64_t ldx, const float *xs, int64_t xs_row, int64_t xs_group,
+                        int64_t P, const void *w, int64_t w_expert, int64_t ldw, const float *ws, int E, int O, int K,
+                        const int32_t *offsets, void *y, int y_type, int64_t ldy, unsigned *status, void *stream);
+
+/* mb_grouped_matmul_t for gate|up matrices w (E, 2I, K), the I gate rows and
+ * then the I up rows (moelan/experts.py:247-263 Expert), with the activation:
+ *   a[p, j] = g / (1 + exp(-g)) * u,  g = x[p] @ w[e][j], u = x[p] @ w[e][I + j]
+ * in f32, then put into operand form of x's type as mb_operand_rows does: q
+ * (P, I) of `type`, and for MB_T_E4M3 its scales qs[p, g] at
+ * qs[p * qs_row + g * qs_group].  ws (E, 2, ceil(I/128), ceil(K/128)): the gate
+ * rows' blocks and the up rows' blocks, each half with its own grid. */
+int mb_grouped_swiglu_t(const void *x, int type, int64_t ldx, const float *xs, int64_t xs_row, int64_t xs_group,
+                        int64_t P, const void *w, int64_t w_expert, int64_t ldw, const float *ws, int E, int I, int K,
+                        const int32_t *offsets, void *q, int64_t ldq, float *qs, int64_t qs_row, int64_t qs_group,
+                        unsigned *status, void *stream);
+
+/* x @ w.T for one e4m3 matrix w (O, K) with block scales ws (ceil(O/128),
+ * ceil(K/128)) and e4m3 rows x (n, K) with scales xs (beside mb_matmul_t):
+ * mb_grouped_matmul_t of one expert with every row. */
+int mb_matmul_t_e4m3(const void *x, int64_t ldx, const float *xs, int64_t xs_row, int64_t xs_group, int64_t n,
+                     const void *w, int64_t ldw, const float *ws, int O, int K, void *y, int y_type, int64_t ldy,
+                     unsigned *status, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
