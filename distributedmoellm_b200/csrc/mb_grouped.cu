@@ -4,19 +4,58 @@
 //   y[p, o] = sum_g xs[p, g] ws[e, o / 128, g] sum_{k in g} x[p, k] w[e, o, k]
 //
 // with g over groups of 128 columns (one group, scales 1, for 16-bit types).
-// Products of e4m3 values are exact in f32; each group's sum is scaled in f32.
 //
-// One CTA per (row, 128 outputs): the row's group of 128 columns in shared
-// memory, one output per thread.
+// One persistent, warp-specialised kernel on the tcgen05 tensor cores.  The
+// weights are the M = 128 side and the rows of x the N side: an expert's row
+// count is ragged, N goes in steps of 16 and costs in proportion, and a decode
+// step's few rows leave the shared memory to a deep ring of weight tiles.  A
+// work item is (expert, block of 128 weight rows, pass of at most NT rows of
+// x), passes of one block next to each other so that its weights come from HBM
+// once; the gate|up form takes the 128 gate rows and the 128 up rows of the
+// same columns together.
+//  * warp 0: TMA loads (128-byte swizzle, K-major) of 128 bytes of every row
+//    of the weight block and of the pass's rows, into a ring of stages;
+//  * warp 1: tcgen05.mma, f32 accumulators in TMEM.  16-bit types accumulate
+//    over all of K; e4m3 writes each group of 128 columns to a fresh
+//    accumulator, since the group's two scales differ from the next one's;
+//  * warps 2, 3 (e4m3): xs * ws of each row and group into shared memory;
+//  * warps 4..11: the accumulators' columns, 32 at a time and alternating
+//    between two sets of four warps.  e4m3: acc += scale * group sum in f32
+//    registers (packed f32x2 fused multiply-adds), group after group while the
+//    next is multiplied.  Then the results.
+// Splitting K: with few items a cluster's CTAs take equal shares of one item's
+// groups and send their f32 partial sums through distributed shared memory to
+// the first of them, which adds them in rank order, so results do not depend on
+// timing.
+// Every wait is bounded (status word + abort flag).
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "mb_common.cuh"
 #include "mb_float.cuh"
+#include "mb_tc.cuh"
 
 namespace {
+
+constexpr int kBM = 128;                  // weight rows of a tile = TMEM lanes
+constexpr int kThreads = 384;
+constexpr int kThreadWarps = kThreads / 32;
+constexpr int kEpiWarp = 4;               // first of the eight epilogue warps
+constexpr int kEpiWarps = 8;
+constexpr int kTileA = kBM * 128;         // bytes of a weight tile: 128 rows of 128 bytes
+constexpr int kMaxN = 256;                // rows of x per pass (128 for gate|up)
+constexpr int kScSlots = 4;               // scale ring; even: two warps fill it in turn
+constexpr int kMaxAcc = 8;
+constexpr int kMaxStages = 16;
+constexpr int kTmemCols = 512;
+constexpr int kRowMaps = 5;               // boxes of 16, 32, .., 256 rows of x
+constexpr int kMaxSmem = 232448;          // 227 KB
+constexpr int kMaxRed = 64 << 10;         // shared memory for partial sums of a split
+
+__device__ unsigned g_no_status;          // where kernels report when the caller gives no status word
 
 struct GroupedArgs {
     const void* x;
@@ -27,107 +66,559 @@ struct GroupedArgs {
     const void* w;
     int64_t w_expert, ldw;
     const float* ws;
-    int E, O, K;               // O: output rows of w (I for the gate|up form, whose matrices have 2I)
+    int E, O, K;               // O: output columns (gate|up: I, whose matrices have 2I rows)
     const int32_t* offsets;    // null: one expert, all rows
     void* y;
     int64_t ldy;
     float* qs;
     int64_t qs_row, qs_group;
     unsigned* status;
+    int y_type;
+    int Kb;                    // K steps (128 bytes of a row each)
+    int Mb;                    // blocks of 128 output columns
+    int NT;                    // rows of x per pass, at most
+    int stages;
+    int nacc;                  // accumulator slots in TMEM
+    int acc_cols;              // TMEM columns of one half of a slot
+    int vec;                   // e4m3 results may be stored 16 bytes at a time
 };
 
-template <int TYPE>
-__device__ __forceinline__ float load_elem(const void* p, int64_t i)
-{
-    if (TYPE == MB_T_E4M3) {
-        const __half_raw h = __nv_cvt_fp8_to_halfraw(reinterpret_cast<const uint8_t*>(p)[i], __NV_E4M3);
-        return __half2float(__half(h));
-    }
-    if (TYPE == MB_T_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-    return __half2float(reinterpret_cast<const __half*>(p)[i]);
-}
+struct Maps {
+    CUtensorMap w;
+    CUtensorMap x[kRowMaps];
+};
 
-// The rows of expert e, or none where the offsets are not what they may be (reported).
-__device__ __forceinline__ int2 expert_rows(const GroupedArgs& a, int e)
-{
-    if (!a.offsets) return make_int2(0, (int)a.P);
-    const int lo = a.offsets[e], hi = a.offsets[e + 1];
-    if (lo < 0 || hi < lo || hi > a.P) {
-        if (a.status) atomicOr(a.status, MB_STATUS_BADARG);
-        return make_int2(0, 0);
+// The items of this CTA (of its group of `split` CTAs, when items are split over K).
+struct Items {
+    const GroupedArgs& a;
+    const int2* meta;          // (first row, rows) of each expert
+    const int* pstart;         // first item of each expert; [E]: all items
+    int it, step, e, mb, row0, nrows;
+    __device__ Items(const GroupedArgs& args, const int2* m, const int* ps, int first, int by)
+        : a(args), meta(m), pstart(ps), it(first - by), step(by), e(0)
+    {
     }
-    return make_int2(lo, hi);
-}
-
-template <int TYPE, int OUT, bool SWIGLU>
-__global__ void grouped_kernel(const GroupedArgs a)
-{
-    __shared__ float xrow[kScaleBlock];
-    __shared__ float red[4];
-    const int o = blockIdx.x * 128 + threadIdx.x;
-    const int Kb = (a.K + kScaleBlock - 1) / kScaleBlock, Ob = (a.O + kScaleBlock - 1) / kScaleBlock;
-    for (int64_t p = blockIdx.y; p < a.P; p += gridDim.y) {
-        int e = -1;
-        for (int i = 0; i < a.E; ++i) {
-            const int2 r = expert_rows(a, i);
-            if (p >= r.x && p < r.y) {
-                e = i;
-                break;
+    __device__ bool next()
+    {
+        it += step;
+        if (it >= pstart[a.E]) return false;
+        if (it >= pstart[e + 1]) {         // the last e with pstart[e] <= it (experts without rows have none)
+            int lo = e + 1, hi = a.E;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (pstart[mid] <= it)
+                    lo = mid;
+                else
+                    hi = mid;
             }
+            e = lo;
         }
-        if (e < 0) continue;
-        float acc[2] = {0.0f, 0.0f};
-        for (int kb = 0; kb < Kb; ++kb) {
-            const int k0 = kb * kScaleBlock, kn = min(kScaleBlock, a.K - k0);
-            __syncthreads();
-            xrow[threadIdx.x] = (int)threadIdx.x < kn ? load_elem<TYPE>(a.x, p * a.ldx + k0 + threadIdx.x) : 0.0f;
-            __syncthreads();
-            if (o >= a.O) continue;
+        const int2 m = meta[e];
+        const int passes = (m.y + a.NT - 1) / a.NT;
+        const int local = it - pstart[e];
+        mb = local / passes;
+        const int pass = local - mb * passes;
+        const int size = ((m.y + passes - 1) / passes + 15) & ~15;     // passes of about equal size
+        row0 = m.x + pass * size;
+        nrows = min(size, m.y - pass * size);
+        return true;
+    }
+};
+
+__device__ __forceinline__ uint64_t pack2(float lo, float hi)
+{
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b)
+{
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+
+// 32 results of one output column (rows r0 .. r0 + n - 1 of the pass).
+template <typename T>
+__device__ __forceinline__ T round_to(float v);
+template <>
+__device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+
+template <typename T>
+__device__ __forceinline__ void store_column(void* y, int64_t ldy, int64_t row, int col, int n, const float (&v)[32])
+{
+    T* p = reinterpret_cast<T*>(y) + row * ldy + col;
 #pragma unroll
-            for (int h = 0; h < (SWIGLU ? 2 : 1); ++h) {
-                const int64_t row = (int64_t)e * a.w_expert + (int64_t)(h * a.O + o) * a.ldw + k0;
-                float sum = 0.0f;
-                for (int k = 0; k < kn; ++k) sum = fmaf(xrow[k], load_elem<TYPE>(a.w, row + k), sum);
-                if (TYPE == MB_T_E4M3)
-                    sum *= a.xs[p * a.xs_row + kb * a.xs_group] *
-                           a.ws[(((int64_t)e * (SWIGLU ? 2 : 1) + h) * Ob + o / kScaleBlock) * Kb + kb];
-                acc[h] += sum;
+    for (int i = 0; i < 32; ++i)
+        if (i < n) p[i * ldy] = round_to<T>(v[i]);
+}
+
+__device__ __forceinline__ void store_column(int type, void* y, int64_t ldy, int64_t row, int col, int n,
+                                             const float (&v)[32])
+{
+    if (type == MB_T_F32)
+        store_column<float>(y, ldy, row, col, n, v);
+    else if (type == MB_T_BF16)
+        store_column<__nv_bfloat16>(y, ldy, row, col, n, v);
+    else
+        store_column<__half>(y, ldy, row, col, n, v);
+}
+
+// Lane l gets the largest of the 32 lanes' v[l] (31 shuffles; v is used up).
+__device__ __forceinline__ float max_transposed(float (&v)[32], int lane)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const bool hi = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float send = hi ? v[i] : v[i + o], keep = hi ? v[i + o] : v[i];
+            v[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, o));
+        }
+    }
+    return v[0];
+}
+
+template <int TYPE, bool DUAL>
+__global__ void __launch_bounds__(kThreads, 1)
+    grouped_kernel(const __grid_constant__ GroupedArgs a, const __grid_constant__ Maps maps)
+{
+    constexpr bool FP8 = TYPE == MB_T_E4M3;
+    constexpr int KS = FP8 ? 128 : 64;    // columns of a K step
+    constexpr int H = DUAL ? 2 : 1;       // weight tiles of a step
+
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int stage_bytes = H * kTileA + a.NT * 128;
+    const uint32_t csize = cluster_size();
+    uint8_t* stage0 = smem;
+    float* red = reinterpret_cast<float*>(stage0 + (size_t)a.stages * stage_bytes);   // [csize - 1][H][NT][128]
+    float* sc = red + (csize - 1) * H * a.NT * 128;                    // [kScSlots][256] scales
+    float* amax = sc + kScSlots * 256;                                 // [2 sets][2][4 quarters][32]
+    float* tsc = amax + 2 * 2 * 4 * 32;                                // [8 warps][32] scales of a chunk's rows
+    uint8_t* qt = reinterpret_cast<uint8_t*>(tsc + kEpiWarps * 32);    // [2 sets][32 rows][128] e4m3 results
+    uint64_t* bars = reinterpret_cast<uint64_t*>(qt + (FP8 && DUAL ? 2 * 32 * 128 : 0));
+    uint64_t* full = bars;
+    uint64_t* empty = full + kMaxStages;
+    uint64_t* acc_full = empty + kMaxStages;
+    uint64_t* acc_empty = acc_full + kMaxAcc;
+    uint64_t* sc_full = acc_empty + kMaxAcc;
+    uint64_t* sc_empty = sc_full + kScSlots;
+    uint64_t* red_full = sc_empty + kScSlots;
+    uint64_t* red_empty = red_full + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_empty + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [kThreadWarps] + split
+    int2* meta = reinterpret_cast<int2*>(wsum + 16);                   // [E]
+    int* pstart = reinterpret_cast<int*>(meta + a.E);                  // [E + 1]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned* const status = a.status ? a.status : &g_no_status;
+
+    mb_pdl_trigger();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < a.stages; ++i) {
+            mb_mbar_init(&full[i], 1);
+            mb_mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < a.nacc; ++i) {
+            mb_mbar_init(&acc_full[i], 1);
+            mb_mbar_init(&acc_empty[i], kEpiWarps);
+        }
+        for (int i = 0; i < kScSlots; ++i) {
+            mb_mbar_init(&sc_full[i], 1);
+            mb_mbar_init(&sc_empty[i], kEpiWarps);
+        }
+        *abort_flag = 0;
+        tma_prefetch_map(&maps.w);
+    }
+    if (warp == 1) tc_alloc(tmem_slot, kTmemCols);
+    mb_pdl_wait();
+
+    // The experts' rows and the first item of each: an exclusive scan over the experts, a run of them per thread.
+    {
+        const int per = (a.E + kThreads - 1) / kThreads;
+        const int e0 = threadIdx.x * per, e1 = min(a.E, e0 + per);
+        int items = 0;
+        for (int e = e0; e < e1; ++e) {
+            int lo = 0, n = (int)a.P;
+            if (a.offsets) {
+                lo = a.offsets[e];
+                const int hi = a.offsets[e + 1];
+                n = hi - lo;
+                if (lo < 0 || hi < lo || hi > a.P) {
+                    atomicOr(status, MB_STATUS_BADARG);
+                    lo = n = 0;
+                }
+            }
+            meta[e] = make_int2(lo, n);
+            pstart[e] = items;
+            items += a.Mb * ((n + a.NT - 1) / a.NT);
+        }
+        int run = items;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += t;
+        }
+        if (lane == 31) wsum[warp] = run;
+        __syncthreads();
+        int before = run - items, total = 0;
+        for (int w = 0; w < kThreadWarps; ++w) {
+            const int s = wsum[w];
+            if (w < warp) before += s;
+            total += s;
+        }
+        for (int e = e0; e < e1; ++e) pstart[e] += before;
+        if (threadIdx.x == 0) {
+            pstart[a.E] = total;
+            // How many CTAs share an item: the split whose longest CTA has the fewest K steps, two more for each
+            // item that is split (the partial sums' way to the first CTA).
+            int best = 0x7fffffff, split = 1;
+            for (int s = 1; s <= (int)csize && s <= a.Kb; s <<= 1) {
+                const int groups = gridDim.x / s;
+                const int64_t c = (int64_t)((total + groups - 1) / groups) * ((a.Kb + s - 1) / s + (s > 1 ? 2 : 0));
+                if (c < best) {
+                    best = (int)c;
+                    split = s;
+                }
+            }
+            wsum[15] = split;
+            mb_mbar_init(red_full, kEpiWarps * max(split - 1, 1));
+            mb_mbar_init(red_empty, kEpiWarps);
+            mb_fence_mbar_init();
+        }
+    }
+    tc_before();
+    __syncthreads();
+    if (csize > 1) cluster_sync();        // the other CTAs' barriers exist
+    tc_after();
+
+    const uint32_t tmem = *tmem_slot;
+    const int split = wsum[15];
+    const int srank = (int)blockIdx.x % split;                          // rank among the CTAs of an item
+    const int k0 = (int)((int64_t)a.Kb * srank / split), k1 = (int)((int64_t)a.Kb * (srank + 1) / split);
+    const uint32_t leader = cluster_rank() - srank;                     // cluster rank of the item's first CTA
+    Items w(a, meta, pstart, blockIdx.x / split, gridDim.x / split);
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ loads
+        Ring st(a.stages);
+        bool ok = true;
+        int issued = 0;
+        while (ok && w.next()) {
+            const int r16 = (w.nrows + 15) >> 4;
+            // lanes 0, 1: weight tiles; lane 2 + b: a box of 16 << b rows, the larger boxes first
+            const int b = lane - 2;
+            const bool box = b >= 0 && b < kRowMaps && ((r16 >> b) & 1);
+            const int brow = b >= 0 && b < kRowMaps ? ((r16 >> (b + 1)) << (b + 1)) * 16 : 0;
+            for (int kb = k0; kb < k1; ++kb, st.next()) {
+                ok = __all_sync(0xffffffffu, mb_mbar_wait_spin(&empty[st.slot], st.empty_parity(), status, abort_flag));
+                if (!ok) break;
+                uint8_t* dst = stage0 + (size_t)st.slot * stage_bytes;
+                if (lane == 0) mb_mbar_arrive_expect_tx(&full[st.slot], H * kTileA + r16 * 16 * 128);
+                __syncwarp();
+                if (lane < H)
+                    tma_load3(dst + lane * kTileA, &maps.w, kb * KS, lane * a.O + w.mb * kBM, w.e, &full[st.slot]);
+                else if (box)
+                    tma_load2(dst + H * kTileA + brow * 128, &maps.x[b], kb * KS, w.row0 + brow, &full[st.slot]);
+                ++issued;
             }
         }
-        if (!SWIGLU) {
-            if (o < a.O) store_out<OUT>(a.y, p * a.ldy + o, acc[0]);
-            continue;
+        if (!ok) {   // wait (bounded) for the copies still in flight before the CTA may end
+            for (int i = 0; i < min(issued, a.stages); ++i) {
+                if (--st.slot < 0) {
+                    st.slot = a.stages - 1;
+                    st.phase ^= 1;
+                }
+                for (int n = 0; n < 100000 && !mb_mbar_try_wait(&full[st.slot], st.full_parity()); ++n) {
+                }
+            }
         }
-        const float act = o < a.O ? acc[0] / (1.0f + expf(-acc[0])) * acc[1] : 0.0f;
-        if (TYPE != MB_T_E4M3) {
-            if (o < a.O) store_out<OUT>(a.y, p * a.ldy + o, act);
-            continue;
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ tensor cores
+        Ring st(a.stages), ac(a.nacc);
+        bool ok = true;
+        // D f32; A and B both K-major: e4m3 / f16 are format 0, bf16 is 1
+        const uint32_t fmt = TYPE == MB_T_BF16 ? (1u << 7) | (1u << 10) : 0u;
+        while (ok && w.next()) {
+            const int n16 = (w.nrows + 15) & ~15;
+            const uint32_t idesc = (1u << 4) | fmt | ((uint32_t)(n16 >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+            if (!FP8) {
+                ok = __all_sync(0xffffffffu,
+                                mb_mbar_wait_spin(&acc_empty[ac.slot], ac.empty_parity(), status, abort_flag));
+                tc_after();
+            }
+            for (int kb = k0; ok && kb < k1; ++kb, st.next()) {
+                if (FP8)
+                    ok = __all_sync(0xffffffffu,
+                                    mb_mbar_wait_spin(&acc_empty[ac.slot], ac.empty_parity(), status, abort_flag));
+                ok = ok && __all_sync(0xffffffffu,
+                                      mb_mbar_wait_spin(&full[st.slot], st.full_parity(), status, abort_flag));
+                if (!ok) break;
+                tc_after();
+                const uint32_t abase = mb_smem_addr(stage0 + (size_t)st.slot * stage_bytes);
+                const uint32_t bbase = abase + H * kTileA;
+                const uint32_t d = tmem + ac.slot * H * a.acc_cols;
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        tc_mma_ss<FP8>(d + h * a.acc_cols, tc_desc_sw128(abase + h * kTileA + j * 32),
+                                       tc_desc_sw128(bbase + j * 32), idesc, (j > 0 || (!FP8 && kb > k0)) ? 1u : 0u);
+                tc_commit(&empty[st.slot]);
+                if (FP8) {
+                    tc_commit(&acc_full[ac.slot]);
+                    ac.next();
+                }
+            }
+            if (!FP8 && ok) {
+                tc_commit(&acc_full[ac.slot]);
+                ac.next();
+            }
         }
-        float m = fabsf(act);
-        for (int s = 16; s; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-        __syncthreads();
-        const float s = e4m3_scale(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        if (o < a.O) reinterpret_cast<uint8_t*>(a.y)[p * a.ldy + o] = to_e4m3(__fdiv_rn(act, s));
-        if (threadIdx.x == 0) a.qs[p * a.qs_row + blockIdx.x * a.qs_group] = s;
+    } else if (warp < kEpiWarp) {
+        // ------------------------------------------------------------------ scales (steps in turn between two warps)
+        if (FP8) {
+            constexpr int NL = DUAL ? 4 : 8;           // rows of x per lane
+            const int Ob = (a.O + kScaleBlock - 1) / kScaleBlock;
+            const int mine = warp - 2;
+            int g0 = 0;                                // steps of the items before
+            bool ok = true;
+            while (ok && w.next()) {
+                const float* wsp = a.ws + ((int64_t)w.e * H * Ob + w.mb) * a.Kb;
+                const float* xsp = a.xs + (int64_t)w.row0 * a.xs_row;
+                const int first = k0 + ((g0 ^ mine) & 1);
+                float v[NL], v2[NL];
+                auto load = [&](int kb) {
+                    const float s0 = __ldg(wsp + kb);
+                    const float s1 = DUAL ? __ldg(wsp + (int64_t)Ob * a.Kb + kb) : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NL; ++i) {
+                        const int n = lane + 32 * i;
+                        const float x = n < w.nrows ? xsp[(int64_t)n * a.xs_row + kb * a.xs_group] : 0.0f;
+                        v[i] = x * s0;
+                        if (DUAL) v2[i] = x * s1;
+                    }
+                };
+                for (int kb = first; kb < k1; kb += 2) {
+                    const int g = g0 + kb - k0, slot = g % kScSlots;
+                    load(kb);
+                    ok = __all_sync(0xffffffffu, mb_mbar_wait_spin(&sc_empty[slot], ((g / kScSlots) & 1) ^ 1, status,
+                                                                  abort_flag));
+                    if (!ok) break;
+                    float* dst = sc + slot * 256;
+#pragma unroll
+                    for (int i = 0; i < NL; ++i) {
+                        if (32 * i >= w.nrows) break;
+                        dst[lane + 32 * i] = v[i];
+                        if (DUAL) dst[128 + lane + 32 * i] = v2[i];
+                    }
+                    __syncwarp();
+                    if (lane == 0) mb_mbar_arrive(&sc_full[slot]);
+                }
+                g0 += k1 - k0;
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ epilogue
+        const int q = warp & 3, set = (warp - kEpiWarp) >> 2;
+        const int L = 32 * q + lane;                       // row of the weight block
+        const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
+        Ring ac(a.nacc), scr(kScSlots);
+        int sent = 0, abuf = 0;
+        while (w.next()) {
+            const int nch = (w.nrows + 31) >> 5;           // chunks of 32 rows; this set takes set, set + 2, ..
+            const int cols = min(32, a.NT);
+            float acc[4][32];                              // DUAL: gate chunks, then up chunks
+            bool ok = true;
+            if (FP8) {
+                uint64_t sum[4][16];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[i][j] = 0;
+                for (int kb = k0; kb < k1; ++kb) {
+                    ok = mb_mbar_wait_spin(&sc_full[scr.slot], scr.full_parity(), status, abort_flag) &&
+                         mb_mbar_wait_spin(&acc_full[ac.slot], ac.full_parity(), status, abort_flag);
+                    tc_after();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = 2 * (DUAL ? i & 1 : i) + set, h = DUAL ? i >> 1 : 0;
+                        if (c < nch) {
+                            float d[32];
+                            tc_ld32(tl + (ac.slot * H + h) * a.acc_cols + 32 * c, d);
+                            tc_wait_ld();
+                            const float4* s4 = reinterpret_cast<const float4*>(sc + scr.slot * 256 + h * 128 + 32 * c);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const float4 s = s4[j];
+                                fma2(sum[i][2 * j], pack2(d[4 * j], d[4 * j + 1]), pack2(s.x, s.y));
+                                fma2(sum[i][2 * j + 1], pack2(d[4 * j + 2], d[4 * j + 3]), pack2(s.z, s.w));
+                            }
+                        }
+                    }
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mb_mbar_arrive(&acc_empty[ac.slot]);
+                        mb_mbar_arrive(&sc_empty[scr.slot]);
+                    }
+                    ac.next();
+                    scr.next();
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) unpack2(sum[i][j], acc[i][2 * j], acc[i][2 * j + 1]);
+            } else {
+                ok = mb_mbar_wait_spin(&acc_full[ac.slot], ac.full_parity(), status, abort_flag);
+                tc_after();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = 2 * (DUAL ? i & 1 : i) + set, h = DUAL ? i >> 1 : 0;
+                    if (c < nch) tc_ld32(tl + (ac.slot * H + h) * a.acc_cols + 32 * c, acc[i]);
+                }
+                tc_wait_ld();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mb_mbar_arrive(&acc_empty[ac.slot]);
+                ac.next();
+            }
+
+            if (split > 1) {
+                // NT <= 32: chunk 0 only, held by set 0 (gate in acc[0], up in acc[2])
+                const int np = min(cols, (w.nrows + 15) & ~15);
+                if (srank > 0) {
+                    // the receiver has read the previous item's sums (the first wait passes at once)
+                    ok = mbar_wait_cluster(red_empty, (sent & 1) ^ 1, status, abort_flag) && ok;
+                    ++sent;
+                    if (set == 0 && ok) {
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            const uint32_t to =
+                                cluster_map(mb_smem_addr(red + (((srank - 1) * H + h) * a.NT) * 128 + L), leader);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (i < np) cluster_st(to + i * 512, acc[2 * h][i]);
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) cluster_arrive(cluster_map(mb_smem_addr(red_full), leader));
+                    continue;
+                }
+                ok = mbar_wait_cluster(red_full, sent & 1, status, abort_flag) && ok;
+                ++sent;
+                if (set == 0 && ok) {
+                    for (int r = 0; r < split - 1; ++r)
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            const float* from = red + ((r * H + h) * a.NT) * 128 + L;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (i < np) acc[2 * h][i] += from[i * 128];
+                        }
+                }
+                __syncwarp();
+                if (lane == 0)
+                    for (int r = 1; r < split; ++r) cluster_arrive(cluster_map(mb_smem_addr(red_empty), leader + r));
+            }
+
+            const int o = w.mb * kBM + L;
+            const bool live = ok && o < a.O;
+            if constexpr (!DUAL) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = 2 * i + set;
+                    if (c < nch && live)
+                        store_column(a.y_type, a.y, a.ldy, (int64_t)w.row0 + 32 * c, o, w.nrows - 32 * c, acc[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int c = 2 * i + set;
+                    if (c >= nch) break;
+                    const int n = w.nrows - 32 * c;        // rows of this chunk (32 or fewer are real)
+                    const int64_t row = (int64_t)w.row0 + 32 * c;
+                    float(&v)[32] = acc[i];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __fdividef(v[j], 1.0f + __expf(-v[j])) * acc[i + 2][j];
+                    if constexpr (!FP8) {
+                        if (live) store_column(TYPE, a.y, a.ldy, row, o, n, v);
+                    } else {
+                        // e4m3: each row's largest of 128 columns across the set's four warps, then its quotients
+                        float m[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) m[j] = o < a.O ? fabsf(v[j]) : 0.0f;
+                        float* am = amax + ((set * 2 + abuf) * 4) * 32;
+                        abuf ^= 1;
+                        am[q * 32 + lane] = max_transposed(m, lane);
+                        mb_named_barrier(1 + set, 128);
+                        const float s =
+                            e4m3_scale(fmaxf(fmaxf(am[lane], am[32 + lane]), fmaxf(am[64 + lane], am[96 + lane])));
+                        float* ts = tsc + (warp - kEpiWarp) * 32;
+                        ts[lane] = s;
+                        if (q == 0 && lane < n && ok) a.qs[(row + lane) * a.qs_row + w.mb * a.qs_group] = s;
+                        __syncwarp();
+                        uint8_t* tile = qt + set * 32 * 128;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) tile[j * 128 + L] = to_e4m3(__fdiv_rn(v[j], ts[j]));
+                        mb_named_barrier(1 + set, 128);
+                        const int r = (threadIdx.x & 127) >> 2, seg = (threadIdx.x & 3) * 32;
+                        const int left = a.O - w.mb * kBM - seg;
+                        if (r < n && left > 0 && ok) {
+                            uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row + r) * a.ldy + w.mb * kBM + seg;
+                            const uint8_t* src = tile + r * 128 + seg;
+                            if (a.vec && left >= 32) {
+                                reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(src)[0];
+                                reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(src)[1];
+                            } else {
+                                for (int j = 0; j < min(32, left); ++j) dst[j] = src[j];
+                            }
+                        }
+                    }
+                }
+            }
+        }
     }
+
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == 1) tc_dealloc(tmem, kTmemCols);
+    if (csize > 1) cluster_sync();        // no CTA ends while another may still write to it
 }
 
-template <int TYPE, int OUT, bool SWIGLU>
-int launch(const GroupedArgs& a, const char* what, cudaStream_t st)
+// ---- host side -----------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn()
 {
-    const dim3 grid((a.O + 127) / 128, (unsigned)std::min<int64_t>(a.P, 65535));
-    grouped_kernel<TYPE, OUT, SWIGLU><<<grid, 128, 0, st>>>(a);
-    return mb_check_launch(what);
+    static EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
 }
 
-template <int TYPE>
-int run_matmul(const GroupedArgs& a, int y_type, const char* what, cudaStream_t st)
+CUtensorMapDataType map_type(int type)
 {
-    if (y_type == MB_T_F32) return launch<TYPE, MB_T_F32, false>(a, what, st);
-    if (y_type == MB_T_BF16) return launch<TYPE, MB_T_BF16, false>(a, what, st);
-    return launch<TYPE, MB_T_F16, false>(a, what, st);
+    return type == MB_T_E4M3  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+           : type == MB_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
 int elem_bytes(int type) { return type == MB_T_F32 ? 4 : type == MB_T_E4M3 ? 1 : 2; }
@@ -155,15 +646,123 @@ int check_args(const GroupedArgs& a, int type, int halves, const char* what)
     return MB_OK;
 }
 
-int matmul(const GroupedArgs& a, int type, int y_type, const char* what, void* stream)
+
+int make_maps(const GroupedArgs& a, int type, int halves, Maps* m, const char* what)
+{
+    const EncodeTiledFn fn = encode_fn();
+    if (!fn) return mb_fail(MB_ECUDA, "%s: cuTensorMapEncodeTiled unavailable", what);
+    const cuuint64_t b = (cuuint64_t)elem_bytes(type);
+    const cuuint32_t inner = (cuuint32_t)(128 / b), one[3] = {1, 1, 1};
+    const cuuint64_t wd[3] = {(cuuint64_t)a.K, (cuuint64_t)a.O * halves, (cuuint64_t)a.E};
+    const cuuint64_t wst[2] = {(cuuint64_t)a.ldw * b,
+                               (cuuint64_t)(a.E > 1 ? a.w_expert : (int64_t)a.O * halves * a.ldw) * b};
+    const cuuint32_t wbox[3] = {inner, kBM, 1};
+    CUresult r = fn(&m->w, map_type(type), 3, const_cast<void*>(a.w), wd, wst, wbox, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint64_t xd[2] = {(cuuint64_t)a.K, (cuuint64_t)a.P};
+    const cuuint64_t xst[1] = {(cuuint64_t)a.ldx * b};
+    for (int i = 0; i < kRowMaps && (16 << i) <= a.NT && r == CUDA_SUCCESS; ++i) {
+        const cuuint32_t xbox[2] = {inner, (cuuint32_t)(16 << i)};
+        r = fn(&m->x[i], map_type(type), 2, const_cast<void*>(a.x), xd, xst, xbox, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    }
+    if (r != CUDA_SUCCESS) return mb_fail(MB_ECUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+    return MB_OK;
+}
+
+int pow2_at_least(int64_t n, int lo, int hi)
+{
+    int p = lo;
+    while (p < n && p < hi) p <<= 1;
+    return p;
+}
+
+template <int TYPE, bool DUAL>
+int launch(GroupedArgs a, const char* what, cudaStream_t st)
+{
+    constexpr bool FP8 = TYPE == MB_T_E4M3;
+    constexpr int H = DUAL ? 2 : 1;
+    const int sms = mb_num_sms();
+    a.Kb = (a.K + (FP8 ? 127 : 63)) / (FP8 ? 128 : 64);
+    a.Mb = (a.O + kBM - 1) / kBM;
+    const int maxn = DUAL ? kMaxN / 2 : kMaxN;
+    const int64_t active = std::min<int64_t>(a.E, a.P);          // experts with rows, at most
+    if (a.offsets) {
+        a.NT = pow2_at_least((a.P * 3 / 2 + a.E - 1) / a.E, 16, maxn);
+    } else {
+        a.NT = pow2_at_least(a.P, 16, maxn);
+        while (a.NT > 32 && a.Mb * ((a.P + a.NT - 1) / a.NT) < sms) a.NT >>= 1;
+    }
+    const int64_t items = (int64_t)a.Mb * (active + a.P / a.NT);   // an upper bound
+    MB_REQUIRE(items < (1ll << 30), "%s: %lld work items", what, (long long)items);
+    int cluster = 1;
+    if (a.NT <= 32 && a.Mb * active < 4 * sms)
+        while (cluster < 8 && cluster * 2 <= a.Kb && (2 * cluster - 1) * H * a.NT * 512 <= kMaxRed &&
+               a.Mb * active * cluster < 4 * sms)
+            cluster *= 2;
+    a.acc_cols = std::max(32, a.NT);
+    a.nacc = std::min(kMaxAcc, kTmemCols / (H * a.acc_cols));
+    const int stage = H * kTileA + a.NT * 128;
+    const int fixed = 1024 + (cluster - 1) * H * a.NT * 512 + kScSlots * 1024 + 2 * 2 * 4 * 32 * 4 + kEpiWarps * 128 +
+                      (FP8 && DUAL ? 2 * 32 * 128 : 0) + (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2) * 8 + 8 + 64 +
+                      a.E * 8 + (a.E + 1) * 4 + 16;
+    a.stages = std::min(kMaxStages, (kMaxSmem - fixed) / stage);
+    const int smem = fixed + a.stages * stage;
+
+    auto kern = grouped_kernel<TYPE, DUAL>;
+    static thread_local uint64_t ready = 0;                        // devices whose attribute is set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(ready >> (dev & 63) & 1)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+        if (e != cudaSuccess) return mb_fail(MB_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+        ready |= 1ull << (dev & 63);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = kThreads;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    int ctas = sms;
+    if (cluster > 1) {
+        // clusters that fit at the same time: a CTA takes an SM, and a cluster stays within one GPC
+        static thread_local int fits[64][4] = {};
+        int& f = fits[dev & 63][cluster == 2 ? 1 : cluster == 4 ? 2 : 3];
+        if (f == 0) {
+            cfg.gridDim = cluster;
+            int n = 0;
+            const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+            if (e != cudaSuccess) return mb_fail(MB_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+            f = std::max(1, n);
+        }
+        ctas = f * cluster;
+    }
+    cfg.gridDim = (unsigned)std::min<int64_t>(ctas, items * cluster);
+    Maps maps;
+    const int rc = make_maps(a, TYPE, H, &maps, what);
+    if (rc) return rc;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, maps);
+    if (e != cudaSuccess) return mb_fail(MB_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+    return MB_OK;
+}
+
+int matmul(GroupedArgs a, int type, int y_type, const char* what, void* stream)
 {
     MB_REQUIRE(y_type == MB_T_F32 || y_type == MB_T_BF16 || y_type == MB_T_F16, "%s: result type %d", what, y_type);
-    int rc = check_args(a, type, 1, what);
+    const int rc = check_args(a, type, 1, what);
     if (rc || a.P == 0) return rc;
+    a.y_type = y_type;
     const cudaStream_t st = mb_stream(stream);
-    if (type == MB_T_E4M3) return run_matmul<MB_T_E4M3>(a, y_type, what, st);
-    if (type == MB_T_BF16) return run_matmul<MB_T_BF16>(a, y_type, what, st);
-    return run_matmul<MB_T_F16>(a, y_type, what, st);
+    if (type == MB_T_E4M3) return launch<MB_T_E4M3, false>(a, what, st);
+    if (type == MB_T_BF16) return launch<MB_T_BF16, false>(a, what, st);
+    return launch<MB_T_F16, false>(a, what, st);
 }
 
 }  // namespace
@@ -195,13 +794,14 @@ extern "C" int mb_grouped_swiglu_t(const void* x, int type, int64_t ldx, const f
 {
     const char* what = "mb_grouped_swiglu_t";
     MB_REQUIRE(offsets || P == 0, "%s: null pointer", what);
-    const GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K,
-                        offsets, q, ldq, qs, qs_row, qs_group, status};
+    GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K,
+                  offsets, q, ldq, qs, qs_row, qs_group, status};
     int rc = check_args(a, type, 2, what);
     if (rc || P == 0) return rc;
     MB_REQUIRE(type != MB_T_E4M3 || qs, "%s: e4m3 results need their scales", what);
     const cudaStream_t st = mb_stream(stream);
-    if (type == MB_T_E4M3) return launch<MB_T_E4M3, MB_T_F32, true>(a, what, st);
-    if (type == MB_T_BF16) return launch<MB_T_BF16, MB_T_BF16, true>(a, what, st);
-    return launch<MB_T_F16, MB_T_F16, true>(a, what, st);
+    a.vec = ((uintptr_t)q & 15) == 0 && ldq % 16 == 0;
+    if (type == MB_T_E4M3) return launch<MB_T_E4M3, true>(a, what, st);
+    if (type == MB_T_BF16) return launch<MB_T_BF16, true>(a, what, st);
+    return launch<MB_T_F16, true>(a, what, st);
 }
