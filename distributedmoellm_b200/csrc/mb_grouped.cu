@@ -15,14 +15,17 @@
 // same columns together.
 //  * warp 0: TMA loads (128-byte swizzle, K-major) of 128 bytes of every row
 //    of the weight block and of the pass's rows, into a ring of stages;
-//  * warp 1: tcgen05.mma, f32 accumulators in TMEM.  16-bit types accumulate
-//    over all of K; e4m3 writes each group of 128 columns to a fresh
-//    accumulator, since the group's two scales differ from the next one's;
+//  * warp 1: tcgen05.mma, f32 accumulators in TMEM.  e4m3 writes each group of
+//    128 columns to a fresh accumulator, since the group's two scales differ
+//    from the next one's.  16-bit types with 16-bit results accumulate over
+//    all of K; with f32 results they start afresh every 256 columns: the tensor
+//    cores' f32 sums are cut rather than rounded, which over 2048 columns
+//    came to 2.1e-6 of the result (f32 itself: 1e-7);
 //  * warps 2, 3 (e4m3): xs * ws of each row and group into shared memory;
 //  * warps 4..11: the accumulators' columns, 32 at a time and alternating
-//    between two sets of four warps.  e4m3: acc += scale * group sum in f32
-//    registers (packed f32x2 fused multiply-adds), group after group while the
-//    next is multiplied.  Then the results.
+//    between two sets of four warps, added (e4m3: times their scale) to f32
+//    registers (packed f32x2 operations) while the next columns of K are
+//    multiplied.  Then the results.
 // Splitting K: with few items a cluster's CTAs take equal shares of one item's
 // groups and send their f32 partial sums through distributed shared memory to
 // the first of them, which adds them in rank order, so results do not depend on
@@ -48,7 +51,11 @@ constexpr int kEpiWarps = 8;
 constexpr int kTileA = kBM * 128;         // bytes of a weight tile: 128 rows of 128 bytes
 constexpr int kMaxN = 256;                // rows of x per pass (128 for gate|up)
 constexpr int kScSlots = 4;               // scale ring; even: two warps fill it in turn
+constexpr int kRaw = 4;                   // steps each scale warp loads ahead
 constexpr int kMaxAcc = 8;
+// Registers: 168 a thread at launch; the epilogue warpgroups hold up to 128 sums and two tiles of 32 columns a thread
+// and take theirs from the first warpgroup: 128 * 88 + 256 * 208 = 64512 = the launch's 384 * 168.
+constexpr int kLoadRegs = 88, kEpiRegs = 208;
 constexpr int kMaxStages = 16;
 constexpr int kTmemCols = 512;
 constexpr int kRowMaps = 5;               // boxes of 16, 32, .., 256 rows of x
@@ -79,7 +86,8 @@ struct GroupedArgs {
     int NT;                    // rows of x per pass, at most
     int stages;
     int nacc;                  // accumulator slots in TMEM
-    int acc_cols;              // TMEM columns of one half of a slot
+    int acc_cols;              // TMEM columns of one half of a slot; also rows of x in a scale slot
+    int prom;                  // K steps summed in TMEM before their sum is added to the f32 registers
     int vec;                   // e4m3 results may be stored 16 bytes at a time
 };
 
@@ -125,6 +133,34 @@ struct Items {
     }
 };
 
+// The K steps k0 .. k1 - 1 of one item after another.
+struct Steps {
+    Items w;
+    int k0, k1, kb;
+    bool live;
+    __device__ Steps(const Items& items, int first, int last) : w(items), k0(first), k1(last), kb(first)
+    {
+        live = w.next();
+    }
+    __device__ void next()
+    {
+        if (live && ++kb == k1) {
+            live = w.next();
+            kb = k0;
+        }
+    }
+};
+
+// Four bytes to shared memory in the background (zero when !real; src must be valid all the same).
+__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool real)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(mb_smem_addr(dst)), "l"(src), "r"(real ? 4 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 __device__ __forceinline__ uint64_t pack2(float lo, float hi)
 {
     uint64_t v;
@@ -138,6 +174,11 @@ __device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi)
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b)
 {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+
+__device__ __forceinline__ void add2(uint64_t& acc, uint64_t a)
+{
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(a));
 }
 
 // 32 results of one output column (rows r0 .. r0 + n - 1 of the pass).
@@ -185,6 +226,194 @@ __device__ __forceinline__ float max_transposed(float (&v)[32], int lane)
     return v[0];
 }
 
+// What an epilogue warp keeps between items.
+struct Epilogue {
+    const GroupedArgs& a;
+    unsigned* status;
+    volatile int* abort_flag;
+    uint32_t tl;               // TMEM address of the warp's lane quarter
+    uint64_t *acc_full, *acc_empty, *sc_full, *sc_empty;
+    const float* sc;
+    float* red;
+    uint64_t *red_full, *red_empty;
+    float *amax, *tsc;
+    uint8_t* qt;
+    int k0, k1, split, srank;
+    uint32_t leader;
+    Ring ac, scr;
+    int sent, abuf;
+
+    // One item with N chunks of 32 rows for this warp's set (a count known at compile time keeps the sums in
+    // registers: with a test around each chunk a step took 3200 cycles at 256 rows, most of them moves).
+    template <int TYPE, bool DUAL, int N>
+    __device__ __forceinline__ void item(const Items& w)
+    {
+        constexpr bool FP8 = TYPE == MB_T_E4M3;
+        constexpr int H = DUAL ? 2 : 1;
+        constexpr int T = H * N;               // tiles of 32 columns: chunk t / H, half t % H
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        const int q = warp & 3, set = (warp - kEpiWarp) >> 2;
+        const int L = 32 * q + lane;           // row of the weight block
+        const int scw = H * a.acc_cols;
+        bool ok = true;
+        uint64_t sum[T > 0 ? T : 1][16];
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum[t][j] = 0;
+        for (int kb = k0; kb < k1; kb += a.prom) {
+            if (FP8) ok = mb_mbar_wait_spin(&sc_full[scr.slot], scr.full_parity(), status, abort_flag);
+            ok = mb_mbar_wait_spin(&acc_full[ac.slot], ac.full_parity(), status, abort_flag) && ok;
+            tc_after();
+            if constexpr (T > 0) {
+                float d[2][32];                // the next tile is on its way while this one is added
+                const uint32_t from = tl + ac.slot * scw + 32 * set;
+                const float* s0 = sc + scr.slot * scw + 32 * set;
+                tc_ld32(from, d[0]);
+                tc_wait_ld();
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    if (t + 1 < T) tc_ld32(from + ((t + 1) % H) * a.acc_cols + 64 * ((t + 1) / H), d[(t + 1) & 1]);
+                    const float(&v)[32] = d[t & 1];
+                    if (FP8) {
+                        const float4* s4 = reinterpret_cast<const float4*>(s0 + (t % H) * a.acc_cols + 64 * (t / H));
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float4 s = s4[j];
+                            fma2(sum[t][2 * j], pack2(v[4 * j], v[4 * j + 1]), pack2(s.x, s.y));
+                            fma2(sum[t][2 * j + 1], pack2(v[4 * j + 2], v[4 * j + 3]), pack2(s.z, s.w));
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) add2(sum[t][j], pack2(v[2 * j], v[2 * j + 1]));
+                    }
+                    if (t + 1 < T) tc_wait_ld();
+                }
+            }
+            tc_before();
+            __syncwarp();
+            if (lane == 0) {
+                mb_mbar_arrive(&acc_empty[ac.slot]);
+                if (FP8) mb_mbar_arrive(&sc_empty[scr.slot]);
+            }
+            ac.next();
+            if (FP8) scr.next();
+        }
+
+        if (split > 1) {
+            // NT <= 32: one chunk, set 0's
+            const int np = (w.nrows + 15) & ~15;
+            if (srank > 0) {
+                // the receiver has read the previous item's sums (the first wait passes at once)
+                ok = mbar_wait_cluster(red_empty, (sent & 1) ^ 1, status, abort_flag) && ok;
+                ++sent;
+                if constexpr (N == 1) {
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        const uint32_t to =
+                            cluster_map(mb_smem_addr(red + (((srank - 1) * H + h) * a.NT) * 128 + L), leader);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            float lo, hi;
+                            unpack2(sum[h][j], lo, hi);
+                            if (2 * j < np && ok) {
+                                cluster_st(to + 2 * j * 512, lo);
+                                cluster_st(to + (2 * j + 1) * 512, hi);
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) cluster_arrive(cluster_map(mb_smem_addr(red_full), leader));
+                return;
+            }
+            ok = mbar_wait_cluster(red_full, sent & 1, status, abort_flag) && ok;
+            ++sent;
+            if constexpr (N == 1) {
+                for (int r = 0; r < split - 1; ++r)
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        const float* from = red + ((r * H + h) * a.NT) * 128 + L;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (2 * j < np) add2(sum[h][j], pack2(from[2 * j * 128], from[(2 * j + 1) * 128]));
+                    }
+            }
+            __syncwarp();
+            if (lane == 0)
+                for (int r = 1; r < split; ++r) cluster_arrive(cluster_map(mb_smem_addr(red_empty), leader + r));
+        }
+
+        const int o = w.mb * kBM + L;
+        const bool live = ok && o < a.O;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = 2 * i + set;
+            const int n = w.nrows - 32 * c;                // rows of this chunk (32 or fewer are real)
+            const int64_t row = (int64_t)w.row0 + 32 * c;
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) unpack2(sum[H * i][j], v[2 * j], v[2 * j + 1]);
+            if constexpr (!DUAL) {
+                if (live) store_column(a.y_type, a.y, a.ldy, row, o, n, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    float u0, u1;
+                    unpack2(sum[H * i + 1][j], u0, u1);
+                    v[2 * j] = __fdividef(v[2 * j], 1.0f + __expf(-v[2 * j])) * u0;
+                    v[2 * j + 1] = __fdividef(v[2 * j + 1], 1.0f + __expf(-v[2 * j + 1])) * u1;
+                }
+                if constexpr (!FP8) {
+                    if (live) store_column(TYPE, a.y, a.ldy, row, o, n, v);
+                } else {
+                    encode(w, v, row, n, L, q, set, ok);
+                }
+            }
+        }
+    }
+
+    // 32 rows of activations (this thread: column L of the block) as e4m3 with a scale per row: each row's largest of
+    // the 128 columns across the set's four warps, the quotients through shared memory into rows of bytes.
+    __device__ __forceinline__ void encode(const Items& w, const float (&v)[32], int64_t row, int n, int L, int q, int set,
+                                           bool ok)
+    {
+        const int lane = L & 31, o = w.mb * kBM + L;
+        float m[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) m[j] = o < a.O ? fabsf(v[j]) : 0.0f;
+        float* am = amax + ((set * 2 + abuf) * 4) * 32;
+        abuf ^= 1;
+        am[q * 32 + lane] = max_transposed(m, lane);
+        mb_named_barrier(1 + set, 128);
+        const float s = e4m3_scale(fmaxf(fmaxf(am[lane], am[32 + lane]), fmaxf(am[64 + lane], am[96 + lane])));
+        float* ts = tsc + (set * 4 + q) * 32;
+        ts[lane] = s;
+        if (q == 0 && lane < n && ok) a.qs[(row + lane) * a.qs_row + w.mb * a.qs_group] = s;
+        __syncwarp();
+        uint8_t* tile = qt + set * 32 * 128;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) tile[j * 128 + L] = to_e4m3(__fdiv_rn(v[j], ts[j]));
+        mb_named_barrier(1 + set, 128);
+        const int r = L >> 2, seg = (L & 3) * 32, left = a.O - w.mb * kBM - seg;
+        if (r < n && left > 0 && ok) {
+            uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row + r) * a.ldy + w.mb * kBM + seg;
+            const uint8_t* src = tile + r * 128 + seg;
+            if (a.vec && left >= 32) {
+                reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(src)[0];
+                reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(src)[1];
+            } else {
+                for (int j = 0; j < min(32, left); ++j) dst[j] = src[j];
+            }
+        }
+    }
+};
+
+template <int R>
+__device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R>
+__device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+
 template <int TYPE, bool DUAL>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ GroupedArgs a, const __grid_constant__ Maps maps)
@@ -199,8 +428,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t csize = cluster_size();
     uint8_t* stage0 = smem;
     float* red = reinterpret_cast<float*>(stage0 + (size_t)a.stages * stage_bytes);   // [csize - 1][H][NT][128]
-    float* sc = red + (csize - 1) * H * a.NT * 128;                    // [kScSlots][256] scales
-    float* amax = sc + kScSlots * 256;                                 // [2 sets][2][4 quarters][32]
+    const int scw = H * a.acc_cols;
+    float* sc = red + (csize - 1) * H * a.NT * 128;                    // [kScSlots][scw] scales
+    float* raw = sc + (FP8 ? kScSlots * scw : 0);                      // [2 warps][kRaw][acc_cols + 4] xs, then ws
+    float* amax = raw + (FP8 ? 2 * kRaw * (a.acc_cols + 4) : 0);       // [2 sets][2][4 quarters][32]
     float* tsc = amax + 2 * 2 * 4 * 32;                                // [8 warps][32] scales of a chunk's rows
     uint8_t* qt = reinterpret_cast<uint8_t*>(tsc + kEpiWarps * 32);    // [2 sets][32 rows][128] e4m3 results
     uint64_t* bars = reinterpret_cast<uint64_t*>(qt + (FP8 && DUAL ? 2 * 32 * 128 : 0));
@@ -307,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t leader = cluster_rank() - srank;                     // cluster rank of the item's first CTA
     Items w(a, meta, pstart, blockIdx.x / split, gridDim.x / split);
 
+    if (warp < kEpiWarp) setmaxnreg_dec<kLoadRegs>();
     if (warp == 0) {
         // ------------------------------------------------------------------ loads
         Ring st(a.stages);
@@ -350,13 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (ok && w.next()) {
             const int n16 = (w.nrows + 15) & ~15;
             const uint32_t idesc = (1u << 4) | fmt | ((uint32_t)(n16 >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-            if (!FP8) {
-                ok = __all_sync(0xffffffffu,
-                                mb_mbar_wait_spin(&acc_empty[ac.slot], ac.empty_parity(), status, abort_flag));
-                tc_after();
-            }
+            int part = 0;                                  // K steps already in the accumulator
             for (int kb = k0; ok && kb < k1; ++kb, st.next()) {
-                if (FP8)
+                if (part == 0)
                     ok = __all_sync(0xffffffffu,
                                     mb_mbar_wait_spin(&acc_empty[ac.slot], ac.empty_parity(), status, abort_flag));
                 ok = ok && __all_sync(0xffffffffu,
@@ -371,219 +599,89 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         tc_mma_ss<FP8>(d + h * a.acc_cols, tc_desc_sw128(abase + h * kTileA + j * 32),
-                                       tc_desc_sw128(bbase + j * 32), idesc, (j > 0 || (!FP8 && kb > k0)) ? 1u : 0u);
+                                       tc_desc_sw128(bbase + j * 32), idesc, (j > 0 || part > 0) ? 1u : 0u);
                 tc_commit(&empty[st.slot]);
-                if (FP8) {
+                if (++part == a.prom || kb + 1 == k1) {
                     tc_commit(&acc_full[ac.slot]);
                     ac.next();
+                    part = 0;
                 }
-            }
-            if (!FP8 && ok) {
-                tc_commit(&acc_full[ac.slot]);
-                ac.next();
             }
         }
     } else if (warp < kEpiWarp) {
         // ------------------------------------------------------------------ scales (steps in turn between two warps)
         if (FP8) {
-            constexpr int NL = DUAL ? 4 : 8;           // rows of x per lane
+            // Each warp takes every second step, kRaw of them ahead: the scales of a step come from global memory (L2
+            // or HBM) and would otherwise cost their latency at every step.
             const int Ob = (a.O + kScaleBlock - 1) / kScaleBlock;
             const int mine = warp - 2;
-            int g0 = 0;                                // steps of the items before
-            bool ok = true;
-            while (ok && w.next()) {
-                const float* wsp = a.ws + ((int64_t)w.e * H * Ob + w.mb) * a.Kb;
-                const float* xsp = a.xs + (int64_t)w.row0 * a.xs_row;
-                const int first = k0 + ((g0 ^ mine) & 1);
-                float v[NL], v2[NL];
-                auto load = [&](int kb) {
-                    const float s0 = __ldg(wsp + kb);
-                    const float s1 = DUAL ? __ldg(wsp + (int64_t)Ob * a.Kb + kb) : 0.0f;
-#pragma unroll
-                    for (int i = 0; i < NL; ++i) {
-                        const int n = lane + 32 * i;
-                        const float x = n < w.nrows ? xsp[(int64_t)n * a.xs_row + kb * a.xs_group] : 0.0f;
-                        v[i] = x * s0;
-                        if (DUAL) v2[i] = x * s1;
-                    }
-                };
-                for (int kb = first; kb < k1; kb += 2) {
-                    const int g = g0 + kb - k0, slot = g % kScSlots;
-                    load(kb);
-                    ok = __all_sync(0xffffffffu, mb_mbar_wait_spin(&sc_empty[slot], ((g / kScSlots) & 1) ^ 1, status,
-                                                                  abort_flag));
-                    if (!ok) break;
-                    float* dst = sc + slot * 256;
-#pragma unroll
-                    for (int i = 0; i < NL; ++i) {
-                        if (32 * i >= w.nrows) break;
-                        dst[lane + 32 * i] = v[i];
-                        if (DUAL) dst[128 + lane + 32 * i] = v2[i];
-                    }
-                    __syncwarp();
-                    if (lane == 0) mb_mbar_arrive(&sc_full[slot]);
-                }
-                g0 += k1 - k0;
+            Steps is(w, k0, k1), fs(w, k0, k1);            // steps being loaded, steps being finished
+            if (mine) {
+                is.next();
+                fs.next();
             }
+            float* const ring = raw + mine * kRaw * (a.acc_cols + 4);
+            auto load = [&](int slot) {
+                if (is.live) {
+                    float* dst = ring + slot * (a.acc_cols + 4);
+                    const float* src = a.xs + (int64_t)is.w.row0 * a.xs_row + (int64_t)is.kb * a.xs_group;
+                    for (int n = lane; n < a.acc_cols && n - lane < is.w.nrows; n += 32)
+                        cp_async4(dst + n, n < is.w.nrows ? src + (int64_t)n * a.xs_row : src, n < is.w.nrows);
+                    if (lane < H)
+                        cp_async4(dst + a.acc_cols + lane,
+                                  a.ws + (((int64_t)is.w.e * H + lane) * Ob + is.w.mb) * a.Kb + is.kb, true);
+                }
+                cp_async_commit();
+                is.next();
+                is.next();
+            };
+            for (int i = 0; i < kRaw; ++i) load(i);
+            int slot = 0;
+            for (int g = mine; fs.live; g += 2) {
+                cp_async_wait<kRaw - 1>();
+                __syncwarp();
+                const int s = g % kScSlots;
+                if (!__all_sync(0xffffffffu, mb_mbar_wait_spin(&sc_empty[s], ((g / kScSlots) & 1) ^ 1, status,
+                                                              abort_flag)))
+                    break;
+                const float* src = ring + slot * (a.acc_cols + 4);
+                const float w0 = src[a.acc_cols], w1 = DUAL ? src[a.acc_cols + 1] : 0.0f;
+                float* dst = sc + s * scw;
+                for (int n = lane; n < a.acc_cols && n - lane < fs.w.nrows; n += 32) {
+                    const float x = src[n];
+                    dst[n] = x * w0;
+                    if (DUAL) dst[a.acc_cols + n] = x * w1;
+                }
+                __syncwarp();
+                if (lane == 0) mb_mbar_arrive(&sc_full[s]);
+                load(slot);
+                slot = (slot + 1) % kRaw;
+                fs.next();
+                fs.next();
+            }
+            cp_async_wait<0>();
         }
     } else {
         // ------------------------------------------------------------------ epilogue
-        const int q = warp & 3, set = (warp - kEpiWarp) >> 2;
-        const int L = 32 * q + lane;                       // row of the weight block
-        const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
-        Ring ac(a.nacc), scr(kScSlots);
-        int sent = 0, abuf = 0;
+        setmaxnreg_inc<kEpiRegs>();
+        const int set = (warp - kEpiWarp) >> 2;
+        Epilogue ep{a, status, abort_flag, tmem + ((uint32_t)(32 * (warp & 3)) << 16), acc_full, acc_empty,
+                    sc_full, sc_empty, sc, red, red_full, red_empty, amax, tsc, qt, k0, k1, split, srank, leader,
+                    Ring(a.nacc), Ring(kScSlots), 0, 0};
         while (w.next()) {
             const int nch = (w.nrows + 31) >> 5;           // chunks of 32 rows; this set takes set, set + 2, ..
-            const int cols = min(32, a.NT);
-            float acc[4][32];                              // DUAL: gate chunks, then up chunks
-            bool ok = true;
-            if (FP8) {
-                uint64_t sum[4][16];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) sum[i][j] = 0;
-                for (int kb = k0; kb < k1; ++kb) {
-                    ok = mb_mbar_wait_spin(&sc_full[scr.slot], scr.full_parity(), status, abort_flag) &&
-                         mb_mbar_wait_spin(&acc_full[ac.slot], ac.full_parity(), status, abort_flag);
-                    tc_after();
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = 2 * (DUAL ? i & 1 : i) + set, h = DUAL ? i >> 1 : 0;
-                        if (c < nch) {
-                            float d[32];
-                            tc_ld32(tl + (ac.slot * H + h) * a.acc_cols + 32 * c, d);
-                            tc_wait_ld();
-                            const float4* s4 = reinterpret_cast<const float4*>(sc + scr.slot * 256 + h * 128 + 32 * c);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float4 s = s4[j];
-                                fma2(sum[i][2 * j], pack2(d[4 * j], d[4 * j + 1]), pack2(s.x, s.y));
-                                fma2(sum[i][2 * j + 1], pack2(d[4 * j + 2], d[4 * j + 3]), pack2(s.z, s.w));
-                            }
-                        }
-                    }
-                    tc_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mb_mbar_arrive(&acc_empty[ac.slot]);
-                        mb_mbar_arrive(&sc_empty[scr.slot]);
-                    }
-                    ac.next();
-                    scr.next();
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) unpack2(sum[i][j], acc[i][2 * j], acc[i][2 * j + 1]);
-            } else {
-                ok = mb_mbar_wait_spin(&acc_full[ac.slot], ac.full_parity(), status, abort_flag);
-                tc_after();
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = 2 * (DUAL ? i & 1 : i) + set, h = DUAL ? i >> 1 : 0;
-                    if (c < nch) tc_ld32(tl + (ac.slot * H + h) * a.acc_cols + 32 * c, acc[i]);
-                }
-                tc_wait_ld();
-                tc_before();
-                __syncwarp();
-                if (lane == 0) mb_mbar_arrive(&acc_empty[ac.slot]);
-                ac.next();
-            }
-
-            if (split > 1) {
-                // NT <= 32: chunk 0 only, held by set 0 (gate in acc[0], up in acc[2])
-                const int np = min(cols, (w.nrows + 15) & ~15);
-                if (srank > 0) {
-                    // the receiver has read the previous item's sums (the first wait passes at once)
-                    ok = mbar_wait_cluster(red_empty, (sent & 1) ^ 1, status, abort_flag) && ok;
-                    ++sent;
-                    if (set == 0 && ok) {
-#pragma unroll
-                        for (int h = 0; h < H; ++h) {
-                            const uint32_t to =
-                                cluster_map(mb_smem_addr(red + (((srank - 1) * H + h) * a.NT) * 128 + L), leader);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (i < np) cluster_st(to + i * 512, acc[2 * h][i]);
-                        }
-                    }
-                    __syncwarp();
-                    if (lane == 0) cluster_arrive(cluster_map(mb_smem_addr(red_full), leader));
-                    continue;
-                }
-                ok = mbar_wait_cluster(red_full, sent & 1, status, abort_flag) && ok;
-                ++sent;
-                if (set == 0 && ok) {
-                    for (int r = 0; r < split - 1; ++r)
-#pragma unroll
-                        for (int h = 0; h < H; ++h) {
-                            const float* from = red + ((r * H + h) * a.NT) * 128 + L;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (i < np) acc[2 * h][i] += from[i * 128];
-                        }
-                }
-                __syncwarp();
-                if (lane == 0)
-                    for (int r = 1; r < split; ++r) cluster_arrive(cluster_map(mb_smem_addr(red_empty), leader + r));
-            }
-
-            const int o = w.mb * kBM + L;
-            const bool live = ok && o < a.O;
-            if constexpr (!DUAL) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = 2 * i + set;
-                    if (c < nch && live)
-                        store_column(a.y_type, a.y, a.ldy, (int64_t)w.row0 + 32 * c, o, w.nrows - 32 * c, acc[i]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int c = 2 * i + set;
-                    if (c >= nch) break;
-                    const int n = w.nrows - 32 * c;        // rows of this chunk (32 or fewer are real)
-                    const int64_t row = (int64_t)w.row0 + 32 * c;
-                    float(&v)[32] = acc[i];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __fdividef(v[j], 1.0f + __expf(-v[j])) * acc[i + 2][j];
-                    if constexpr (!FP8) {
-                        if (live) store_column(TYPE, a.y, a.ldy, row, o, n, v);
-                    } else {
-                        // e4m3: each row's largest of 128 columns across the set's four warps, then its quotients
-                        float m[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) m[j] = o < a.O ? fabsf(v[j]) : 0.0f;
-                        float* am = amax + ((set * 2 + abuf) * 4) * 32;
-                        abuf ^= 1;
-                        am[q * 32 + lane] = max_transposed(m, lane);
-                        mb_named_barrier(1 + set, 128);
-                        const float s =
-                            e4m3_scale(fmaxf(fmaxf(am[lane], am[32 + lane]), fmaxf(am[64 + lane], am[96 + lane])));
-                        float* ts = tsc + (warp - kEpiWarp) * 32;
-                        ts[lane] = s;
-                        if (q == 0 && lane < n && ok) a.qs[(row + lane) * a.qs_row + w.mb * a.qs_group] = s;
-                        __syncwarp();
-                        uint8_t* tile = qt + set * 32 * 128;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) tile[j * 128 + L] = to_e4m3(__fdiv_rn(v[j], ts[j]));
-                        mb_named_barrier(1 + set, 128);
-                        const int r = (threadIdx.x & 127) >> 2, seg = (threadIdx.x & 3) * 32;
-                        const int left = a.O - w.mb * kBM - seg;
-                        if (r < n && left > 0 && ok) {
-                            uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row + r) * a.ldy + w.mb * kBM + seg;
-                            const uint8_t* src = tile + r * 128 + seg;
-                            if (a.vec && left >= 32) {
-                                reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(src)[0];
-                                reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(src)[1];
-                            } else {
-                                for (int j = 0; j < min(32, left); ++j) dst[j] = src[j];
-                            }
-                        }
-                    }
-                }
+            const int mine = (nch - set + 1) >> 1;
+            if (mine == 0)
+                ep.item<TYPE, DUAL, 0>(w);
+            else if (mine == 1)
+                ep.item<TYPE, DUAL, 1>(w);
+            else if (mine == 2)
+                ep.item<TYPE, DUAL, 2>(w);
+            else if constexpr (!DUAL) {
+                if (mine == 3)
+                    ep.item<TYPE, DUAL, 3>(w);
+                else
+                    ep.item<TYPE, DUAL, 4>(w);
             }
         }
     }
@@ -702,8 +800,10 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
             cluster *= 2;
     a.acc_cols = std::max(32, a.NT);
     a.nacc = std::min(kMaxAcc, kTmemCols / (H * a.acc_cols));
+    a.prom = FP8 ? 1 : !DUAL && a.y_type == MB_T_F32 ? 4 : a.Kb;
     const int stage = H * kTileA + a.NT * 128;
-    const int fixed = 1024 + (cluster - 1) * H * a.NT * 512 + kScSlots * 1024 + 2 * 2 * 4 * 32 * 4 + kEpiWarps * 128 +
+    const int scales = FP8 ? (kScSlots * H * a.acc_cols + 2 * kRaw * (a.acc_cols + 4)) * 4 : 0;
+    const int fixed = 1024 + (cluster - 1) * H * a.NT * 512 + scales + 2 * 2 * 4 * 32 * 4 + kEpiWarps * 128 +
                       (FP8 && DUAL ? 2 * 32 * 128 : 0) + (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2) * 8 + 8 + 64 +
                       a.E * 8 + (a.E + 1) * 4 + 16;
     a.stages = std::min(kMaxStages, (kMaxSmem - fixed) / stage);
