@@ -20,6 +20,29 @@ __device__ __forceinline__ float e4m3_scale(float m)
 // Nearest e4m3 (ties to even).  Saturation matters only where s is subnormal: x / s may then round to above 448.
 __device__ __forceinline__ uint8_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 
+// x / s, correctly rounded, for many x and one s: r = 1 / s correctly rounded, then one correction of x * r by its
+// remainder (Markstein, IBM J. Res. Dev. 34, 1990).  Holds while nothing leaves the normal range, which `fast` says: with
+// |x| <= 449 s only remainders of quotients below 2^-20 can, and those round to e4m3's zero either way.
+struct Quotient {
+    float s, r;
+    bool fast;
+    __device__ __forceinline__ explicit Quotient(float scale)
+        : s(scale), r(1.0f / scale), fast(scale > 0x1p-100f && scale < 0x1p100f)
+    {
+    }
+};
+__device__ __forceinline__ float quotient(float x, float s, float r)
+{
+    const float q = x * r;
+    return fmaf(fmaf(-q, s, x), r, q);
+}
+
+// Nearest e4m3 of two values, as bytes lo, hi.
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi)
+{
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
 // out[i] = v, rounded once (to nearest even) to the type; not e4m3.
 template <int TYPE>
 __device__ __forceinline__ void store_out(void* out, int64_t i, float v)

@@ -21,11 +21,16 @@
 //    all of K; with f32 results they start afresh every 256 columns: the tensor
 //    cores' f32 sums are cut rather than rounded, which over 2048 columns
 //    came to 2.1e-6 of the result (f32 itself: 1e-7);
-//  * warps 2, 3 (e4m3): xs * ws of each row and group into shared memory;
+//  * warps 2, 3 (e4m3): xs * ws of each row and group into shared memory, four
+//    groups at a time;
 //  * warps 4..11: the accumulators' columns, 32 at a time and alternating
-//    between two sets of four warps, added (e4m3: times their scale) to f32
-//    registers (packed f32x2 operations) while the next columns of K are
-//    multiplied.  Then the results.
+//    between two sets of four warps (one set alone for passes of 32 rows or
+//    fewer), added (e4m3: times their scale) to f32 registers (packed f32x2
+//    operations) while the next columns of K are multiplied.  They are read as
+//    16 x 256-bit fragments: a thread then meets 8 rows of x in 32, and needs
+//    8 scales from shared memory where whole TMEM rows need all 32 (at 256 rows
+//    those reads alone took 1024 cycles a step, twice the products).  Results go
+//    through shared memory and leave as whole rows by bulk copies.
 // Splitting K: with few items a cluster's CTAs take equal shares of one item's
 // groups and send their f32 partial sums through distributed shared memory to
 // the first of them, which adds them in rank order, so results do not depend on
@@ -50,8 +55,8 @@ constexpr int kEpiWarp = 4;               // first of the eight epilogue warps
 constexpr int kEpiWarps = 8;
 constexpr int kTileA = kBM * 128;         // bytes of a weight tile: 128 rows of 128 bytes
 constexpr int kMaxN = 256;                // rows of x per pass (128 for gate|up)
-constexpr int kScSlots = 4;               // scale ring; even: two warps fill it in turn
-constexpr int kRaw = 4;                   // steps each scale warp loads ahead
+constexpr int kUnit = 4;                  // K steps whose scales are handed over together
+constexpr int kScSlots = 3;               // ring of such units
 constexpr int kMaxAcc = 8;
 // Registers: 168 a thread at launch; the epilogue warpgroups hold up to 128 sums and two tiles of 32 columns a thread
 // and take theirs from the first warpgroup: 128 * 88 + 256 * 208 = 64512 = the launch's 384 * 168.
@@ -80,7 +85,6 @@ struct GroupedArgs {
     float* qs;
     int64_t qs_row, qs_group;
     unsigned* status;
-    int y_type;
     int Kb;                    // K steps (128 bytes of a row each)
     int Mb;                    // blocks of 128 output columns
     int NT;                    // rows of x per pass, at most
@@ -88,7 +92,7 @@ struct GroupedArgs {
     int nacc;                  // accumulator slots in TMEM
     int acc_cols;              // TMEM columns of one half of a slot; also rows of x in a scale slot
     int prom;                  // K steps summed in TMEM before their sum is added to the f32 registers
-    int vec;                   // e4m3 results may be stored 16 bytes at a time
+    int vec;                   // whole rows of results start on 16-byte boundaries
 };
 
 struct Maps {
@@ -133,33 +137,23 @@ struct Items {
     }
 };
 
-// The K steps k0 .. k1 - 1 of one item after another.
-struct Steps {
+// The K steps k0 .. k1 - 1 of one item after another, kUnit at a time.
+struct Units {
     Items w;
     int k0, k1, kb;
     bool live;
-    __device__ Steps(const Items& items, int first, int last) : w(items), k0(first), k1(last), kb(first)
+    __device__ Units(const Items& items, int first, int last) : w(items), k0(first), k1(last), kb(first)
     {
         live = w.next();
     }
     __device__ void next()
     {
-        if (live && ++kb == k1) {
+        if (live && (kb += kUnit) >= k1) {
             live = w.next();
             kb = k0;
         }
     }
 };
-
-// Four bytes to shared memory in the background (zero when !real; src must be valid all the same).
-__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool real)
-{
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(mb_smem_addr(dst)), "l"(src), "r"(real ? 4 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ uint64_t pack2(float lo, float hi)
 {
@@ -181,50 +175,32 @@ __device__ __forceinline__ void add2(uint64_t& acc, uint64_t a)
     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(a));
 }
 
-// 32 results of one output column (rows r0 .. r0 + n - 1 of the pass).
-template <typename T>
-__device__ __forceinline__ T round_to(float v);
+template <int OUT>
+struct OutOf;
 template <>
-__device__ __forceinline__ float round_to<float>(float v) { return v; }
+struct OutOf<MB_T_F32> {
+    using T = float;
+    static __device__ __forceinline__ T round(float v) { return v; }
+};
 template <>
-__device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+struct OutOf<MB_T_BF16> {
+    using T = __nv_bfloat16;
+    static __device__ __forceinline__ T round(float v) { return __float2bfloat16_rn(v); }
+};
 template <>
-__device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+struct OutOf<MB_T_F16> {
+    using T = __half;
+    static __device__ __forceinline__ T round(float v) { return __float2half_rn(v); }
+};
 
-template <typename T>
-__device__ __forceinline__ void store_column(void* y, int64_t ldy, int64_t row, int col, int n, const float (&v)[32])
-{
-    T* p = reinterpret_cast<T*>(y) + row * ldy + col;
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-        if (i < n) p[i * ldy] = round_to<T>(v[i]);
-}
+// Results of 32 rows wait in shared memory as rows of 128 outputs, f32 ones in two halves of 16 rows.  The distance
+// between rows keeps the fragments' stores (4 rows 2 apart x 8 outputs) on different banks.
+__host__ __device__ constexpr int out_bytes(int out) { return out == MB_T_F32 ? 4 : out == MB_T_E4M3 ? 1 : 2; }
+__host__ __device__ constexpr int tile_rows(int out) { return out == MB_T_F32 ? 16 : 32; }
+__host__ __device__ constexpr int tile_pitch(int out) { return 128 * out_bytes(out) + 16; }
 
-__device__ __forceinline__ void store_column(int type, void* y, int64_t ldy, int64_t row, int col, int n,
-                                             const float (&v)[32])
-{
-    if (type == MB_T_F32)
-        store_column<float>(y, ldy, row, col, n, v);
-    else if (type == MB_T_BF16)
-        store_column<__nv_bfloat16>(y, ldy, row, col, n, v);
-    else
-        store_column<__half>(y, ldy, row, col, n, v);
-}
-
-// Lane l gets the largest of the 32 lanes' v[l] (31 shuffles; v is used up).
-__device__ __forceinline__ float max_transposed(float (&v)[32], int lane)
-{
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const bool hi = lane & o;
-#pragma unroll
-        for (int i = 0; i < o; ++i) {
-            const float send = hi ? v[i] : v[i + o], keep = hi ? v[i + o] : v[i];
-            v[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, o));
-        }
-    }
-    return v[0];
-}
+// Where scale n of 32 lies: a thread reads those of its columns 8 b + 2 i + e (i = lane % 4), b = 0, 1, as one vector.
+__device__ __forceinline__ int scale_pos(int n) { return (n & ~15) + ((n >> 1) & 3) * 4 + ((n >> 3) & 1) * 2 + (n & 1); }
 
 // What an epilogue warp keeps between items.
 struct Epilogue {
@@ -234,26 +210,25 @@ struct Epilogue {
     uint32_t tl;               // TMEM address of the warp's lane quarter
     uint64_t *acc_full, *acc_empty, *sc_full, *sc_empty;
     const float* sc;
-    float* red;
+    uint64_t* red;
     uint64_t *red_full, *red_empty;
     float *amax, *tsc;
-    uint8_t* qt;
+    uint8_t* tile;             // the set's rows of results
     int k0, k1, split, srank;
     uint32_t leader;
+    int q, set, lane;
     Ring ac, scr;
     int sent, abuf;
 
     // One item with N chunks of 32 rows for this warp's set (a count known at compile time keeps the sums in
     // registers: with a test around each chunk a step took 3200 cycles at 256 rows, most of them moves).
-    template <int TYPE, bool DUAL, int N>
+    // sum[t][8 h + 2 b + s]: weight row 32 q + 16 h + 8 s + lane / 4, rows of x 8 b + 2 (lane % 4) + {0, 1} of tile t.
+    template <int TYPE, bool DUAL, int OUT, int N>
     __device__ __forceinline__ void item(const Items& w)
     {
         constexpr bool FP8 = TYPE == MB_T_E4M3;
         constexpr int H = DUAL ? 2 : 1;
         constexpr int T = H * N;               // tiles of 32 columns: chunk t / H, half t % H
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        const int q = warp & 3, set = (warp - kEpiWarp) >> 2;
-        const int L = 32 * q + lane;           // row of the weight block
         const int scw = H * a.acc_cols;
         bool ok = true;
         uint64_t sum[T > 0 ? T : 1][16];
@@ -262,47 +237,53 @@ struct Epilogue {
 #pragma unroll
             for (int j = 0; j < 16; ++j) sum[t][j] = 0;
         for (int kb = k0; kb < k1; kb += a.prom) {
-            if (FP8) ok = mb_mbar_wait_spin(&sc_full[scr.slot], scr.full_parity(), status, abort_flag);
+            const int us = (kb - k0) % kUnit;
+            if (FP8 && us == 0) ok = mb_mbar_wait_spin(&sc_full[scr.slot], scr.full_parity(), status, abort_flag) && ok;
             ok = mb_mbar_wait_spin(&acc_full[ac.slot], ac.full_parity(), status, abort_flag) && ok;
             tc_after();
             if constexpr (T > 0) {
                 float d[2][32];                // the next tile is on its way while this one is added
                 const uint32_t from = tl + ac.slot * scw + 32 * set;
-                const float* s0 = sc + scr.slot * scw + 32 * set;
+                const float* s0 = sc + (scr.slot * kUnit + us) * scw + 32 * set + 4 * (lane & 3);
                 tc_ld32(from, d[0]);
                 tc_wait_ld();
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
                     if (t + 1 < T) tc_ld32(from + ((t + 1) % H) * a.acc_cols + 64 * ((t + 1) / H), d[(t + 1) & 1]);
                     const float(&v)[32] = d[t & 1];
-                    if (FP8) {
-                        const float4* s4 = reinterpret_cast<const float4*>(s0 + (t % H) * a.acc_cols + 64 * (t / H));
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float4 s = s4[j];
-                            fma2(sum[t][2 * j], pack2(v[4 * j], v[4 * j + 1]), pack2(s.x, s.y));
-                            fma2(sum[t][2 * j + 1], pack2(v[4 * j + 2], v[4 * j + 3]), pack2(s.z, s.w));
+                    for (int bp = 0; bp < 2; ++bp) {
+                        float4 s = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                        if (FP8)
+                            s = *reinterpret_cast<const float4*>(s0 + (t % H) * a.acc_cols + 64 * (t / H) + 16 * bp);
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {      // b = 2 bp + r % 2, s = r / 2 % 2, h = r / 4
+                            const int b = 2 * bp + (r & 1), j = 8 * (r >> 2) + 2 * b + ((r >> 1) & 1);
+                            const uint64_t x = pack2(v[2 * j], v[2 * j + 1]);
+                            if (FP8)
+                                fma2(sum[t][j], x, r & 1 ? pack2(s.z, s.w) : pack2(s.x, s.y));
+                            else
+                                add2(sum[t][j], x);
                         }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) add2(sum[t][j], pack2(v[2 * j], v[2 * j + 1]));
                     }
                     if (t + 1 < T) tc_wait_ld();
                 }
             }
             tc_before();
             __syncwarp();
+            const bool unit_done = FP8 && (us == kUnit - 1 || kb + 1 == k1);
             if (lane == 0) {
                 mb_mbar_arrive(&acc_empty[ac.slot]);
-                if (FP8) mb_mbar_arrive(&sc_empty[scr.slot]);
+                if (unit_done) mb_mbar_arrive(&sc_empty[scr.slot]);
             }
             ac.next();
-            if (FP8) scr.next();
+            if (unit_done) scr.next();
         }
 
         if (split > 1) {
-            // NT <= 32: one chunk, set 0's
-            const int np = (w.nrows + 15) & ~15;
+            // NT <= 32: one chunk, one set.  Partial sums: [sender][half][h, b, s][128 threads] pairs.
+            const int np = (w.nrows + 15) & ~15, nb = a.NT / 8;
+            const int me = 32 * q + lane;
             if (srank > 0) {
                 // the receiver has read the previous item's sums (the first wait passes at once)
                 ok = mbar_wait_cluster(red_empty, (sent & 1) ^ 1, status, abort_flag) && ok;
@@ -311,15 +292,11 @@ struct Epilogue {
 #pragma unroll
                     for (int h = 0; h < H; ++h) {
                         const uint32_t to =
-                            cluster_map(mb_smem_addr(red + (((srank - 1) * H + h) * a.NT) * 128 + L), leader);
+                            cluster_map(mb_smem_addr(red + ((srank - 1) * H + h) * 4 * nb * 128 + me), leader);
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            float lo, hi;
-                            unpack2(sum[h][j], lo, hi);
-                            if (2 * j < np && ok) {
-                                cluster_st(to + 2 * j * 512, lo);
-                                cluster_st(to + (2 * j + 1) * 512, hi);
-                            }
+                            const int b = (j >> 1) & 3;
+                            if (8 * b < np && ok) cluster_st(to + (((j >> 3) * nb + b) * 2 + (j & 1)) * 1024, sum[h][j]);
                         }
                     }
                 }
@@ -333,10 +310,12 @@ struct Epilogue {
                 for (int r = 0; r < split - 1; ++r)
 #pragma unroll
                     for (int h = 0; h < H; ++h) {
-                        const float* from = red + ((r * H + h) * a.NT) * 128 + L;
+                        const uint64_t* from = red + (r * H + h) * 4 * nb * 128 + me;
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (2 * j < np) add2(sum[h][j], pack2(from[2 * j * 128], from[(2 * j + 1) * 128]));
+                        for (int j = 0; j < 16; ++j) {
+                            const int b = (j >> 1) & 3;
+                            if (8 * b < np) add2(sum[h][j], from[(((j >> 3) * nb + b) * 2 + (j & 1)) * 128]);
+                        }
                     }
             }
             __syncwarp();
@@ -344,8 +323,6 @@ struct Epilogue {
                 for (int r = 1; r < split; ++r) cluster_arrive(cluster_map(mb_smem_addr(red_empty), leader + r));
         }
 
-        const int o = w.mb * kBM + L;
-        const bool live = ok && o < a.O;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = 2 * i + set;
@@ -354,9 +331,7 @@ struct Epilogue {
             float v[32];
 #pragma unroll
             for (int j = 0; j < 16; ++j) unpack2(sum[H * i][j], v[2 * j], v[2 * j + 1]);
-            if constexpr (!DUAL) {
-                if (live) store_column(a.y_type, a.y, a.ldy, row, o, n, v);
-            } else {
+            if constexpr (DUAL) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     float u0, u1;
@@ -364,48 +339,121 @@ struct Epilogue {
                     v[2 * j] = __fdividef(v[2 * j], 1.0f + __expf(-v[2 * j])) * u0;
                     v[2 * j + 1] = __fdividef(v[2 * j + 1], 1.0f + __expf(-v[2 * j + 1])) * u1;
                 }
-                if constexpr (!FP8) {
-                    if (live) store_column(TYPE, a.y, a.ldy, row, o, n, v);
-                } else {
-                    encode(w, v, row, n, L, q, set, ok);
-                }
             }
+            if constexpr (OUT == MB_T_E4M3)
+                encode(w.mb, v, row, n, ok);
+            else
+                store<OUT>(w.mb, v, row, n, ok);
         }
     }
 
-    // 32 rows of activations (this thread: column L of the block) as e4m3 with a scale per row: each row's largest of
-    // the 128 columns across the set's four warps, the quotients through shared memory into rows of bytes.
-    __device__ __forceinline__ void encode(const Items& w, const float (&v)[32], int64_t row, int n, int L, int q, int set,
-                                           bool ok)
+    // The tile's rows to y, 128 outputs (fewer in the last block) from column 128 mb on: `rows` rows of out bytes each.
+    template <int OUT>
+    __device__ __forceinline__ void send(int mb, int64_t row, int rows, bool ok)
     {
-        const int lane = L & 31, o = w.mb * kBM + L;
-        float m[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) m[j] = o < a.O ? fabsf(v[j]) : 0.0f;
-        float* am = amax + ((set * 2 + abuf) * 4) * 32;
-        abuf ^= 1;
-        am[q * 32 + lane] = max_transposed(m, lane);
+        constexpr int R = tile_rows(OUT), B = out_bytes(OUT), pitch = tile_pitch(OUT);
+        bulk_fence();
         mb_named_barrier(1 + set, 128);
-        const float s = e4m3_scale(fmaxf(fmaxf(am[lane], am[32 + lane]), fmaxf(am[64 + lane], am[96 + lane])));
-        float* ts = tsc + (set * 4 + q) * 32;
-        ts[lane] = s;
-        if (q == 0 && lane < n && ok) a.qs[(row + lane) * a.qs_row + w.mb * a.qs_group] = s;
-        __syncwarp();
-        uint8_t* tile = qt + set * 32 * 128;
+        const int me = 32 * q + lane, bytes = min(kBM, a.O - mb * kBM) * B;
+        uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row * a.ldy + (int64_t)mb * kBM) * B;
+        if (a.vec && bytes % 16 == 0) {
+            const int r = me / (128 / R);
+            if (me % (128 / R) == 0 && r < rows && ok)
+                bulk_s2g(dst + r * a.ldy * B, tile + r * pitch, bytes);
+            bulk_commit();
+        } else if (ok) {
+            for (int r = q; r < min(rows, R); r += 4)
+                for (int i = lane; i < bytes / B; i += 32)
+                    if (B == 4)
+                        reinterpret_cast<uint32_t*>(dst + r * a.ldy * B)[i] = reinterpret_cast<uint32_t*>(tile + r * pitch)[i];
+                    else if (B == 2)
+                        reinterpret_cast<uint16_t*>(dst + r * a.ldy * B)[i] = reinterpret_cast<uint16_t*>(tile + r * pitch)[i];
+                    else
+                        (dst + r * a.ldy)[i] = (tile + r * pitch)[i];
+        }
+    }
+
+    // 32 rows of results (this thread's fragment of them), rounded to the output type.
+    template <int OUT>
+    __device__ __forceinline__ void store(int mb, const float (&v)[32], int64_t row, int n, bool ok)
+    {
+        constexpr int R = tile_rows(OUT), pitch = tile_pitch(OUT);
+        using O = OutOf<OUT>;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) tile[j * 128 + L] = to_e4m3(__fdiv_rn(v[j], ts[j]));
-        mb_named_barrier(1 + set, 128);
-        const int r = L >> 2, seg = (L & 3) * 32, left = a.O - w.mb * kBM - seg;
-        if (r < n && left > 0 && ok) {
-            uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row + r) * a.ldy + w.mb * kBM + seg;
-            const uint8_t* src = tile + r * 128 + seg;
-            if (a.vec && left >= 32) {
-                reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(src)[0];
-                reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(src)[1];
-            } else {
-                for (int j = 0; j < min(32, left); ++j) dst[j] = src[j];
+        for (int p = 0; p < 32 / R; ++p) {
+            if (p * R >= n) break;
+            bulk_wait_read();
+            mb_named_barrier(1 + set, 128);                // the tile's last rows have left
+            uint8_t* to = tile + 2 * (lane & 3) * pitch + (32 * q + (lane >> 2)) * out_bytes(OUT);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int b = (j >> 1) & 3, w = 16 * (j >> 3) + 8 * (j & 1);
+                if (8 * b / R == p) {
+                    typename O::T* d = reinterpret_cast<typename O::T*>(to + (8 * b - p * R) * pitch) + w;
+                    d[0] = O::round(v[2 * j]);
+                    d[pitch / out_bytes(OUT)] = O::round(v[2 * j + 1]);
+                }
+            }
+            send<OUT>(mb, row + p * R, n - p * R, ok);
+        }
+    }
+
+    // 32 rows of results as e4m3 with a scale per row: each row's largest of the block's 128 columns (over a thread's
+    // four, the eight lanes that share its rows, and the set's four warps), then the quotients.
+    __device__ __forceinline__ void encode(int mb, const float (&v)[32], int64_t row, int n, bool ok)
+    {
+        constexpr int pitch = tile_pitch(MB_T_E4M3);
+        const int o = mb * kBM + 32 * q + (lane >> 2);
+        float m[8];                                        // index 2 b + e
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int b = (j >> 1) & 3;
+            if (o + 16 * (j >> 3) + 8 * (j & 1) < a.O) {
+                m[2 * b] = fmaxf(m[2 * b], fabsf(v[2 * j]));
+                m[2 * b + 1] = fmaxf(m[2 * b + 1], fabsf(v[2 * j + 1]));
             }
         }
+#pragma unroll
+        for (int s = 16, h = 4; s >= 4; s >>= 1, h >>= 1) {
+            const bool hi = lane & s;
+#pragma unroll
+            for (int i = 0; i < h; ++i) {
+                const float send = hi ? m[i] : m[i + h], keep = hi ? m[i + h] : m[i];
+                m[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, s));
+            }
+        }
+        // this lane now has index lane / 4
+        float* am = amax + ((set * 2 + abuf) * 4) * 32;
+        abuf ^= 1;
+        am[q * 32 + 8 * (lane >> 3) + 2 * (lane & 3) + ((lane >> 2) & 1)] = m[0];
+        bulk_wait_read();
+        mb_named_barrier(1 + set, 128);                    // also: the tile's last rows have left
+        const Quotient qu(e4m3_scale(fmaxf(fmaxf(am[lane], am[32 + lane]), fmaxf(am[64 + lane], am[96 + lane]))));
+        const bool fast = __all_sync(0xffffffffu, qu.fast);
+        float* ts = tsc + (set * 4 + q) * 64;
+        ts[lane] = qu.s;
+        ts[32 + lane] = qu.r;
+        if (q == 0 && lane < n && ok) a.qs[(row + lane) * a.qs_row + mb * a.qs_group] = qu.s;
+        __syncwarp();
+        uint8_t* to = tile + 2 * (lane & 3) * pitch + 32 * q + (lane >> 2);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float2 s = *reinterpret_cast<const float2*>(ts + 8 * b + 2 * (lane & 3));
+            const float2 r = *reinterpret_cast<const float2*>(ts + 32 + 8 * b + 2 * (lane & 3));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = 8 * (i >> 1) + 2 * b + (i & 1);
+                const float x0 = v[2 * j], x1 = v[2 * j + 1];
+                const uint32_t e = fast ? to_e4m3x2(quotient(x0, s.x, r.x), quotient(x1, s.y, r.y))
+                                        : to_e4m3x2(__fdiv_rn(x0, s.x), __fdiv_rn(x1, s.y));
+                uint8_t* d = to + 8 * b * pitch + 16 * (i >> 1) + 8 * (i & 1);
+                d[0] = (uint8_t)e;
+                d[pitch] = (uint8_t)(e >> 8);
+            }
+        }
+        send<MB_T_E4M3>(mb, row, n, ok);
     }
 };
 
@@ -414,7 +462,8 @@ __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.
 template <int R>
 __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
-template <int TYPE, bool DUAL>
+// OUT: the result type (gate|up: TYPE)
+template <int TYPE, bool DUAL, int OUT>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ GroupedArgs a, const __grid_constant__ Maps maps)
 {
@@ -427,14 +476,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int stage_bytes = H * kTileA + a.NT * 128;
     const uint32_t csize = cluster_size();
     uint8_t* stage0 = smem;
-    float* red = reinterpret_cast<float*>(stage0 + (size_t)a.stages * stage_bytes);   // [csize - 1][H][NT][128]
+    const int sets = a.NT > 32 ? 2 : 1;   // passes of 32 rows or fewer have one chunk: one set of epilogue warps
     const int scw = H * a.acc_cols;
-    float* sc = red + (csize - 1) * H * a.NT * 128;                    // [kScSlots][scw] scales
-    float* raw = sc + (FP8 ? kScSlots * scw : 0);                      // [2 warps][kRaw][acc_cols + 4] xs, then ws
-    float* amax = raw + (FP8 ? 2 * kRaw * (a.acc_cols + 4) : 0);       // [2 sets][2][4 quarters][32]
-    float* tsc = amax + 2 * 2 * 4 * 32;                                // [8 warps][32] scales of a chunk's rows
-    uint8_t* qt = reinterpret_cast<uint8_t*>(tsc + kEpiWarps * 32);    // [2 sets][32 rows][128] e4m3 results
-    uint64_t* bars = reinterpret_cast<uint64_t*>(qt + (FP8 && DUAL ? 2 * 32 * 128 : 0));
+    uint64_t* red = reinterpret_cast<uint64_t*>(stage0 + (size_t)a.stages * stage_bytes);   // [csize - 1][H][NT / 2][128]
+    float* sc = reinterpret_cast<float*>(red + (csize - 1) * H * a.NT * 64);                // [kScSlots][kUnit][scw]
+    float* amax = sc + (FP8 ? kScSlots * kUnit * scw : 0);             // [2 sets][2][4 quarters][32]
+    float* tsc = amax + (OUT == MB_T_E4M3 ? 2 * 2 * 4 * 32 : 0);       // [8 warps][scale, 1 / scale][32]
+    uint8_t* tiles = reinterpret_cast<uint8_t*>(tsc + (OUT == MB_T_E4M3 ? kEpiWarps * 64 : 0));   // [sets][rows][pitch]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + sets * tile_rows(OUT) * tile_pitch(OUT));
     uint64_t* full = bars;
     uint64_t* empty = full + kMaxStages;
     uint64_t* acc_full = empty + kMaxStages;
@@ -460,11 +509,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < a.nacc; ++i) {
             mb_mbar_init(&acc_full[i], 1);
-            mb_mbar_init(&acc_empty[i], kEpiWarps);
+            mb_mbar_init(&acc_empty[i], 4 * sets);
         }
         for (int i = 0; i < kScSlots; ++i) {
             mb_mbar_init(&sc_full[i], 1);
-            mb_mbar_init(&sc_empty[i], kEpiWarps);
+            mb_mbar_init(&sc_empty[i], 4 * sets);
         }
         *abort_flag = 0;
         tma_prefetch_map(&maps.w);
@@ -521,8 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             wsum[15] = split;
-            mb_mbar_init(red_full, kEpiWarps * max(split - 1, 1));
-            mb_mbar_init(red_empty, kEpiWarps);
+            mb_mbar_init(red_full, 4 * max(split - 1, 1));  // a split needs NT <= 32: one set
+            mb_mbar_init(red_empty, 4);
             mb_fence_mbar_init();
         }
     }
@@ -575,114 +624,116 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------ tensor cores
-        Ring st(a.stages), ac(a.nacc);
-        bool ok = true;
-        // D f32; A and B both K-major: e4m3 / f16 are format 0, bf16 is 1
-        const uint32_t fmt = TYPE == MB_T_BF16 ? (1u << 7) | (1u << 10) : 0u;
-        while (ok && w.next()) {
-            const int n16 = (w.nrows + 15) & ~15;
-            const uint32_t idesc = (1u << 4) | fmt | ((uint32_t)(n16 >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-            int part = 0;                                  // K steps already in the accumulator
-            for (int kb = k0; ok && kb < k1; ++kb, st.next()) {
-                if (part == 0)
-                    ok = __all_sync(0xffffffffu,
-                                    mb_mbar_wait_spin(&acc_empty[ac.slot], ac.empty_parity(), status, abort_flag));
-                ok = ok && __all_sync(0xffffffffu,
-                                      mb_mbar_wait_spin(&full[st.slot], st.full_parity(), status, abort_flag));
-                if (!ok) break;
-                tc_after();
-                const uint32_t abase = mb_smem_addr(stage0 + (size_t)st.slot * stage_bytes);
-                const uint32_t bbase = abase + H * kTileA;
-                const uint32_t d = tmem + ac.slot * H * a.acc_cols;
+        if (elect_one()) {
+            Ring st(a.stages), ac(a.nacc);
+            bool ok = true;
+            // D f32; A and B both K-major: e4m3 / f16 are format 0, bf16 is 1
+            const uint32_t fmt = TYPE == MB_T_BF16 ? (1u << 7) | (1u << 10) : 0u;
+            const uint64_t desc0 = tc_desc_sw128(mb_smem_addr(stage0));
+            while (ok && w.next()) {
+                const int n16 = (w.nrows + 15) & ~15;
+                const uint32_t idesc = (1u << 4) | fmt | ((uint32_t)(n16 >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+                int part = 0;                              // K steps already in the accumulator
+                for (int kb = k0; kb < k1; ++kb, st.next()) {
+                    if (part == 0)
+                        ok = mb_mbar_wait_spin(&acc_empty[ac.slot], ac.empty_parity(), status, abort_flag);
+                    ok = ok && mb_mbar_wait_spin(&full[st.slot], st.full_parity(), status, abort_flag);
+                    if (!ok) break;
+                    tc_after();
+                    const uint64_t da = desc0 + (uint64_t)((st.slot * stage_bytes) >> 4);
+                    const uint64_t db = da + (H * kTileA >> 4);
+                    const uint32_t d = tmem + ac.slot * scw;
 #pragma unroll
-                for (int h = 0; h < H; ++h)
+                    for (int h = 0; h < H; ++h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        tc_mma_ss<FP8>(d + h * a.acc_cols, tc_desc_sw128(abase + h * kTileA + j * 32),
-                                       tc_desc_sw128(bbase + j * 32), idesc, (j > 0 || part > 0) ? 1u : 0u);
-                tc_commit(&empty[st.slot]);
-                if (++part == a.prom || kb + 1 == k1) {
-                    tc_commit(&acc_full[ac.slot]);
-                    ac.next();
-                    part = 0;
+                        for (int j = 0; j < 4; ++j)
+                            tc_mma_ss<FP8>(d + h * a.acc_cols, da + (h * kTileA >> 4) + 2 * j, db + 2 * j, idesc,
+                                           (j > 0 || part > 0) ? 1u : 0u);
+                    tc_commit(&empty[st.slot]);
+                    if (++part == a.prom || kb + 1 == k1) {
+                        tc_commit(&acc_full[ac.slot]);
+                        ac.next();
+                        part = 0;
+                    }
                 }
             }
         }
+        __syncwarp();
     } else if (warp < kEpiWarp) {
         // ------------------------------------------------------------------ scales (steps in turn between two warps)
         if (FP8) {
-            // Each warp takes every second step, kRaw of them ahead: the scales of a step come from global memory (L2
-            // or HBM) and would otherwise cost their latency at every step.
+            // Each warp takes every second unit.  A lane loads kUnit groups of its rows at once: the scales come from L2 or
+            // HBM, and four groups share that latency and the hand-over.
+            constexpr int NL = DUAL ? 4 : 8;               // rows per lane
             const int Ob = (a.O + kScaleBlock - 1) / kScaleBlock;
-            const int mine = warp - 2;
-            Steps is(w, k0, k1), fs(w, k0, k1);            // steps being loaded, steps being finished
-            if (mine) {
-                is.next();
-                fs.next();
-            }
-            float* const ring = raw + mine * kRaw * (a.acc_cols + 4);
-            auto load = [&](int slot) {
-                if (is.live) {
-                    float* dst = ring + slot * (a.acc_cols + 4);
-                    const float* src = a.xs + (int64_t)is.w.row0 * a.xs_row + (int64_t)is.kb * a.xs_group;
-                    for (int n = lane; n < a.acc_cols && n - lane < is.w.nrows; n += 32)
-                        cp_async4(dst + n, n < is.w.nrows ? src + (int64_t)n * a.xs_row : src, n < is.w.nrows);
-                    if (lane < H)
-                        cp_async4(dst + a.acc_cols + lane,
-                                  a.ws + (((int64_t)is.w.e * H + lane) * Ob + is.w.mb) * a.Kb + is.kb, true);
+            Units un(w, k0, k1);
+            if (warp == 3) un.next();
+            Ring slot(kScSlots);
+            if (warp == 3) slot.next();
+            while (un.live) {
+                const int m = min(kUnit, k1 - un.kb);
+                const float* wsp = a.ws + ((int64_t)un.w.e * H * Ob + un.w.mb) * a.Kb + un.kb;
+                const float* xsp = a.xs + ((int64_t)un.w.row0 + lane) * a.xs_row + (int64_t)un.kb * a.xs_group;
+                float v[NL][kUnit], w0[kUnit], w1[kUnit];
+#pragma unroll
+                for (int s = 0; s < kUnit; ++s) {
+                    w0[s] = s < m ? wsp[s] : 0.0f;
+                    if (DUAL) w1[s] = s < m ? wsp[(int64_t)Ob * a.Kb + s] : 0.0f;
                 }
-                cp_async_commit();
-                is.next();
-                is.next();
-            };
-            for (int i = 0; i < kRaw; ++i) load(i);
-            int slot = 0;
-            for (int g = mine; fs.live; g += 2) {
-                cp_async_wait<kRaw - 1>();
-                __syncwarp();
-                const int s = g % kScSlots;
-                if (!__all_sync(0xffffffffu, mb_mbar_wait_spin(&sc_empty[s], ((g / kScSlots) & 1) ^ 1, status,
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    const bool real = lane + 32 * i < un.w.nrows;
+#pragma unroll
+                    for (int s = 0; s < kUnit; ++s)
+                        v[i][s] = real && s < m ? xsp[(int64_t)(32 * i) * a.xs_row + s * a.xs_group] : 0.0f;
+                }
+                if (!__all_sync(0xffffffffu, mb_mbar_wait_spin(&sc_empty[slot.slot], slot.empty_parity(), status,
                                                               abort_flag)))
                     break;
-                const float* src = ring + slot * (a.acc_cols + 4);
-                const float w0 = src[a.acc_cols], w1 = DUAL ? src[a.acc_cols + 1] : 0.0f;
-                float* dst = sc + s * scw;
-                for (int n = lane; n < a.acc_cols && n - lane < fs.w.nrows; n += 32) {
-                    const float x = src[n];
-                    dst[n] = x * w0;
-                    if (DUAL) dst[a.acc_cols + n] = x * w1;
+                float* dst = sc + slot.slot * kUnit * scw + scale_pos(lane);
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    if (32 * i >= un.w.nrows) break;
+#pragma unroll
+                    for (int s = 0; s < kUnit; ++s) {
+                        dst[s * scw + 32 * i] = v[i][s] * w0[s];
+                        if (DUAL) dst[s * scw + a.acc_cols + 32 * i] = v[i][s] * w1[s];
+                    }
                 }
                 __syncwarp();
-                if (lane == 0) mb_mbar_arrive(&sc_full[s]);
-                load(slot);
-                slot = (slot + 1) % kRaw;
-                fs.next();
-                fs.next();
+                if (lane == 0) mb_mbar_arrive(&sc_full[slot.slot]);
+                un.next();
+                un.next();
+                slot.next();
+                slot.next();
             }
-            cp_async_wait<0>();
         }
     } else {
         // ------------------------------------------------------------------ epilogue
         setmaxnreg_inc<kEpiRegs>();
         const int set = (warp - kEpiWarp) >> 2;
-        Epilogue ep{a, status, abort_flag, tmem + ((uint32_t)(32 * (warp & 3)) << 16), acc_full, acc_empty,
-                    sc_full, sc_empty, sc, red, red_full, red_empty, amax, tsc, qt, k0, k1, split, srank, leader,
-                    Ring(a.nacc), Ring(kScSlots), 0, 0};
-        while (w.next()) {
-            const int nch = (w.nrows + 31) >> 5;           // chunks of 32 rows; this set takes set, set + 2, ..
-            const int mine = (nch - set + 1) >> 1;
-            if (mine == 0)
-                ep.item<TYPE, DUAL, 0>(w);
-            else if (mine == 1)
-                ep.item<TYPE, DUAL, 1>(w);
-            else if (mine == 2)
-                ep.item<TYPE, DUAL, 2>(w);
-            else if constexpr (!DUAL) {
-                if (mine == 3)
-                    ep.item<TYPE, DUAL, 3>(w);
-                else
-                    ep.item<TYPE, DUAL, 4>(w);
+        if (set < sets) {
+            Epilogue ep{a, status, abort_flag, tmem + ((uint32_t)(32 * (warp & 3)) << 16), acc_full, acc_empty,
+                        sc_full, sc_empty, sc, red, red_full, red_empty, amax, tsc,
+                        tiles + set * tile_rows(OUT) * tile_pitch(OUT), k0, k1, split, srank, leader,
+                        warp & 3, set, lane, Ring(a.nacc), Ring(kScSlots), 0, 0};
+            while (w.next()) {
+                const int nch = (w.nrows + 31) >> 5;       // chunks of 32 rows; this set takes set, set + 2, ..
+                const int mine = (nch - set + 1) >> 1;
+                if (mine == 0)
+                    ep.item<TYPE, DUAL, OUT, 0>(w);
+                else if (mine == 1)
+                    ep.item<TYPE, DUAL, OUT, 1>(w);
+                else if (mine == 2)
+                    ep.item<TYPE, DUAL, OUT, 2>(w);
+                else if constexpr (!DUAL) {
+                    if (mine == 3)
+                        ep.item<TYPE, DUAL, OUT, 3>(w);
+                    else
+                        ep.item<TYPE, DUAL, OUT, 4>(w);
+                }
             }
+            bulk_wait();
         }
     }
 
@@ -775,7 +826,7 @@ int pow2_at_least(int64_t n, int lo, int hi)
     return p;
 }
 
-template <int TYPE, bool DUAL>
+template <int TYPE, bool DUAL, int OUT>
 int launch(GroupedArgs a, const char* what, cudaStream_t st)
 {
     constexpr bool FP8 = TYPE == MB_T_E4M3;
@@ -800,16 +851,18 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
             cluster *= 2;
     a.acc_cols = std::max(32, a.NT);
     a.nacc = std::min(kMaxAcc, kTmemCols / (H * a.acc_cols));
-    a.prom = FP8 ? 1 : !DUAL && a.y_type == MB_T_F32 ? 4 : a.Kb;
+    a.prom = FP8 ? 1 : OUT == MB_T_F32 ? 4 : a.Kb;
+    a.vec = ((uintptr_t)a.y & 15) == 0 && a.ldy * out_bytes(OUT) % 16 == 0;
     const int stage = H * kTileA + a.NT * 128;
-    const int scales = FP8 ? (kScSlots * H * a.acc_cols + 2 * kRaw * (a.acc_cols + 4)) * 4 : 0;
-    const int fixed = 1024 + (cluster - 1) * H * a.NT * 512 + scales + 2 * 2 * 4 * 32 * 4 + kEpiWarps * 128 +
-                      (FP8 && DUAL ? 2 * 32 * 128 : 0) + (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2) * 8 + 8 + 64 +
-                      a.E * 8 + (a.E + 1) * 4 + 16;
+    const int scales = FP8 ? kScSlots * kUnit * H * a.acc_cols * 4 : 0;
+    const int encode = OUT == MB_T_E4M3 ? 2 * 2 * 4 * 32 * 4 + kEpiWarps * 64 * 4 : 0;
+    const int tiles = (a.NT > 32 ? 2 : 1) * tile_rows(OUT) * tile_pitch(OUT);
+    const int fixed = 1024 + (cluster - 1) * H * a.NT * 512 + scales + encode + tiles +
+                      (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2) * 8 + 8 + 64 + a.E * 8 + (a.E + 1) * 4 + 16;
     a.stages = std::min(kMaxStages, (kMaxSmem - fixed) / stage);
     const int smem = fixed + a.stages * stage;
 
-    auto kern = grouped_kernel<TYPE, DUAL>;
+    auto kern = grouped_kernel<TYPE, DUAL, OUT>;
     static thread_local uint64_t ready = 0;                        // devices whose attribute is set
     int dev = 0;
     cudaGetDevice(&dev);
@@ -853,16 +906,23 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     return MB_OK;
 }
 
+template <int TYPE>
+int launch_as(const GroupedArgs& a, int y_type, const char* what, cudaStream_t st)
+{
+    if (y_type == MB_T_F32) return launch<TYPE, false, MB_T_F32>(a, what, st);
+    if (y_type == MB_T_BF16) return launch<TYPE, false, MB_T_BF16>(a, what, st);
+    return launch<TYPE, false, MB_T_F16>(a, what, st);
+}
+
 int matmul(GroupedArgs a, int type, int y_type, const char* what, void* stream)
 {
     MB_REQUIRE(y_type == MB_T_F32 || y_type == MB_T_BF16 || y_type == MB_T_F16, "%s: result type %d", what, y_type);
     const int rc = check_args(a, type, 1, what);
     if (rc || a.P == 0) return rc;
-    a.y_type = y_type;
     const cudaStream_t st = mb_stream(stream);
-    if (type == MB_T_E4M3) return launch<MB_T_E4M3, false>(a, what, st);
-    if (type == MB_T_BF16) return launch<MB_T_BF16, false>(a, what, st);
-    return launch<MB_T_F16, false>(a, what, st);
+    if (type == MB_T_E4M3) return launch_as<MB_T_E4M3>(a, y_type, what, st);
+    if (type == MB_T_BF16) return launch_as<MB_T_BF16>(a, y_type, what, st);
+    return launch_as<MB_T_F16>(a, y_type, what, st);
 }
 
 }  // namespace
@@ -894,14 +954,13 @@ extern "C" int mb_grouped_swiglu_t(const void* x, int type, int64_t ldx, const f
 {
     const char* what = "mb_grouped_swiglu_t";
     MB_REQUIRE(offsets || P == 0, "%s: null pointer", what);
-    GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K,
-                  offsets, q, ldq, qs, qs_row, qs_group, status};
+    const GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K,
+                        offsets, q, ldq, qs, qs_row, qs_group, status};
     int rc = check_args(a, type, 2, what);
     if (rc || P == 0) return rc;
     MB_REQUIRE(type != MB_T_E4M3 || qs, "%s: e4m3 results need their scales", what);
     const cudaStream_t st = mb_stream(stream);
-    a.vec = ((uintptr_t)q & 15) == 0 && ldq % 16 == 0;
-    if (type == MB_T_E4M3) return launch<MB_T_E4M3, true>(a, what, st);
-    if (type == MB_T_BF16) return launch<MB_T_BF16, true>(a, what, st);
-    return launch<MB_T_F16, true>(a, what, st);
+    if (type == MB_T_E4M3) return launch<MB_T_E4M3, true, MB_T_E4M3>(a, what, st);
+    if (type == MB_T_BF16) return launch<MB_T_BF16, true, MB_T_BF16>(a, what, st);
+    return launch<MB_T_F16, true, MB_T_F16>(a, what, st);
 }

@@ -19,46 +19,58 @@ __device__ __forceinline__ void tc_dealloc(uint32_t base, uint32_t cols)
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// D[tmem] (+)= A[smem] * B[smem]^T (f32 accumulation), issued by one elected lane of a converged warp.
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T (f32 accumulation).
 template <bool FP8>
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
 {
     if (FP8)
         asm volatile(
-            "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
             "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
             : "memory");
     else
         asm volatile(
-            "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
             "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
             : "memory");
 }
 
-// Arrives on bar once every MMA issued so far by this thread has completed (one elected lane).
+// Arrives on bar once every MMA issued so far by this thread has completed.
 __device__ __forceinline__ void tc_commit(uint64_t* bar)
 {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\t"
-        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(mb_smem_addr(bar))
-        : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mb_smem_addr(bar))
+                 : "memory");
 }
 
-// 32 consecutive f32 columns of this thread's TMEM lane; complete after tc_wait_ld().
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32])
+// 32 consecutive f32 columns of the 32 TMEM lanes at taddr, complete after tc_wait_ld().  v[16 h + 4 b + 2 s + e] of
+// lane l: TMEM lane 16 h + 8 s + l / 4, column 8 b + 2 (l % 4) + e (the fragment of 16 lanes x 256 bits, for both halves of
+// the lanes), so a thread meets 8 of the 32 columns, not all.
+__device__ __forceinline__ void tc_ld_half(uint32_t taddr, float* v)
 {
     uint32_t* u = reinterpret_cast<uint32_t*>(v);
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
-          "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
-          "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
-          "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+          "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
         : "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32])
+{
+    tc_ld_half(taddr, v);
+    tc_ld_half(taddr + (16u << 16), v + 16);
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
@@ -92,6 +104,20 @@ __device__ __forceinline__ void tma_load3(void* dst, const CUtensorMap* map, int
         : "memory");
 }
 
+// Shared -> global copies of whole rows in the background (both addresses 16-byte aligned, bytes a multiple of 16): the
+// writers of the shared rows fence, then (after a barrier) the issuing thread copies, commits, and waits for its copies to
+// have read shared memory before that is written again.
+__device__ __forceinline__ void bulk_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t bytes)
+{
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(mb_smem_addr(src)),
+                 "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ---- thread-block clusters -------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t cluster_size()
@@ -117,9 +143,9 @@ __device__ __forceinline__ uint32_t cluster_map(uint32_t local, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void cluster_st(uint32_t addr, float v)
+__device__ __forceinline__ void cluster_st(uint32_t addr, uint64_t v)
 {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+    asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 // Arrival on another CTA's mbarrier, after which that CTA's waiters see this thread's earlier stores.
 __device__ __forceinline__ void cluster_arrive(uint32_t bar_addr)
