@@ -6,31 +6,29 @@
 // with g over groups of 128 columns (one group, scales 1, for 16-bit types).
 //
 // One persistent, warp-specialised kernel on the tcgen05 tensor cores.  The
-// weights are the M = 128 side and the rows of x the N side: an expert's row
-// count is ragged, N goes in steps of 16 and costs in proportion, and a decode
-// step's few rows leave the shared memory to a deep ring of weight tiles.  A
-// work item is (expert, block of 128 weight rows, pass of at most NT rows of
-// x), passes of one block next to each other so that its weights come from HBM
-// once; the gate|up form takes the 128 gate rows and the 128 up rows of the
-// same columns together.
+// rows of x are the M side (128 TMEM lanes, padded), 128 or 256 weight rows the
+// N side.  An epilogue thread then owns one row of x: a step's scale is one
+// number for all its columns, a row's largest value is found without other
+// lanes, and results are runs of a row.  (The other way round, weights as M,
+// ragged groups waste no tensor work, but every thread needs every row's scale
+// at every step: those shared-memory reads and the stores of single columns
+// cost 2.3 times the time at 4096 rows.)  A work item is (expert, block of
+// weight rows, pass of at most MT rows of x), passes of one block next to each
+// other so that its weights come from HBM once; the gate|up form takes 128 gate
+// rows and the 128 up rows of the same columns together.
 //  * warp 0: TMA loads (128-byte swizzle, K-major) of 128 bytes of every row
-//    of the weight block and of the pass's rows, into a ring of stages;
+//    of the pass and of the weight block, into a ring of stages;
 //  * warp 1: tcgen05.mma, f32 accumulators in TMEM.  e4m3 writes each group of
 //    128 columns to a fresh accumulator, since the group's two scales differ
 //    from the next one's.  16-bit types with 16-bit results accumulate over
 //    all of K; with f32 results they start afresh every 256 columns: the tensor
 //    cores' f32 sums are cut rather than rounded, which over 2048 columns
 //    came to 2.1e-6 of the result (f32 itself: 1e-7);
-//  * warps 2, 3 (e4m3): xs * ws of each row and group into shared memory, four
-//    groups at a time;
-//  * warps 4..11: the accumulators' columns, 32 at a time and alternating
-//    between two sets of four warps (one set alone for passes of 32 rows or
-//    fewer), added (e4m3: times their scale) to f32 registers (packed f32x2
-//    operations) while the next columns of K are multiplied.  They are read as
-//    16 x 256-bit fragments: a thread then meets 8 rows of x in 32, and needs
-//    8 scales from shared memory where whole TMEM rows need all 32 (at 256 rows
-//    those reads alone took 1024 cycles a step, twice the products).  Results go
-//    through shared memory and leave as whole rows by bulk copies.
+//  * warps 4..11: two sets of four (one warp per TMEM lane quarter), each with
+//    half of the columns: sums (e4m3: times their scale) into f32 registers
+//    while the next columns of K are multiplied, then the results, through
+//    shared memory of the warp's own so that they leave as 64-byte runs.  A
+//    quarter without rows is skipped.
 // Splitting K: with few items a cluster's CTAs take equal shares of one item's
 // groups and send their f32 partial sums through distributed shared memory to
 // the first of them, which adds them in rank order, so results do not depend on
@@ -40,7 +38,6 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "mb_common.cuh"
 #include "mb_float.cuh"
@@ -48,24 +45,25 @@
 
 namespace {
 
-constexpr int kBM = 128;                  // weight rows of a tile = TMEM lanes
-constexpr int kThreads = 384;
-constexpr int kThreadWarps = kThreads / 32;
+constexpr int kWarps = 12;
+constexpr int kThreads = 32 * kWarps;
 constexpr int kEpiWarp = 4;               // first of the eight epilogue warps
+// Registers: 168 a thread at launch; the epilogue warpgroups (up to 128 sums a thread) take theirs from the first
+// warpgroup: 128 * 56 + 256 * 224 = 64512 = the launch's 384 * 168.
+constexpr int kLoadRegs = 56, kEpiRegs = 224;
 constexpr int kEpiWarps = 8;
-constexpr int kTileA = kBM * 128;         // bytes of a weight tile: 128 rows of 128 bytes
-constexpr int kMaxN = 256;                // rows of x per pass (128 for gate|up)
-constexpr int kUnit = 4;                  // K steps whose scales are handed over together
-constexpr int kScSlots = 3;               // ring of such units
-constexpr int kMaxAcc = 8;
-// Registers: 168 a thread at launch; the epilogue warpgroups hold up to 128 sums and two tiles of 32 columns a thread
-// and take theirs from the first warpgroup: 128 * 88 + 256 * 208 = 64512 = the launch's 384 * 168.
-constexpr int kLoadRegs = 88, kEpiRegs = 208;
+constexpr int kBlock = 128;               // weight rows of a block
+constexpr int kTileW = kBlock * 128;      // bytes of a block's tile: 128 rows of 128 bytes
+constexpr int kMaxM = 128;                // rows of x per pass
+constexpr int kUnit = 4;                  // K steps whose scales a thread loads together, one such unit ahead
+constexpr int kMaxAcc = 4;
 constexpr int kMaxStages = 16;
 constexpr int kTmemCols = 512;
-constexpr int kRowMaps = 5;               // boxes of 16, 32, .., 256 rows of x
+constexpr int kRowMaps = 4;               // boxes of 16, 32, 64, 128 rows of x
 constexpr int kMaxSmem = 232448;          // 227 KB
-constexpr int kMaxRed = 64 << 10;         // shared memory for partial sums of a split
+constexpr int kMaxRed = 112 << 10;        // shared memory for partial sums of a split
+constexpr int kSplitRows = 32;            // a split item's rows, at most
+constexpr int kRun = 64, kPitch = 80;     // results leave in runs of 64 bytes a row; rows 80 apart in shared memory
 
 __device__ unsigned g_no_status;          // where kernels report when the caller gives no status word
 
@@ -86,13 +84,11 @@ struct GroupedArgs {
     int64_t qs_row, qs_group;
     unsigned* status;
     int Kb;                    // K steps (128 bytes of a row each)
-    int Mb;                    // blocks of 128 output columns
-    int NT;                    // rows of x per pass, at most
+    int Nb;                    // column blocks of an item's width
+    int MT;                    // rows of x per pass, at most
     int stages;
-    int nacc;                  // accumulator slots in TMEM
-    int acc_cols;              // TMEM columns of one half of a slot; also rows of x in a scale slot
     int prom;                  // K steps summed in TMEM before their sum is added to the f32 registers
-    int vec;                   // whole rows of results start on 16-byte boundaries
+    int vec;                   // rows of results start on 16-byte boundaries
 };
 
 struct Maps {
@@ -105,7 +101,7 @@ struct Items {
     const GroupedArgs& a;
     const int2* meta;          // (first row, rows) of each expert
     const int* pstart;         // first item of each expert; [E]: all items
-    int it, step, e, mb, row0, nrows;
+    int it, step, e, nb, row0, nrows;
     __device__ Items(const GroupedArgs& args, const int2* m, const int* ps, int first, int by)
         : a(args), meta(m), pstart(ps), it(first - by), step(by), e(0)
     {
@@ -126,10 +122,10 @@ struct Items {
             e = lo;
         }
         const int2 m = meta[e];
-        const int passes = (m.y + a.NT - 1) / a.NT;
+        const int passes = (m.y + a.MT - 1) / a.MT;
         const int local = it - pstart[e];
-        mb = local / passes;
-        const int pass = local - mb * passes;
+        nb = local / passes;
+        const int pass = local - nb * passes;
         const int size = ((m.y + passes - 1) / passes + 15) & ~15;     // passes of about equal size
         row0 = m.x + pass * size;
         nrows = min(size, m.y - pass * size);
@@ -155,149 +151,131 @@ struct Units {
     }
 };
 
-__device__ __forceinline__ uint64_t pack2(float lo, float hi)
-{
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-    return v;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi)
-{
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b)
-{
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
-}
-
-__device__ __forceinline__ void add2(uint64_t& acc, uint64_t a)
-{
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(a));
-}
-
-template <int OUT>
-struct OutOf;
-template <>
-struct OutOf<MB_T_F32> {
-    using T = float;
-    static __device__ __forceinline__ T round(float v) { return v; }
-};
-template <>
-struct OutOf<MB_T_BF16> {
-    using T = __nv_bfloat16;
-    static __device__ __forceinline__ T round(float v) { return __float2bfloat16_rn(v); }
-};
-template <>
-struct OutOf<MB_T_F16> {
-    using T = __half;
-    static __device__ __forceinline__ T round(float v) { return __float2half_rn(v); }
-};
-
-// Results of 32 rows wait in shared memory as rows of 128 outputs, f32 ones in two halves of 16 rows.  The distance
-// between rows keeps the fragments' stores (4 rows 2 apart x 8 outputs) on different banks.
 __host__ __device__ constexpr int out_bytes(int out) { return out == MB_T_F32 ? 4 : out == MB_T_E4M3 ? 1 : 2; }
-__host__ __device__ constexpr int tile_rows(int out) { return out == MB_T_F32 ? 16 : 32; }
-__host__ __device__ constexpr int tile_pitch(int out) { return 128 * out_bytes(out) + 16; }
 
-// Where scale n of 32 lies: a thread reads those of its columns 8 b + 2 i + e (i = lane % 4), b = 0, 1, as one vector.
-__device__ __forceinline__ int scale_pos(int n) { return (n & ~15) + ((n >> 1) & 3) * 4 + ((n >> 3) & 1) * 2 + (n & 1); }
+// Two results as 16-bit numbers, packed.
+template <int OUT>
+__device__ __forceinline__ uint32_t round2(float lo, float hi)
+{
+    if (OUT == MB_T_BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 
-// What an epilogue warp keeps between items.
+// WIDE: an item is two blocks of 128 weight rows, one per epilogue set (gate|up: the gate and the up rows of 128 columns,
+// of which each set takes 64); else one block, 64 columns per set.  OUT: the result type (gate|up: TYPE).
+template <int TYPE, bool DUAL, bool WIDE, int OUT>
 struct Epilogue {
+    static constexpr bool FP8 = TYPE == MB_T_E4M3;
+    static constexpr int H = DUAL ? 2 : 1;
+    static constexpr int N = WIDE ? 256 : 128;             // accumulator columns of an item
+    static constexpr int S = N / 2;                        // of them this thread's
+    static constexpr int C = S / 16;                       // chunks of 16
+
     const GroupedArgs& a;
     unsigned* status;
     volatile int* abort_flag;
     uint32_t tl;               // TMEM address of the warp's lane quarter
-    uint64_t *acc_full, *acc_empty, *sc_full, *sc_empty;
-    const float* sc;
-    uint64_t* red;
+    uint64_t *acc_full, *acc_empty;
+    float4* red;               // partial sums: [sender][set][S / 4][32 lanes]
     uint64_t *red_full, *red_empty;
-    float *amax, *tsc;
-    uint8_t* tile;             // the set's rows of results
-    int k0, k1, split, srank;
+    float* amax;               // [2][2 sets][128 rows]
+    uint8_t* stage;            // the warp's 32 rows of kRun bytes
+    int split, srank;
     uint32_t leader;
     int q, set, lane;
-    Ring ac, scr;
+    Ring ac;
     int sent, abuf;
+    float xr[kUnit], wr[H][kUnit];                         // the next unit's scales, on their way
 
-    // One item with N chunks of 32 rows for this warp's set (a count known at compile time keeps the sums in
-    // registers: with a test around each chunk a step took 3200 cycles at 256 rows, most of them moves).
-    // sum[t][8 h + 2 b + s]: weight row 32 q + 16 h + 8 s + lane / 4, rows of x 8 b + 2 (lane % 4) + {0, 1} of tile t.
-    template <int TYPE, bool DUAL, int OUT, int N>
-    __device__ __forceinline__ void item(const Items& w)
+    // Accumulator column of this thread's chunk c.  Gate|up: its first half of chunks are gate columns, then the up
+    // columns of the same place.
+    __device__ __forceinline__ int column(int c) const
     {
-        constexpr bool FP8 = TYPE == MB_T_E4M3;
-        constexpr int H = DUAL ? 2 : 1;
-        constexpr int T = H * N;               // tiles of 32 columns: chunk t / H, half t % H
-        const int scw = H * a.acc_cols;
+        if (DUAL) return (c >= C / 2 ? kBlock : 0) + 64 * set + 16 * (c % (C / 2));
+        return S * set + 16 * c;
+    }
+
+    __device__ __forceinline__ void load_scales(const Units& un)
+    {
+        if (!FP8 || !un.live) return;
+        const int Ob = (a.O + kScaleBlock - 1) / kScaleBlock;
+        const int block = DUAL ? un.w.nb : WIDE ? min(2 * un.w.nb + set, Ob - 1) : un.w.nb;
+        const int r = 32 * q + lane;
+        const float* xp = a.xs + (int64_t)(un.w.row0 + min(r, un.w.nrows - 1)) * a.xs_row + (int64_t)un.kb * a.xs_group;
+        const float* wp = a.ws + ((int64_t)un.w.e * H * Ob + block) * a.Kb + un.kb;
+#pragma unroll
+        for (int s = 0; s < kUnit; ++s) {
+            const bool real = un.kb + s < un.k1;
+            xr[s] = real ? __ldg(xp + s * a.xs_group) : 0.0f;
+#pragma unroll
+            for (int h = 0; h < H; ++h) wr[h][s] = real ? __ldg(wp + (int64_t)h * Ob * a.Kb + s) : 0.0f;
+        }
+    }
+
+    // One item's K steps k0 .. k1 - 1 and its results; `ahead` is this item's first unit, whose scales are loading.
+    __device__ __forceinline__ void item(const Items& w, Units& ahead, int k0, int k1)
+    {
+        const bool rows = 32 * q < w.nrows;                // this quarter has some
         bool ok = true;
-        uint64_t sum[T > 0 ? T : 1][16];
+        float sum[C][16];
 #pragma unroll
-        for (int t = 0; t < T; ++t)
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sum[t][j] = 0;
-        for (int kb = k0; kb < k1; kb += a.prom) {
-            const int us = (kb - k0) % kUnit;
-            if (FP8 && us == 0) ok = mb_mbar_wait_spin(&sc_full[scr.slot], scr.full_parity(), status, abort_flag) && ok;
+            for (int i = 0; i < 16; ++i) sum[c][i] = 0.0f;
+        float sc[H][kUnit];
+        for (int kb = k0, us = 0; kb < k1; kb += a.prom, us = (us + 1) % kUnit) {
+            if (FP8 && us == 0) {
+#pragma unroll
+                for (int s = 0; s < kUnit; ++s)
+#pragma unroll
+                    for (int h = 0; h < H; ++h) sc[h][s] = xr[s] * wr[h][s];
+                ahead.next();
+                load_scales(ahead);
+            }
             ok = mb_mbar_wait_spin(&acc_full[ac.slot], ac.full_parity(), status, abort_flag) && ok;
             tc_after();
-            if constexpr (T > 0) {
-                float d[2][32];                // the next tile is on its way while this one is added
-                const uint32_t from = tl + ac.slot * scw + 32 * set;
-                const float* s0 = sc + (scr.slot * kUnit + us) * scw + 32 * set + 4 * (lane & 3);
-                tc_ld32(from, d[0]);
-                tc_wait_ld();
+            if (rows) {
+                const uint32_t from = tl + ac.slot * N;
+                float d[2][16];                            // the next chunk is on its way while this one is added
+                tc_ld16(from + column(0), d[0]);
+                tc_wait_ld(d[0]);
 #pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    if (t + 1 < T) tc_ld32(from + ((t + 1) % H) * a.acc_cols + 64 * ((t + 1) / H), d[(t + 1) & 1]);
-                    const float(&v)[32] = d[t & 1];
+                for (int c = 0; c < C; ++c) {
+                    if (c + 1 < C) tc_ld16(from + column(c + 1), d[(c + 1) & 1]);
+                    const float s = sc[DUAL && c >= C / 2 ? H - 1 : 0][0];
 #pragma unroll
-                    for (int bp = 0; bp < 2; ++bp) {
-                        float4 s = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                        if (FP8)
-                            s = *reinterpret_cast<const float4*>(s0 + (t % H) * a.acc_cols + 64 * (t / H) + 16 * bp);
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) {      // b = 2 bp + r % 2, s = r / 2 % 2, h = r / 4
-                            const int b = 2 * bp + (r & 1), j = 8 * (r >> 2) + 2 * b + ((r >> 1) & 1);
-                            const uint64_t x = pack2(v[2 * j], v[2 * j + 1]);
-                            if (FP8)
-                                fma2(sum[t][j], x, r & 1 ? pack2(s.z, s.w) : pack2(s.x, s.y));
-                            else
-                                add2(sum[t][j], x);
-                        }
-                    }
-                    if (t + 1 < T) tc_wait_ld();
+                    for (int i = 0; i < 16; ++i)
+                        sum[c][i] = FP8 ? fmaf(d[c & 1][i], s, sum[c][i]) : sum[c][i] + d[c & 1][i];
+                    if (c + 1 < C) tc_wait_ld(d[(c + 1) & 1]);
                 }
             }
+#pragma unroll
+            for (int h = 0; h < H; ++h)                    // the unit's next step
+#pragma unroll
+                for (int s = 0; s + 1 < kUnit; ++s) sc[h][s] = sc[h][s + 1];
             tc_before();
             __syncwarp();
-            const bool unit_done = FP8 && (us == kUnit - 1 || kb + 1 == k1);
-            if (lane == 0) {
-                mb_mbar_arrive(&acc_empty[ac.slot]);
-                if (unit_done) mb_mbar_arrive(&sc_empty[scr.slot]);
-            }
+            if (lane == 0) mb_mbar_arrive(&acc_empty[ac.slot]);
             ac.next();
-            if (unit_done) scr.next();
         }
 
         if (split > 1) {
-            // NT <= 32: one chunk, one set.  Partial sums: [sender][half][h, b, s][128 threads] pairs.
-            const int np = (w.nrows + 15) & ~15, nb = a.NT / 8;
-            const int me = 32 * q + lane;
+            // at most 32 rows: the first lane quarter's two warps
             if (srank > 0) {
                 // the receiver has read the previous item's sums (the first wait passes at once)
                 ok = mbar_wait_cluster(red_empty, (sent & 1) ^ 1, status, abort_flag) && ok;
                 ++sent;
-                if constexpr (N == 1) {
+                if (rows && ok) {
+                    const uint32_t to =
+                        cluster_map(mb_smem_addr(red + ((srank - 1) * 2 + set) * (S / 4) * 32 + lane), leader);
 #pragma unroll
-                    for (int h = 0; h < H; ++h) {
-                        const uint32_t to =
-                            cluster_map(mb_smem_addr(red + ((srank - 1) * H + h) * 4 * nb * 128 + me), leader);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int b = (j >> 1) & 3;
-                            if (8 * b < np && ok) cluster_st(to + (((j >> 3) * nb + b) * 2 + (j & 1)) * 1024, sum[h][j]);
-                        }
+                    for (int j = 0; j < S / 4; ++j) {
+                        const float* v = &sum[j / 4][4 * (j % 4)];
+                        cluster_st4(to + j * 512, v[0], v[1], v[2], v[3]);
                     }
                 }
                 __syncwarp();
@@ -306,154 +284,121 @@ struct Epilogue {
             }
             ok = mbar_wait_cluster(red_full, sent & 1, status, abort_flag) && ok;
             ++sent;
-            if constexpr (N == 1) {
-                for (int r = 0; r < split - 1; ++r)
+            if (rows) {
+                for (int r = 0; r < split - 1; ++r) {
+                    const float4* from = red + (r * 2 + set) * (S / 4) * 32 + lane;
 #pragma unroll
-                    for (int h = 0; h < H; ++h) {
-                        const uint64_t* from = red + (r * H + h) * 4 * nb * 128 + me;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int b = (j >> 1) & 3;
-                            if (8 * b < np) add2(sum[h][j], from[(((j >> 3) * nb + b) * 2 + (j & 1)) * 128]);
-                        }
+                    for (int j = 0; j < S / 4; ++j) {
+                        const float4 v = from[j * 32];
+                        float* to = &sum[j / 4][4 * (j % 4)];
+                        to[0] += v.x, to[1] += v.y, to[2] += v.z, to[3] += v.w;
                     }
+                }
             }
             __syncwarp();
             if (lane == 0)
                 for (int r = 1; r < split; ++r) cluster_arrive(cluster_map(mb_smem_addr(red_empty), leader + r));
         }
 
+        if constexpr (DUAL) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = 2 * i + set;
-            const int n = w.nrows - 32 * c;                // rows of this chunk (32 or fewer are real)
-            const int64_t row = (int64_t)w.row0 + 32 * c;
-            float v[32];
+            for (int c = 0; c < C / 2; ++c)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) unpack2(sum[H * i][j], v[2 * j], v[2 * j + 1]);
-            if constexpr (DUAL) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    float u0, u1;
-                    unpack2(sum[H * i + 1][j], u0, u1);
-                    v[2 * j] = __fdividef(v[2 * j], 1.0f + __expf(-v[2 * j])) * u0;
-                    v[2 * j + 1] = __fdividef(v[2 * j + 1], 1.0f + __expf(-v[2 * j + 1])) * u1;
+                for (int i = 0; i < 16; ++i) {
+                    const float g = sum[c][i];
+                    sum[c][i] = __fdividef(g, 1.0f + __expf(-g)) * sum[c + C / 2][i];
                 }
-            }
-            if constexpr (OUT == MB_T_E4M3)
-                encode(w.mb, v, row, n, ok);
-            else
-                store<OUT>(w.mb, v, row, n, ok);
         }
-    }
-
-    // The tile's rows to y, 128 outputs (fewer in the last block) from column 128 mb on: `rows` rows of out bytes each.
-    template <int OUT>
-    __device__ __forceinline__ void send(int mb, int64_t row, int rows, bool ok)
-    {
-        constexpr int R = tile_rows(OUT), B = out_bytes(OUT), pitch = tile_pitch(OUT);
-        bulk_fence();
-        mb_named_barrier(1 + set, 128);
-        const int me = 32 * q + lane, bytes = min(kBM, a.O - mb * kBM) * B;
-        uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row * a.ldy + (int64_t)mb * kBM) * B;
-        if (a.vec && bytes % 16 == 0) {
-            const int r = me / (128 / R);
-            if (me % (128 / R) == 0 && r < rows && ok)
-                bulk_s2g(dst + r * a.ldy * B, tile + r * pitch, bytes);
-            bulk_commit();
-        } else if (ok) {
-            for (int r = q; r < min(rows, R); r += 4)
-                for (int i = lane; i < bytes / B; i += 32)
-                    if (B == 4)
-                        reinterpret_cast<uint32_t*>(dst + r * a.ldy * B)[i] = reinterpret_cast<uint32_t*>(tile + r * pitch)[i];
-                    else if (B == 2)
-                        reinterpret_cast<uint16_t*>(dst + r * a.ldy * B)[i] = reinterpret_cast<uint16_t*>(tile + r * pitch)[i];
+        const int n = ok ? min(32, w.nrows - 32 * q) : 0;  // rows of this quarter to write
+        const int64_t row = (int64_t)w.row0 + 32 * q;
+        const int col = DUAL ? w.nb * kBlock + 64 * set : w.nb * N + S * set;
+        if constexpr (OUT == MB_T_E4M3) {
+            encode(sum, row, n, w.nb, col);
+        } else if (rows) {
+            constexpr int RC = kRun / out_bytes(OUT);      // columns of a run: 16 of f32, 32 of 16 bits
+#pragma unroll
+            for (int r = 0; r < (DUAL ? 64 : S) / RC; ++r) {
+                uint4* to = reinterpret_cast<uint4*>(stage + lane * kPitch);
+#pragma unroll
+                for (int j = 0; j < kRun / 16; ++j) {
+                    constexpr int VC = 16 / out_bytes(OUT);
+                    const int i = r * RC + j * VC;
+                    const float* v = &sum[i / 16][i % 16];
+                    if constexpr (OUT == MB_T_F32)
+                        to[j] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                           __float_as_uint(v[3]));
                     else
-                        (dst + r * a.ldy)[i] = (tile + r * pitch)[i];
-        }
-    }
-
-    // 32 rows of results (this thread's fragment of them), rounded to the output type.
-    template <int OUT>
-    __device__ __forceinline__ void store(int mb, const float (&v)[32], int64_t row, int n, bool ok)
-    {
-        constexpr int R = tile_rows(OUT), pitch = tile_pitch(OUT);
-        using O = OutOf<OUT>;
-#pragma unroll
-        for (int p = 0; p < 32 / R; ++p) {
-            if (p * R >= n) break;
-            bulk_wait_read();
-            mb_named_barrier(1 + set, 128);                // the tile's last rows have left
-            uint8_t* to = tile + 2 * (lane & 3) * pitch + (32 * q + (lane >> 2)) * out_bytes(OUT);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int b = (j >> 1) & 3, w = 16 * (j >> 3) + 8 * (j & 1);
-                if (8 * b / R == p) {
-                    typename O::T* d = reinterpret_cast<typename O::T*>(to + (8 * b - p * R) * pitch) + w;
-                    d[0] = O::round(v[2 * j]);
-                    d[pitch / out_bytes(OUT)] = O::round(v[2 * j + 1]);
+                        to[j] = make_uint4(round2<OUT>(v[0], v[1]), round2<OUT>(v[2], v[3]), round2<OUT>(v[4], v[5]),
+                                           round2<OUT>(v[6], v[7]));
                 }
+                send(row, n, col + r * RC);
             }
-            send<OUT>(mb, row + p * R, n - p * R, ok);
         }
     }
 
-    // 32 rows of results as e4m3 with a scale per row: each row's largest of the block's 128 columns (over a thread's
-    // four, the eight lanes that share its rows, and the set's four warps), then the quotients.
-    __device__ __forceinline__ void encode(int mb, const float (&v)[32], int64_t row, int n, bool ok)
+    // The warp's 32 staged runs to rows row .. row + n - 1 of y, from column col on (not past column O).
+    __device__ __forceinline__ void send(int64_t row, int n, int col)
     {
-        constexpr int pitch = tile_pitch(MB_T_E4M3);
-        const int o = mb * kBM + 32 * q + (lane >> 2);
-        float m[8];                                        // index 2 b + e
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m[i] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int b = (j >> 1) & 3;
-            if (o + 16 * (j >> 3) + 8 * (j & 1) < a.O) {
-                m[2 * b] = fmaxf(m[2 * b], fabsf(v[2 * j]));
-                m[2 * b + 1] = fmaxf(m[2 * b + 1], fabsf(v[2 * j + 1]));
-            }
-        }
-#pragma unroll
-        for (int s = 16, h = 4; s >= 4; s >>= 1, h >>= 1) {
-            const bool hi = lane & s;
-#pragma unroll
-            for (int i = 0; i < h; ++i) {
-                const float send = hi ? m[i] : m[i + h], keep = hi ? m[i + h] : m[i];
-                m[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, s));
-            }
-        }
-        // this lane now has index lane / 4
-        float* am = amax + ((set * 2 + abuf) * 4) * 32;
-        abuf ^= 1;
-        am[q * 32 + 8 * (lane >> 3) + 2 * (lane & 3) + ((lane >> 2) & 1)] = m[0];
-        bulk_wait_read();
-        mb_named_barrier(1 + set, 128);                    // also: the tile's last rows have left
-        const Quotient qu(e4m3_scale(fmaxf(fmaxf(am[lane], am[32 + lane]), fmaxf(am[64 + lane], am[96 + lane]))));
-        const bool fast = __all_sync(0xffffffffu, qu.fast);
-        float* ts = tsc + (set * 4 + q) * 64;
-        ts[lane] = qu.s;
-        ts[32 + lane] = qu.r;
-        if (q == 0 && lane < n && ok) a.qs[(row + lane) * a.qs_row + mb * a.qs_group] = qu.s;
+        constexpr int B = out_bytes(OUT);
         __syncwarp();
-        uint8_t* to = tile + 2 * (lane & 3) * pitch + 32 * q + (lane >> 2);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const float2 s = *reinterpret_cast<const float2*>(ts + 8 * b + 2 * (lane & 3));
-            const float2 r = *reinterpret_cast<const float2*>(ts + 32 + 8 * b + 2 * (lane & 3));
+        uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row * a.ldy + col) * B;
+        if (a.vec && col + kRun / B <= a.O) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int j = 8 * (i >> 1) + 2 * b + (i & 1);
-                const float x0 = v[2 * j], x1 = v[2 * j + 1];
-                const uint32_t e = fast ? to_e4m3x2(quotient(x0, s.x, r.x), quotient(x1, s.y, r.y))
-                                        : to_e4m3x2(__fdiv_rn(x0, s.x), __fdiv_rn(x1, s.y));
-                uint8_t* d = to + 8 * b * pitch + 16 * (i >> 1) + 8 * (i & 1);
-                d[0] = (uint8_t)e;
-                d[pitch] = (uint8_t)(e >> 8);
+                const int r = 8 * i + (lane >> 2), s = 16 * (lane & 3);
+                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * kPitch + s);
+                if (r < n) *reinterpret_cast<uint4*>(dst + r * a.ldy * B + s) = v;
             }
+        } else {
+            const int cols = min(kRun / B, a.O - col);
+            for (int r = 0; r < n; ++r)
+                for (int i = lane; i < cols; i += 32) {
+                    if (B == 4)
+                        reinterpret_cast<uint32_t*>(dst + r * a.ldy * B)[i] =
+                            reinterpret_cast<const uint32_t*>(stage + r * kPitch)[i];
+                    else if (B == 2)
+                        reinterpret_cast<uint16_t*>(dst + r * a.ldy * B)[i] =
+                            reinterpret_cast<const uint16_t*>(stage + r * kPitch)[i];
+                    else
+                        dst[r * a.ldy + i] = stage[r * kPitch + i];
+                }
         }
-        send<MB_T_E4M3>(mb, row, n, ok);
+        __syncwarp();
+    }
+
+    // This thread's 64 activations of a row as e4m3, the row's scale over them and the other set's 64.
+    __device__ __forceinline__ void encode(const float (&v)[C][16], int64_t row, int n, int nb, int col)
+    {
+        float m = 0.0f;
+        if (col + 64 <= a.O) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) m = fmaxf(m, fabsf(v[i / 16][i % 16]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) m = col + i < a.O ? fmaxf(m, fabsf(v[i / 16][i % 16])) : m;
+        }
+        float* am = amax + abuf * 2 * kMaxM + 32 * q + lane;
+        abuf ^= 1;
+        am[set * kMaxM] = m;
+        mb_named_barrier(1 + q, 64);
+        const Quotient qu(e4m3_scale(fmaxf(am[0], am[kMaxM])));
+        const bool fast = __all_sync(0xffffffffu, qu.fast || lane >= n);
+        if (set == 0 && lane < n) a.qs[(row + lane) * a.qs_row + nb * a.qs_group] = qu.s;
+        uint4* to = reinterpret_cast<uint4*>(stage + lane * kPitch);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* x = &v[j][4 * i];
+                u[i] = fast ? to_e4m3x2(quotient(x[0], qu.s, qu.r), quotient(x[1], qu.s, qu.r)) |
+                                  to_e4m3x2(quotient(x[2], qu.s, qu.r), quotient(x[3], qu.s, qu.r)) << 16
+                            : to_e4m3x2(__fdiv_rn(x[0], qu.s), __fdiv_rn(x[1], qu.s)) |
+                                  to_e4m3x2(__fdiv_rn(x[2], qu.s), __fdiv_rn(x[3], qu.s)) << 16;
+            }
+            to[j] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        send(row, n, col);
     }
 };
 
@@ -462,39 +407,35 @@ __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.
 template <int R>
 __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
-// OUT: the result type (gate|up: TYPE)
-template <int TYPE, bool DUAL, int OUT>
+template <int TYPE, bool DUAL, bool WIDE, int OUT>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ GroupedArgs a, const __grid_constant__ Maps maps)
 {
+    using Epi = Epilogue<TYPE, DUAL, WIDE, OUT>;
     constexpr bool FP8 = TYPE == MB_T_E4M3;
     constexpr int KS = FP8 ? 128 : 64;    // columns of a K step
-    constexpr int H = DUAL ? 2 : 1;       // weight tiles of a step
+    constexpr int NB = WIDE ? 2 : 1;      // weight tiles of a step
+    constexpr int kAcc = kTmemCols / Epi::N;
 
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    const int stage_bytes = H * kTileA + a.NT * 128;
+    // a stage: the pass's rows, then the weight tiles.  The products always read 128 rows: past MT they find the weight
+    // tiles' bytes, whose results stay in lanes that nobody reads.
+    const int stage_bytes = a.MT * 128 + NB * kTileW;
     const uint32_t csize = cluster_size();
     uint8_t* stage0 = smem;
-    const int sets = a.NT > 32 ? 2 : 1;   // passes of 32 rows or fewer have one chunk: one set of epilogue warps
-    const int scw = H * a.acc_cols;
-    uint64_t* red = reinterpret_cast<uint64_t*>(stage0 + (size_t)a.stages * stage_bytes);   // [csize - 1][H][NT / 2][128]
-    float* sc = reinterpret_cast<float*>(red + (csize - 1) * H * a.NT * 64);                // [kScSlots][kUnit][scw]
-    float* amax = sc + (FP8 ? kScSlots * kUnit * scw : 0);             // [2 sets][2][4 quarters][32]
-    float* tsc = amax + (OUT == MB_T_E4M3 ? 2 * 2 * 4 * 32 : 0);       // [8 warps][scale, 1 / scale][32]
-    uint8_t* tiles = reinterpret_cast<uint8_t*>(tsc + (OUT == MB_T_E4M3 ? kEpiWarps * 64 : 0));   // [sets][rows][pitch]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + sets * tile_rows(OUT) * tile_pitch(OUT));
-    uint64_t* full = bars;
+    float4* red = reinterpret_cast<float4*>(stage0 + (size_t)a.stages * stage_bytes);
+    float* amax = reinterpret_cast<float*>(red + (csize - 1) * Epi::N / 4 * 32);
+    uint8_t* runs = reinterpret_cast<uint8_t*>(amax + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM : 0));
+    uint64_t* full = reinterpret_cast<uint64_t*>(runs + kEpiWarps * 32 * kPitch);
     uint64_t* empty = full + kMaxStages;
     uint64_t* acc_full = empty + kMaxStages;
     uint64_t* acc_empty = acc_full + kMaxAcc;
-    uint64_t* sc_full = acc_empty + kMaxAcc;
-    uint64_t* sc_empty = sc_full + kScSlots;
-    uint64_t* red_full = sc_empty + kScSlots;
+    uint64_t* red_full = acc_empty + kMaxAcc;
     uint64_t* red_empty = red_full + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_empty + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [kThreadWarps] + split
+    int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [kWarps], [15]: split
     int2* meta = reinterpret_cast<int2*>(wsum + 16);                   // [E]
     int* pstart = reinterpret_cast<int*>(meta + a.E);                  // [E + 1]
 
@@ -507,13 +448,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             mb_mbar_init(&full[i], 1);
             mb_mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < a.nacc; ++i) {
+        for (int i = 0; i < kAcc; ++i) {
             mb_mbar_init(&acc_full[i], 1);
-            mb_mbar_init(&acc_empty[i], 4 * sets);
-        }
-        for (int i = 0; i < kScSlots; ++i) {
-            mb_mbar_init(&sc_full[i], 1);
-            mb_mbar_init(&sc_empty[i], 4 * sets);
+            mb_mbar_init(&acc_empty[i], kEpiWarps);
         }
         *abort_flag = 0;
         tma_prefetch_map(&maps.w);
@@ -524,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The experts' rows and the first item of each: an exclusive scan over the experts, a run of them per thread.
     {
         const int per = (a.E + kThreads - 1) / kThreads;
-        const int e0 = threadIdx.x * per, e1 = min(a.E, e0 + per);
+        const int e0 = min(a.E, (int)threadIdx.x * per), e1 = min(a.E, e0 + per);
         int items = 0;
         for (int e = e0; e < e1; ++e) {
             int lo = 0, n = (int)a.P;
@@ -539,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             meta[e] = make_int2(lo, n);
             pstart[e] = items;
-            items += a.Mb * ((n + a.NT - 1) / a.NT);
+            items += a.Nb * ((n + a.MT - 1) / a.MT);
         }
         int run = items;
 #pragma unroll
@@ -550,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 31) wsum[warp] = run;
         __syncthreads();
         int before = run - items, total = 0;
-        for (int w = 0; w < kThreadWarps; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
             const int s = wsum[w];
             if (w < warp) before += s;
             total += s;
@@ -560,18 +497,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             pstart[a.E] = total;
             // How many CTAs share an item: the split whose longest CTA has the fewest K steps, two more for each
             // item that is split (the partial sums' way to the first CTA).
-            int best = 0x7fffffff, split = 1;
+            int64_t best = (int64_t)1 << 62;
+            int split = 1;
             for (int s = 1; s <= (int)csize && s <= a.Kb; s <<= 1) {
                 const int groups = gridDim.x / s;
                 const int64_t c = (int64_t)((total + groups - 1) / groups) * ((a.Kb + s - 1) / s + (s > 1 ? 2 : 0));
                 if (c < best) {
-                    best = (int)c;
+                    best = c;
                     split = s;
                 }
             }
             wsum[15] = split;
-            mb_mbar_init(red_full, 4 * max(split - 1, 1));  // a split needs NT <= 32: one set
-            mb_mbar_init(red_empty, 4);
+            mb_mbar_init(red_full, kEpiWarps * max(split - 1, 1));
+            mb_mbar_init(red_empty, kEpiWarps);
             mb_fence_mbar_init();
         }
     }
@@ -584,7 +522,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int split = wsum[15];
     const int srank = (int)blockIdx.x % split;                          // rank among the CTAs of an item
     const int k0 = (int)((int64_t)a.Kb * srank / split), k1 = (int)((int64_t)a.Kb * (srank + 1) / split);
-    const uint32_t leader = cluster_rank() - srank;                     // cluster rank of the item's first CTA
     Items w(a, meta, pstart, blockIdx.x / split, gridDim.x / split);
 
     if (warp < kEpiWarp) setmaxnreg_dec<kLoadRegs>();
@@ -599,16 +536,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int b = lane - 2;
             const bool box = b >= 0 && b < kRowMaps && ((r16 >> b) & 1);
             const int brow = b >= 0 && b < kRowMaps ? ((r16 >> (b + 1)) << (b + 1)) * 16 : 0;
+            const int wrow = DUAL ? lane * a.O + w.nb * kBlock : (w.nb * NB + lane) * kBlock;
             for (int kb = k0; kb < k1; ++kb, st.next()) {
                 ok = __all_sync(0xffffffffu, mb_mbar_wait_spin(&empty[st.slot], st.empty_parity(), status, abort_flag));
                 if (!ok) break;
                 uint8_t* dst = stage0 + (size_t)st.slot * stage_bytes;
-                if (lane == 0) mb_mbar_arrive_expect_tx(&full[st.slot], H * kTileA + r16 * 16 * 128);
+                if (lane == 0) mb_mbar_arrive_expect_tx(&full[st.slot], NB * kTileW + r16 * 16 * 128);
                 __syncwarp();
-                if (lane < H)
-                    tma_load3(dst + lane * kTileA, &maps.w, kb * KS, lane * a.O + w.mb * kBM, w.e, &full[st.slot]);
+                if (lane < NB)
+                    tma_load3(dst + a.MT * 128 + lane * kTileW, &maps.w, kb * KS, wrow, w.e, &full[st.slot]);
                 else if (box)
-                    tma_load2(dst + H * kTileA + brow * 128, &maps.x[b], kb * KS, w.row0 + brow, &full[st.slot]);
+                    tma_load2(dst + brow * 128, &maps.x[b], kb * KS, w.row0 + brow, &full[st.slot]);
                 ++issued;
             }
         }
@@ -625,14 +563,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         // ------------------------------------------------------------------ tensor cores
         if (elect_one()) {
-            Ring st(a.stages), ac(a.nacc);
+            Ring st(a.stages), ac(kAcc);
             bool ok = true;
-            // D f32; A and B both K-major: e4m3 / f16 are format 0, bf16 is 1
-            const uint32_t fmt = TYPE == MB_T_BF16 ? (1u << 7) | (1u << 10) : 0u;
+            // M = 128, N, D f32; A and B both K-major: e4m3 / f16 are format 0, bf16 is 1
+            constexpr uint32_t idesc = (1u << 4) | (TYPE == MB_T_BF16 ? (1u << 7) | (1u << 10) : 0u) |
+                                       ((uint32_t)(Epi::N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             const uint64_t desc0 = tc_desc_sw128(mb_smem_addr(stage0));
             while (ok && w.next()) {
-                const int n16 = (w.nrows + 15) & ~15;
-                const uint32_t idesc = (1u << 4) | fmt | ((uint32_t)(n16 >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
                 int part = 0;                              // K steps already in the accumulator
                 for (int kb = k0; kb < k1; ++kb, st.next()) {
                     if (part == 0)
@@ -640,15 +577,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ok = ok && mb_mbar_wait_spin(&full[st.slot], st.full_parity(), status, abort_flag);
                     if (!ok) break;
                     tc_after();
-                    const uint64_t da = desc0 + (uint64_t)((st.slot * stage_bytes) >> 4);
-                    const uint64_t db = da + (H * kTileA >> 4);
-                    const uint32_t d = tmem + ac.slot * scw;
+                    const uint64_t dx = desc0 + (uint64_t)((st.slot * stage_bytes) >> 4);
+                    const uint64_t dw = dx + (uint64_t)(a.MT * 128 >> 4);
 #pragma unroll
-                    for (int h = 0; h < H; ++h)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            tc_mma_ss<FP8>(d + h * a.acc_cols, da + (h * kTileA >> 4) + 2 * j, db + 2 * j, idesc,
-                                           (j > 0 || part > 0) ? 1u : 0u);
+                    for (int j = 0; j < 4; ++j)
+                        tc_mma_ss<FP8>(tmem + ac.slot * Epi::N, dx + 2 * j, dw + 2 * j, idesc,
+                                       (j > 0 || part > 0) ? 1u : 0u);
                     tc_commit(&empty[st.slot]);
                     if (++part == a.prom || kb + 1 == k1) {
                         tc_commit(&acc_full[ac.slot]);
@@ -659,82 +593,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp < kEpiWarp) {
-        // ------------------------------------------------------------------ scales (steps in turn between two warps)
-        if (FP8) {
-            // Each warp takes every second unit.  A lane loads kUnit groups of its rows at once: the scales come from L2 or
-            // HBM, and four groups share that latency and the hand-over.
-            constexpr int NL = DUAL ? 4 : 8;               // rows per lane
-            const int Ob = (a.O + kScaleBlock - 1) / kScaleBlock;
-            Units un(w, k0, k1);
-            if (warp == 3) un.next();
-            Ring slot(kScSlots);
-            if (warp == 3) slot.next();
-            while (un.live) {
-                const int m = min(kUnit, k1 - un.kb);
-                const float* wsp = a.ws + ((int64_t)un.w.e * H * Ob + un.w.mb) * a.Kb + un.kb;
-                const float* xsp = a.xs + ((int64_t)un.w.row0 + lane) * a.xs_row + (int64_t)un.kb * a.xs_group;
-                float v[NL][kUnit], w0[kUnit], w1[kUnit];
-#pragma unroll
-                for (int s = 0; s < kUnit; ++s) {
-                    w0[s] = s < m ? wsp[s] : 0.0f;
-                    if (DUAL) w1[s] = s < m ? wsp[(int64_t)Ob * a.Kb + s] : 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < NL; ++i) {
-                    const bool real = lane + 32 * i < un.w.nrows;
-#pragma unroll
-                    for (int s = 0; s < kUnit; ++s)
-                        v[i][s] = real && s < m ? xsp[(int64_t)(32 * i) * a.xs_row + s * a.xs_group] : 0.0f;
-                }
-                if (!__all_sync(0xffffffffu, mb_mbar_wait_spin(&sc_empty[slot.slot], slot.empty_parity(), status,
-                                                              abort_flag)))
-                    break;
-                float* dst = sc + slot.slot * kUnit * scw + scale_pos(lane);
-#pragma unroll
-                for (int i = 0; i < NL; ++i) {
-                    if (32 * i >= un.w.nrows) break;
-#pragma unroll
-                    for (int s = 0; s < kUnit; ++s) {
-                        dst[s * scw + 32 * i] = v[i][s] * w0[s];
-                        if (DUAL) dst[s * scw + a.acc_cols + 32 * i] = v[i][s] * w1[s];
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) mb_mbar_arrive(&sc_full[slot.slot]);
-                un.next();
-                un.next();
-                slot.next();
-                slot.next();
-            }
-        }
-    } else {
+    } else if (warp >= kEpiWarp) {
         // ------------------------------------------------------------------ epilogue
         setmaxnreg_inc<kEpiRegs>();
-        const int set = (warp - kEpiWarp) >> 2;
-        if (set < sets) {
-            Epilogue ep{a, status, abort_flag, tmem + ((uint32_t)(32 * (warp & 3)) << 16), acc_full, acc_empty,
-                        sc_full, sc_empty, sc, red, red_full, red_empty, amax, tsc,
-                        tiles + set * tile_rows(OUT) * tile_pitch(OUT), k0, k1, split, srank, leader,
-                        warp & 3, set, lane, Ring(a.nacc), Ring(kScSlots), 0, 0};
-            while (w.next()) {
-                const int nch = (w.nrows + 31) >> 5;       // chunks of 32 rows; this set takes set, set + 2, ..
-                const int mine = (nch - set + 1) >> 1;
-                if (mine == 0)
-                    ep.item<TYPE, DUAL, OUT, 0>(w);
-                else if (mine == 1)
-                    ep.item<TYPE, DUAL, OUT, 1>(w);
-                else if (mine == 2)
-                    ep.item<TYPE, DUAL, OUT, 2>(w);
-                else if constexpr (!DUAL) {
-                    if (mine == 3)
-                        ep.item<TYPE, DUAL, OUT, 3>(w);
-                    else
-                        ep.item<TYPE, DUAL, OUT, 4>(w);
-                }
-            }
-            bulk_wait();
-        }
+        const int q = warp & 3, set = (warp - kEpiWarp) >> 2;
+        Epi ep{a, status, abort_flag, tmem + ((uint32_t)(32 * q) << 16), acc_full, acc_empty, red, red_full, red_empty,
+               amax, runs + (warp - kEpiWarp) * 32 * kPitch, split, srank, cluster_rank() - srank, q, set, lane,
+               Ring(kAcc), 0, 0, {}, {}};
+        Units ahead(w, k0, k1);
+        ep.load_scales(ahead);
+        while (w.next()) ep.item(w, ahead, k0, k1);
     }
 
     tc_before();
@@ -805,12 +673,12 @@ int make_maps(const GroupedArgs& a, int type, int halves, Maps* m, const char* w
     const cuuint64_t wd[3] = {(cuuint64_t)a.K, (cuuint64_t)a.O * halves, (cuuint64_t)a.E};
     const cuuint64_t wst[2] = {(cuuint64_t)a.ldw * b,
                                (cuuint64_t)(a.E > 1 ? a.w_expert : (int64_t)a.O * halves * a.ldw) * b};
-    const cuuint32_t wbox[3] = {inner, kBM, 1};
+    const cuuint32_t wbox[3] = {inner, kBlock, 1};
     CUresult r = fn(&m->w, map_type(type), 3, const_cast<void*>(a.w), wd, wst, wbox, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     const cuuint64_t xd[2] = {(cuuint64_t)a.K, (cuuint64_t)a.P};
     const cuuint64_t xst[1] = {(cuuint64_t)a.ldx * b};
-    for (int i = 0; i < kRowMaps && (16 << i) <= a.NT && r == CUDA_SUCCESS; ++i) {
+    for (int i = 0; i < kRowMaps && (16 << i) <= a.MT && r == CUDA_SUCCESS; ++i) {
         const cuuint32_t xbox[2] = {inner, (cuuint32_t)(16 << i)};
         r = fn(&m->x[i], map_type(type), 2, const_cast<void*>(a.x), xd, xst, xbox, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -826,43 +694,32 @@ int pow2_at_least(int64_t n, int lo, int hi)
     return p;
 }
 
-template <int TYPE, bool DUAL, int OUT>
+template <int TYPE, bool DUAL, bool WIDE, int OUT>
 int launch(GroupedArgs a, const char* what, cudaStream_t st)
 {
     constexpr bool FP8 = TYPE == MB_T_E4M3;
-    constexpr int H = DUAL ? 2 : 1;
+    constexpr int N = WIDE ? 256 : 128;
     const int sms = mb_num_sms();
-    a.Kb = (a.K + (FP8 ? 127 : 63)) / (FP8 ? 128 : 64);
-    a.Mb = (a.O + kBM - 1) / kBM;
-    const int maxn = DUAL ? kMaxN / 2 : kMaxN;
     const int64_t active = std::min<int64_t>(a.E, a.P);          // experts with rows, at most
-    if (a.offsets) {
-        a.NT = pow2_at_least((a.P * 3 / 2 + a.E - 1) / a.E, 16, maxn);
-    } else {
-        a.NT = pow2_at_least(a.P, 16, maxn);
-        while (a.NT > 32 && a.Mb * ((a.P + a.NT - 1) / a.NT) < sms) a.NT >>= 1;
-    }
-    const int64_t items = (int64_t)a.Mb * (active + a.P / a.NT);   // an upper bound
-    MB_REQUIRE(items < (1ll << 30), "%s: %lld work items", what, (long long)items);
-    int cluster = 1;
-    if (a.NT <= 32 && a.Mb * active < 4 * sms)
-        while (cluster < 8 && cluster * 2 <= a.Kb && (2 * cluster - 1) * H * a.NT * 512 <= kMaxRed &&
-               a.Mb * active * cluster < 4 * sms)
-            cluster *= 2;
-    a.acc_cols = std::max(32, a.NT);
-    a.nacc = std::min(kMaxAcc, kTmemCols / (H * a.acc_cols));
+    a.Kb = (a.K + (FP8 ? 127 : 63)) / (FP8 ? 128 : 64);
+    a.Nb = DUAL ? (a.O + kBlock - 1) / kBlock : (a.O + N - 1) / N;
     a.prom = FP8 ? 1 : OUT == MB_T_F32 ? 4 : a.Kb;
     a.vec = ((uintptr_t)a.y & 15) == 0 && a.ldy * out_bytes(OUT) % 16 == 0;
-    const int stage = H * kTileA + a.NT * 128;
-    const int scales = FP8 ? kScSlots * kUnit * H * a.acc_cols * 4 : 0;
-    const int encode = OUT == MB_T_E4M3 ? 2 * 2 * 4 * 32 * 4 + kEpiWarps * 64 * 4 : 0;
-    const int tiles = (a.NT > 32 ? 2 : 1) * tile_rows(OUT) * tile_pitch(OUT);
-    const int fixed = 1024 + (cluster - 1) * H * a.NT * 512 + scales + encode + tiles +
-                      (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2) * 8 + 8 + 64 + a.E * 8 + (a.E + 1) * 4 + 16;
+    const int64_t items = a.Nb * (active + a.P / a.MT);            // an upper bound
+    MB_REQUIRE(items < (1ll << 30), "%s: %lld work items", what, (long long)items);
+    int cluster = 1;
+    if (a.MT <= kSplitRows)
+        while (cluster < 8 && cluster * 2 <= a.Kb && (2 * cluster - 1) * N * 128 <= kMaxRed &&
+               a.Nb * active * cluster < 4 * sms)
+            cluster *= 2;
+    const int stage = a.MT * 128 + N * 128;
+    const int fixed = 1024 + (cluster - 1) * N * 128 + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM * 4 : 0) +
+                      kEpiWarps * 32 * kPitch + (2 * kMaxStages + 2 * kMaxAcc + 2) * 8 + 8 + 64 + a.E * 8 +
+                      (a.E + 1) * 4 + 16;
     a.stages = std::min(kMaxStages, (kMaxSmem - fixed) / stage);
     const int smem = fixed + a.stages * stage;
 
-    auto kern = grouped_kernel<TYPE, DUAL, OUT>;
+    auto kern = grouped_kernel<TYPE, DUAL, WIDE, OUT>;
     static thread_local uint64_t ready = 0;                        // devices whose attribute is set
     int dev = 0;
     cudaGetDevice(&dev);
@@ -899,22 +756,43 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     }
     cfg.gridDim = (unsigned)std::min<int64_t>(ctas, items * cluster);
     Maps maps;
-    const int rc = make_maps(a, TYPE, H, &maps, what);
+    const int rc = make_maps(a, TYPE, DUAL ? 2 : 1, &maps, what);
     if (rc) return rc;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, maps);
     if (e != cudaSuccess) return mb_fail(MB_ECUDA, "%s: %s", what, cudaGetErrorString(e));
     return MB_OK;
 }
 
+// Rows per pass: half as many again as an expert has on average (loads differ), as a power of two.
+int pass_rows(const GroupedArgs& a)
+{
+    return pow2_at_least(a.offsets ? (a.P * 3 / 2 + a.E - 1) / a.E : a.P, 16, kMaxM);
+}
+
+// Blocks of 256 weight rows where that still gives every SM an item, else of 128: the wider items move fewer bytes of x
+// per product, the narrower ones spread small calls over more SMs.
+bool wide(const GroupedArgs& a)
+{
+    const int64_t active = std::min<int64_t>(a.E, a.P);
+    return a.MT > kSplitRows && (a.O + 255) / 256 * (active + a.P / a.MT) >= mb_num_sms();
+}
+
+template <int TYPE, int OUT>
+int launch_width(GroupedArgs a, const char* what, cudaStream_t st)
+{
+    a.MT = pass_rows(a);
+    return wide(a) ? launch<TYPE, false, true, OUT>(a, what, st) : launch<TYPE, false, false, OUT>(a, what, st);
+}
+
 template <int TYPE>
 int launch_as(const GroupedArgs& a, int y_type, const char* what, cudaStream_t st)
 {
-    if (y_type == MB_T_F32) return launch<TYPE, false, MB_T_F32>(a, what, st);
-    if (y_type == MB_T_BF16) return launch<TYPE, false, MB_T_BF16>(a, what, st);
-    return launch<TYPE, false, MB_T_F16>(a, what, st);
+    if (y_type == MB_T_F32) return launch_width<TYPE, MB_T_F32>(a, what, st);
+    if (y_type == MB_T_BF16) return launch_width<TYPE, MB_T_BF16>(a, what, st);
+    return launch_width<TYPE, MB_T_F16>(a, what, st);
 }
 
-int matmul(GroupedArgs a, int type, int y_type, const char* what, void* stream)
+int matmul(const GroupedArgs& a, int type, int y_type, const char* what, void* stream)
 {
     MB_REQUIRE(y_type == MB_T_F32 || y_type == MB_T_BF16 || y_type == MB_T_F16, "%s: result type %d", what, y_type);
     const int rc = check_args(a, type, 1, what);
@@ -954,13 +832,14 @@ extern "C" int mb_grouped_swiglu_t(const void* x, int type, int64_t ldx, const f
 {
     const char* what = "mb_grouped_swiglu_t";
     MB_REQUIRE(offsets || P == 0, "%s: null pointer", what);
-    const GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K,
-                        offsets, q, ldq, qs, qs_row, qs_group, status};
+    GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K,
+                  offsets, q, ldq, qs, qs_row, qs_group, status};
     int rc = check_args(a, type, 2, what);
     if (rc || P == 0) return rc;
     MB_REQUIRE(type != MB_T_E4M3 || qs, "%s: e4m3 results need their scales", what);
     const cudaStream_t st = mb_stream(stream);
-    if (type == MB_T_E4M3) return launch<MB_T_E4M3, true, MB_T_E4M3>(a, what, st);
-    if (type == MB_T_BF16) return launch<MB_T_BF16, true, MB_T_BF16>(a, what, st);
-    return launch<MB_T_F16, true, MB_T_F16>(a, what, st);
+    a.MT = pass_rows(a);
+    if (type == MB_T_E4M3) return launch<MB_T_E4M3, true, true, MB_T_E4M3>(a, what, st);
+    if (type == MB_T_BF16) return launch<MB_T_BF16, true, true, MB_T_BF16>(a, what, st);
+    return launch<MB_T_F16, true, true, MB_T_F16>(a, what, st);
 }

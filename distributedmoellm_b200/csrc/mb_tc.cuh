@@ -54,25 +54,27 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar)
                  : "memory");
 }
 
-// 32 consecutive f32 columns of the 32 TMEM lanes at taddr, complete after tc_wait_ld().  v[16 h + 4 b + 2 s + e] of
-// lane l: TMEM lane 16 h + 8 s + l / 4, column 8 b + 2 (l % 4) + e (the fragment of 16 lanes x 256 bits, for both halves of
-// the lanes), so a thread meets 8 of the 32 columns, not all.
-__device__ __forceinline__ void tc_ld_half(uint32_t taddr, float* v)
+// 16 consecutive f32 columns of this thread's TMEM lane (one of the 32 lanes at taddr); the values are there after
+// tc_wait_ld on them, which is an operand of that wait so that no use can move in front of it.
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, float (&v)[16])
 {
     uint32_t* u = reinterpret_cast<uint32_t*>(v);
     asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
           "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32])
+__device__ __forceinline__ void tc_wait_ld(float (&v)[16])
 {
-    tc_ld_half(taddr, v);
-    tc_ld_half(taddr + (16u << 16), v + 16);
+    uint32_t* u = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]),
+                   "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15])
+                 :
+                 : "memory");
 }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Shared-memory descriptor of a K-major tile with 128-byte swizzle: rows 128 bytes apart, 8-row groups 1024.
 __device__ __forceinline__ uint64_t tc_desc_sw128(uint32_t saddr)
@@ -104,20 +106,6 @@ __device__ __forceinline__ void tma_load3(void* dst, const CUtensorMap* map, int
         : "memory");
 }
 
-// Shared -> global copies of whole rows in the background (both addresses 16-byte aligned, bytes a multiple of 16): the
-// writers of the shared rows fence, then (after a barrier) the issuing thread copies, commits, and waits for its copies to
-// have read shared memory before that is written again.
-__device__ __forceinline__ void bulk_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t bytes)
-{
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(mb_smem_addr(src)),
-                 "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
 // ---- thread-block clusters -------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t cluster_size()
@@ -143,9 +131,10 @@ __device__ __forceinline__ uint32_t cluster_map(uint32_t local, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void cluster_st(uint32_t addr, uint64_t v)
+__device__ __forceinline__ void cluster_st4(uint32_t addr, float a, float b, float c, float d)
 {
-    asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
+                 : "memory");
 }
 // Arrival on another CTA's mbarrier, after which that CTA's waiters see this thread's earlier stores.
 __device__ __forceinline__ void cluster_arrive(uint32_t bar_addr)
