@@ -24,6 +24,8 @@
 //    all of K; with f32 results they start afresh every 256 columns: the tensor
 //    cores' f32 sums are cut rather than rounded, which over 2048 columns
 //    came to 2.1e-6 of the result (f32 itself: 1e-7);
+//  * warp 2 finds the items; warp 3 (e4m3) brings the scales of four steps at a
+//    time into shared memory;
 //  * warps 4..11: two sets of four (one warp per TMEM lane quarter), each with
 //    half of the columns: sums (e4m3: times their scale) into f32 registers
 //    while the next columns of K are multiplied, then the results, through
@@ -49,13 +51,16 @@ constexpr int kWarps = 12;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kEpiWarp = 4;               // first of the eight epilogue warps
 // Registers: 168 a thread at launch; the epilogue warpgroups (up to 128 sums a thread) take theirs from the first
-// warpgroup: 128 * 56 + 256 * 224 = 64512 = the launch's 384 * 168.
-constexpr int kLoadRegs = 56, kEpiRegs = 224;
+// warpgroup: 128 * 72 + 256 * 216 = 64512 = the launch's 384 * 168.
+constexpr int kLoadRegs = 72, kEpiRegs = 216;
 constexpr int kEpiWarps = 8;
 constexpr int kBlock = 128;               // weight rows of a block
 constexpr int kTileW = kBlock * 128;      // bytes of a block's tile: 128 rows of 128 bytes
 constexpr int kMaxM = 128;                // rows of x per pass
-constexpr int kUnit = 4;                  // K steps whose scales a thread loads together, one such unit ahead
+constexpr int kUnit = 4;                  // K steps whose scales are handed over together
+constexpr int kScSlots = 3;               // ring of such units
+constexpr int kScFloats = kUnit * (128 + 2);   // of each step: xs of the pass's rows, ws of the item's (up to) two blocks
+constexpr int kItemSlots = 4;
 constexpr int kMaxAcc = 4;
 constexpr int kMaxStages = 16;
 constexpr int kTmemCols = 512;
@@ -96,20 +101,22 @@ struct Maps {
     CUtensorMap x[kRowMaps];
 };
 
-// The items of this CTA (of its group of `split` CTAs, when items are split over K).
-struct Items {
+// A work item: expert, block of weight rows, first row of x and how many (none: no more items).
+struct Item {
+    int e, nb, row0, nrows;
+};
+
+// The items of this CTA (of its group of `split` CTAs, when items are split over K) in order.  Finding one takes a search
+// and divisions, so one warp does it and hands the items on.
+struct Finder {
     const GroupedArgs& a;
     const int2* meta;          // (first row, rows) of each expert
     const int* pstart;         // first item of each expert; [E]: all items
-    int it, step, e, nb, row0, nrows;
-    __device__ Items(const GroupedArgs& args, const int2* m, const int* ps, int first, int by)
-        : a(args), meta(m), pstart(ps), it(first - by), step(by), e(0)
-    {
-    }
-    __device__ bool next()
+    int it, step, e;
+    __device__ Item next()
     {
         it += step;
-        if (it >= pstart[a.E]) return false;
+        if (it >= pstart[a.E]) return {0, 0, 0, 0};
         if (it >= pstart[e + 1]) {         // the last e with pstart[e] <= it (experts without rows have none)
             int lo = e + 1, hi = a.E;
             while (hi - lo > 1) {
@@ -124,30 +131,29 @@ struct Items {
         const int2 m = meta[e];
         const int passes = (m.y + a.MT - 1) / a.MT;
         const int local = it - pstart[e];
-        nb = local / passes;
-        const int pass = local - nb * passes;
+        const int nb = local / passes, pass = local - nb * passes;
         const int size = ((m.y + passes - 1) / passes + 15) & ~15;     // passes of about equal size
-        row0 = m.x + pass * size;
-        nrows = min(size, m.y - pass * size);
-        return true;
+        return {e, nb, m.x + pass * size, min(size, m.y - pass * size)};
     }
 };
 
-// The K steps k0 .. k1 - 1 of one item after another, kUnit at a time.
-struct Units {
-    Items w;
-    int k0, k1, kb;
-    bool live;
-    __device__ Units(const Items& items, int first, int last) : w(items), k0(first), k1(last), kb(first)
+// Where the other roles take the items from.
+struct ItemRing {
+    const Item* slots;
+    uint64_t *full, *empty;
+    unsigned* status;
+    volatile int* abort_flag;
+    Ring r;
+    // The next item (of a whole warp, or of one thread alone); false when there is none.
+    template <bool WARP>
+    __device__ __forceinline__ bool pop(Item& v)
     {
-        live = w.next();
-    }
-    __device__ void next()
-    {
-        if (live && (kb += kUnit) >= k1) {
-            live = w.next();
-            kb = k0;
-        }
+        if (!mb_mbar_wait_spin(&full[r.slot], r.full_parity(), status, abort_flag)) return false;
+        v = slots[r.slot];
+        if (WARP) __syncwarp();
+        if (!WARP || (threadIdx.x & 31) == 0) mb_mbar_arrive(&empty[r.slot]);
+        r.next();
+        return v.nrows > 0;
     }
 };
 
@@ -179,7 +185,8 @@ struct Epilogue {
     unsigned* status;
     volatile int* abort_flag;
     uint32_t tl;               // TMEM address of the warp's lane quarter
-    uint64_t *acc_full, *acc_empty;
+    uint64_t *acc_full, *acc_empty, *sc_full, *sc_empty;
+    const float* sc;
     float4* red;               // partial sums: [sender][set][S / 4][32 lanes]
     uint64_t *red_full, *red_empty;
     float* amax;               // [2][2 sets][128 rows]
@@ -187,9 +194,8 @@ struct Epilogue {
     int split, srank;
     uint32_t leader;
     int q, set, lane;
-    Ring ac;
+    Ring ac, scr;
     int sent, abuf;
-    float xr[kUnit], wr[H][kUnit];                         // the next unit's scales, on their way
 
     // Accumulator column of this thread's chunk c.  Gate|up: its first half of chunks are gate columns, then the up
     // columns of the same place.
@@ -199,25 +205,8 @@ struct Epilogue {
         return S * set + 16 * c;
     }
 
-    __device__ __forceinline__ void load_scales(const Units& un)
-    {
-        if (!FP8 || !un.live) return;
-        const int Ob = (a.O + kScaleBlock - 1) / kScaleBlock;
-        const int block = DUAL ? un.w.nb : WIDE ? min(2 * un.w.nb + set, Ob - 1) : un.w.nb;
-        const int r = 32 * q + lane;
-        const float* xp = a.xs + (int64_t)(un.w.row0 + min(r, un.w.nrows - 1)) * a.xs_row + (int64_t)un.kb * a.xs_group;
-        const float* wp = a.ws + ((int64_t)un.w.e * H * Ob + block) * a.Kb + un.kb;
-#pragma unroll
-        for (int s = 0; s < kUnit; ++s) {
-            const bool real = un.kb + s < un.k1;
-            xr[s] = real ? __ldg(xp + s * a.xs_group) : 0.0f;
-#pragma unroll
-            for (int h = 0; h < H; ++h) wr[h][s] = real ? __ldg(wp + (int64_t)h * Ob * a.Kb + s) : 0.0f;
-        }
-    }
-
-    // One item's K steps k0 .. k1 - 1 and its results; `ahead` is this item's first unit, whose scales are loading.
-    __device__ __forceinline__ void item(const Items& w, Units& ahead, int k0, int k1)
+    // One item's K steps k0 .. k1 - 1 and its results.
+    __device__ __forceinline__ void item(const Item& w, int k0, int k1)
     {
         const bool rows = 32 * q < w.nrows;                // this quarter has some
         bool ok = true;
@@ -226,15 +215,15 @@ struct Epilogue {
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sum[c][i] = 0.0f;
-        float sc[H][kUnit];
-        for (int kb = k0, us = 0; kb < k1; kb += a.prom, us = (us + 1) % kUnit) {
-            if (FP8 && us == 0) {
-#pragma unroll
-                for (int s = 0; s < kUnit; ++s)
-#pragma unroll
-                    for (int h = 0; h < H; ++h) sc[h][s] = xr[s] * wr[h][s];
-                ahead.next();
-                load_scales(ahead);
+        for (int kb = k0, us = 0; kb < k1; kb += a.prom) {
+            float s[H];
+            if (FP8) {
+                if (us == 0) ok = mb_mbar_wait_spin(&sc_full[scr.slot], scr.full_parity(), status, abort_flag) && ok;
+                const float* from = sc + scr.slot * kScFloats + us * 130;
+                const float x = from[32 * q + lane];
+                const float2 b = *reinterpret_cast<const float2*>(from + 128);
+                s[0] = x * (!DUAL && WIDE && set ? b.y : b.x);
+                if (DUAL) s[H - 1] = x * b.y;
             }
             ok = mb_mbar_wait_spin(&acc_full[ac.slot], ac.full_parity(), status, abort_flag) && ok;
             tc_after();
@@ -246,21 +235,23 @@ struct Epilogue {
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     if (c + 1 < C) tc_ld16(from + column(c + 1), d[(c + 1) & 1]);
-                    const float s = sc[DUAL && c >= C / 2 ? H - 1 : 0][0];
+                    const float f = s[DUAL && c >= C / 2 ? H - 1 : 0];
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        sum[c][i] = FP8 ? fmaf(d[c & 1][i], s, sum[c][i]) : sum[c][i] + d[c & 1][i];
+                        sum[c][i] = FP8 ? fmaf(d[c & 1][i], f, sum[c][i]) : sum[c][i] + d[c & 1][i];
                     if (c + 1 < C) tc_wait_ld(d[(c + 1) & 1]);
                 }
             }
-#pragma unroll
-            for (int h = 0; h < H; ++h)                    // the unit's next step
-#pragma unroll
-                for (int s = 0; s + 1 < kUnit; ++s) sc[h][s] = sc[h][s + 1];
+            const bool unit_done = FP8 && (us == kUnit - 1 || kb + 1 == k1);
+            us = unit_done ? 0 : us + 1;
             tc_before();
             __syncwarp();
-            if (lane == 0) mb_mbar_arrive(&acc_empty[ac.slot]);
+            if (lane == 0) {
+                mb_mbar_arrive(&acc_empty[ac.slot]);
+                if (unit_done) mb_mbar_arrive(&sc_empty[scr.slot]);
+            }
             ac.next();
+            if (unit_done) scr.next();
         }
 
         if (split > 1) {
@@ -426,14 +417,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* stage0 = smem;
     float4* red = reinterpret_cast<float4*>(stage0 + (size_t)a.stages * stage_bytes);
     float* amax = reinterpret_cast<float*>(red + (csize - 1) * Epi::N / 4 * 32);
-    uint8_t* runs = reinterpret_cast<uint8_t*>(amax + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM : 0));
+    float* sc = amax + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM : 0);
+    uint8_t* runs = reinterpret_cast<uint8_t*>(sc + (FP8 ? kScSlots * kScFloats : 0));
     uint64_t* full = reinterpret_cast<uint64_t*>(runs + kEpiWarps * 32 * kPitch);
     uint64_t* empty = full + kMaxStages;
     uint64_t* acc_full = empty + kMaxStages;
     uint64_t* acc_empty = acc_full + kMaxAcc;
-    uint64_t* red_full = acc_empty + kMaxAcc;
+    uint64_t* sc_full = acc_empty + kMaxAcc;
+    uint64_t* sc_empty = sc_full + kScSlots;
+    uint64_t* item_full = sc_empty + kScSlots;
+    uint64_t* item_empty = item_full + kItemSlots;
+    uint64_t* red_full = item_empty + kItemSlots;
     uint64_t* red_empty = red_full + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_empty + 1);
+    Item* items = reinterpret_cast<Item*>(red_empty + 1);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kItemSlots);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [kWarps], [15]: split
     int2* meta = reinterpret_cast<int2*>(wsum + 16);                   // [E]
@@ -452,6 +449,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             mb_mbar_init(&acc_full[i], 1);
             mb_mbar_init(&acc_empty[i], kEpiWarps);
         }
+        for (int i = 0; i < kScSlots; ++i) {
+            mb_mbar_init(&sc_full[i], 1);
+            mb_mbar_init(&sc_empty[i], kEpiWarps);
+        }
+        for (int i = 0; i < kItemSlots; ++i) {
+            mb_mbar_init(&item_full[i], 1);
+            mb_mbar_init(&item_empty[i], kEpiWarps + (FP8 ? 3 : 2));
+        }
         *abort_flag = 0;
         tma_prefetch_map(&maps.w);
     }
@@ -462,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     {
         const int per = (a.E + kThreads - 1) / kThreads;
         const int e0 = min(a.E, (int)threadIdx.x * per), e1 = min(a.E, e0 + per);
-        int items = 0;
+        int mine = 0;
         for (int e = e0; e < e1; ++e) {
             int lo = 0, n = (int)a.P;
             if (a.offsets) {
@@ -475,10 +480,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             meta[e] = make_int2(lo, n);
-            pstart[e] = items;
-            items += a.Nb * ((n + a.MT - 1) / a.MT);
+            pstart[e] = mine;
+            mine += a.Nb * ((n + a.MT - 1) / a.MT);
         }
-        int run = items;
+        int run = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int t = __shfl_up_sync(0xffffffffu, run, o);
@@ -486,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (lane == 31) wsum[warp] = run;
         __syncthreads();
-        int before = run - items, total = 0;
+        int before = run - mine, total = 0;
         for (int w = 0; w < kWarps; ++w) {
             const int s = wsum[w];
             if (w < warp) before += s;
@@ -522,7 +527,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int split = wsum[15];
     const int srank = (int)blockIdx.x % split;                          // rank among the CTAs of an item
     const int k0 = (int)((int64_t)a.Kb * srank / split), k1 = (int)((int64_t)a.Kb * (srank + 1) / split);
-    Items w(a, meta, pstart, blockIdx.x / split, gridDim.x / split);
+    ItemRing ring{items, item_full, item_empty, status, abort_flag, Ring(kItemSlots)};
+    Item w;
 
     if (warp < kEpiWarp) setmaxnreg_dec<kLoadRegs>();
     if (warp == 0) {
@@ -530,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         Ring st(a.stages);
         bool ok = true;
         int issued = 0;
-        while (ok && w.next()) {
+        while (ok && ring.pop<true>(w)) {
             const int r16 = (w.nrows + 15) >> 4;
             // lanes 0, 1: weight tiles; lane 2 + b: a box of 16 << b rows, the larger boxes first
             const int b = lane - 2;
@@ -550,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ++issued;
             }
         }
-        if (!ok) {   // wait (bounded) for the copies still in flight before the CTA may end
+        if (!ok || *abort_flag) {   // wait (bounded) for the copies still in flight before the CTA may end
             for (int i = 0; i < min(issued, a.stages); ++i) {
                 if (--st.slot < 0) {
                     st.slot = a.stages - 1;
@@ -569,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr uint32_t idesc = (1u << 4) | (TYPE == MB_T_BF16 ? (1u << 7) | (1u << 10) : 0u) |
                                        ((uint32_t)(Epi::N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             const uint64_t desc0 = tc_desc_sw128(mb_smem_addr(stage0));
-            while (ok && w.next()) {
+            while (ok && ring.pop<false>(w)) {
                 int part = 0;                              // K steps already in the accumulator
                 for (int kb = k0; kb < k1; ++kb, st.next()) {
                     if (part == 0)
@@ -593,16 +599,69 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp >= kEpiWarp) {
+    } else if (warp == 2) {
+        // ------------------------------------------------------------------ items
+        Finder find{a, meta, pstart, (int)blockIdx.x / split - (int)gridDim.x / split, (int)gridDim.x / split, 0};
+        Ring r(kItemSlots);
+        for (bool more = true; more; r.next()) {
+            const Item v = find.next();
+            more = v.nrows > 0;
+            if (!__all_sync(0xffffffffu, mb_mbar_wait_spin(&item_empty[r.slot], r.empty_parity(), status, abort_flag)))
+                break;
+            if (lane == 0) {
+                items[r.slot] = v;
+                mb_mbar_arrive(&item_full[r.slot]);
+            }
+        }
+    } else if (warp == 3) {
+        // ------------------------------------------------------------------ scales
+        if (FP8) {
+            const int Ob = (a.O + kScaleBlock - 1) / kScaleBlock;
+            Ring slot(kScSlots);
+            bool ok = true;
+            while (ok && ring.pop<true>(w)) {
+                // lanes 0, 1: the item's two blocks of weight rows (the last item of an odd count has one)
+                const int block = DUAL ? (w.e * 2 + (lane & 1)) * Ob + w.nb
+                                       : w.e * Ob + min(NB * w.nb + (WIDE ? lane & 1 : 0), Ob - 1);
+                const float* wsp = a.ws + (int64_t)block * a.Kb;
+                const float* xsp = a.xs + ((int64_t)w.row0 + lane) * a.xs_row;
+                for (int kb = k0; kb < k1; kb += kUnit) {
+                    float v[kUnit][4], b[kUnit];
+#pragma unroll
+                    for (int s = 0; s < kUnit; ++s) {
+                        const bool real = kb + s < k1;
+                        b[s] = real ? wsp[kb + s] : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            v[s][i] = real && lane + 32 * i < w.nrows
+                                          ? xsp[(int64_t)(32 * i) * a.xs_row + (int64_t)(kb + s) * a.xs_group]
+                                          : 0.0f;
+                    }
+                    ok = __all_sync(0xffffffffu, mb_mbar_wait_spin(&sc_empty[slot.slot], slot.empty_parity(), status,
+                                                                  abort_flag));
+                    if (!ok) break;
+                    float* dst = sc + slot.slot * kScFloats;
+#pragma unroll
+                    for (int s = 0; s < kUnit; ++s) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (32 * i < w.nrows) dst[s * 130 + lane + 32 * i] = v[s][i];
+                        if (lane < 2) dst[s * 130 + 128 + lane] = b[s];
+                    }
+                    __syncwarp();
+                    if (lane == 0) mb_mbar_arrive(&sc_full[slot.slot]);
+                    slot.next();
+                }
+            }
+        }
+    } else {
         // ------------------------------------------------------------------ epilogue
         setmaxnreg_inc<kEpiRegs>();
         const int q = warp & 3, set = (warp - kEpiWarp) >> 2;
-        Epi ep{a, status, abort_flag, tmem + ((uint32_t)(32 * q) << 16), acc_full, acc_empty, red, red_full, red_empty,
-               amax, runs + (warp - kEpiWarp) * 32 * kPitch, split, srank, cluster_rank() - srank, q, set, lane,
-               Ring(kAcc), 0, 0, {}, {}};
-        Units ahead(w, k0, k1);
-        ep.load_scales(ahead);
-        while (w.next()) ep.item(w, ahead, k0, k1);
+        Epi ep{a, status, abort_flag, tmem + ((uint32_t)(32 * q) << 16), acc_full, acc_empty, sc_full, sc_empty, sc, red,
+               red_full, red_empty, amax, runs + (warp - kEpiWarp) * 32 * kPitch, split, srank, cluster_rank() - srank,
+               q, set, lane, Ring(kAcc), Ring(kScSlots), 0, 0};
+        while (ring.pop<true>(w)) ep.item(w, k0, k1);
     }
 
     tc_before();
@@ -714,8 +773,9 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
             cluster *= 2;
     const int stage = a.MT * 128 + N * 128;
     const int fixed = 1024 + (cluster - 1) * N * 128 + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM * 4 : 0) +
-                      kEpiWarps * 32 * kPitch + (2 * kMaxStages + 2 * kMaxAcc + 2) * 8 + 8 + 64 + a.E * 8 +
-                      (a.E + 1) * 4 + 16;
+                      (FP8 ? kScSlots * kScFloats * 4 : 0) + kEpiWarps * 32 * kPitch +
+                      (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2) * 8 + kItemSlots * 16 + 8 + 64 +
+                      a.E * 8 + (a.E + 1) * 4 + 16;
     a.stages = std::min(kMaxStages, (kMaxSmem - fixed) / stage);
     const int smem = fixed + a.stages * stage;
 
