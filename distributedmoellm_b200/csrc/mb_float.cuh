@@ -34,7 +34,7 @@ struct Quotient {
 __device__ __forceinline__ float quotient(float x, float s, float r)
 {
     const float q = x * r;
-    return fmaf(fmaf(-q, s, x), r, q);
+    return copysignf(fmaf(fmaf(-q, s, x), r, q), x);       // the correction would turn -0 into +0
 }
 
 // Nearest e4m3 of two values, as bytes lo, hi.

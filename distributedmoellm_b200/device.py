@@ -337,27 +337,37 @@ OPERAND_TYPES = (torch.float8_e4m3fn, torch.bfloat16, torch.float16)
 RESULT_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
+# Small calls cost what their checks cost on the host: shapes are compared whole, the device is an index, the stream comes
+# as a raw handle, and the messages are put together only when something is wrong.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_fns: dict = {}
+_E4M3 = torch.float8_e4m3fn
+
+
 def _blocks(n: int) -> int:
     return -(-n // SCALE_BLOCK)
 
 
-def _want(t, name, shape, dtypes):
+def _want(t, name, shape, dtype):
     if t is None:
         raise ValueError(f"{name} is missing")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} is {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
+    if t.dtype is not dtype:
+        raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
 
 
 def _rows_of(t, name):
     """Elements between the rows of t (..., rows, columns), whose columns must be adjacent."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"the columns of {name} must be adjacent (strides {t.stride()})")
-    return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], t.stride(-2))
+    st = t.stride()
+    cols = t.shape[-1]
+    if st[-1] != 1 and cols > 1:
+        raise ValueError(f"the columns of {name} must be adjacent (strides {st})")
+    return st[-2] if t.shape[-2] > 1 else max(cols, st[-2])
 
 
-def _row_stride(t, name):
+def _operand_stride(t, name):
     """As :func:`_rows_of`; a single row's distance is rounded up to 16 bytes, since nothing lies behind it."""
     ld = _rows_of(t, name)
     if t.shape[-2] <= 1:
@@ -366,28 +376,44 @@ def _row_stride(t, name):
     return ld
 
 
-def _one_device(*ts):
-    """The device all of ts are on."""
-    dev = None
-    for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
+def _status_ptr(status):
+    if status is None:
+        return None
+    if status.dtype is not torch.int32 or status.numel() != 1:
+        raise ValueError("status must be one int32")
+    return status.data_ptr()
+
+
+def _on(t, *others):
+    """The index of the CUDA device that t and the others (but for None) are on."""
+    dev = t.get_device()
+    if dev < 0:
+        raise RuntimeError("expected CUDA tensors")
+    for o in others:
+        if o is not None and o.get_device() != dev:
+            if o.is_cuda:
+                raise ValueError(f"tensors on different devices ({t.device}, {o.device})")
             raise RuntimeError("expected CUDA tensors")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices ({dev}, {t.device})")
-        dev = t.device
     return dev
 
 
-def _status_word(status):
-    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
-        raise ValueError("status must be one int32")
+def _call(name, dev, *args):
+    """The library's ``name`` on device ``dev``'s current stream, which is the last argument."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(lib(), name)
+    if _current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        check(rc, name)
 
 
-def _new_scales(n: int, groups: int, device):
+def _new_scales(like: torch.Tensor, n: int, groups: int):
     """Scales (n, groups), stored group after group: the products read one group of many rows at a time."""
-    return torch.empty((groups, n), dtype=torch.float32, device=device).t()
+    return torch.empty_strided((n, groups), (1, n), dtype=torch.float32, device=like.device)
 
 
 def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None = None, q: torch.Tensor | None = None,
@@ -403,57 +429,70 @@ def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None 
         raise ValueError(f"operand_rows takes (rows, columns) of f32, bf16 or f16, got {tuple(x.shape)} {x.dtype}")
     if dtype not in OPERAND_TYPES:
         raise ValueError(f"operand type {dtype}, expected one of {', '.join(str(d) for d in OPERAND_TYPES)}")
-    if rows is not None and (rows.dim() != 1 or rows.dtype != torch.int32 or not rows.is_contiguous()):
+    if rows is not None and (rows.dim() != 1 or rows.dtype is not torch.int32 or not rows.is_contiguous()):
         raise ValueError("rows must be a contiguous vector of int32")
     T, d = x.shape
-    n = T if rows is None else rows.numel()
-    e4m3 = dtype == torch.float8_e4m3fn
+    n = T if rows is None else rows.shape[0]
     if q is not None:
-        _want(q, "q", (n, d), (dtype,))
-        _rows_of(q, "q")
+        _want(q, "q", (n, d), dtype)
     if scales is not None:
-        if not e4m3:
+        if dtype is not _E4M3:
             raise ValueError(f"{dtype} rows have no scales")
-        _want(scales, "scales", (n, _blocks(d)), (torch.float32,))
-    _rows_of(x, "x")
-    _status_word(status)
-    dev = _one_device(x, rows, q, scales, status)
-    with torch.cuda.device(dev):
-        q = torch.empty((n, d), dtype=dtype, device=dev) if q is None else q
-        if e4m3 and scales is None:
-            scales = _new_scales(n, _blocks(d), dev)
-        sr, sg = scales.stride() if e4m3 else (0, 0)
-        check(lib().mb_operand_rows(_p(x), _TYPES[x.dtype], _rows_of(x, "x"), T, _p(rows), n, d, _TYPES[dtype],
-                                    _p(q), _rows_of(q, "q"), _p(scales), sr, sg, _p(status), _stream()),
-              "mb_operand_rows")
+        _want(scales, "scales", (n, _blocks(d)), torch.float32)
+    ldx = _rows_of(x, "x")
+    st = _status_ptr(status)
+    dev = _on(x, rows, q, scales, status)
+    if q is None:
+        q = x.new_empty((n, d), dtype=dtype)
+    s, sr, sg = None, 0, 0
+    if dtype is _E4M3:
+        scales = _new_scales(x, n, _blocks(d)) if scales is None else scales
+        s, (sr, sg) = scales.data_ptr(), scales.stride()
+    _call("mb_operand_rows", dev, x.data_ptr(), _TYPES[x.dtype], ldx, T, None if rows is None else rows.data_ptr(), n, d,
+          _TYPES[dtype], q.data_ptr(), _rows_of(q, "q"), s, sr, sg, st)
     return q, scales
 
 
 def _operands(x, w, xs, ws, ws_shape):
-    """Checks of a product's rows x (P, K) and matrices w (..., O, K) with their scales."""
+    """Checks of a product's rows x (P, K) and matrices w (..., O, K) with their scales; the scales' addresses and the
+    strides of xs."""
     if x.dim() != 2 or x.dtype not in OPERAND_TYPES:
         raise ValueError(f"rows must be (P, K) of e4m3, bf16 or f16, got {tuple(x.shape)} {x.dtype}")
-    if w.dtype != x.dtype:
+    if w.dtype is not x.dtype:
         raise ValueError(f"rows of {x.dtype} with weights of {w.dtype}")
-    if w.shape[-1] != x.shape[1]:
-        raise ValueError(f"rows of {x.shape[1]} columns with weights of {w.shape[-1]}")
-    if x.dtype == torch.float8_e4m3fn:
-        _want(xs, "xs", (x.shape[0], _blocks(x.shape[1])), (torch.float32,))
-        _want(ws, "ws", ws_shape, (torch.float32,))
+    P, K = x.shape
+    if w.shape[-1] != K:
+        raise ValueError(f"rows of {K} columns with weights of {w.shape[-1]}")
+    if x.dtype is _E4M3:
+        _want(xs, "xs", (P, _blocks(K)), torch.float32)
+        _want(ws, "ws", ws_shape, torch.float32)
         if not ws.is_contiguous():
             raise ValueError("ws must be contiguous")
-        return xs.stride()
+        sr, sg = xs.stride()
+        return xs.data_ptr(), sr, sg, ws.data_ptr()
     if xs is not None or ws is not None:
         raise ValueError(f"{x.dtype} operands have no scales")
-    return 0, 0
+    return None, 0, 0, None
 
 
 def _groups(w, offsets):
     if w.dim() != 3:
         raise ValueError(f"weights must be (E, O, K), got {tuple(w.shape)}")
-    _want(offsets, "offsets", (w.shape[0] + 1,), (torch.int32,))
+    _want(offsets, "offsets", (w.shape[0] + 1,), torch.int32)
     if not offsets.is_contiguous():
         raise ValueError("offsets must be contiguous")
+
+
+def _result(x, y, shape, dtype):
+    """A product's result: y, checked, or a new tensor of ``dtype`` (f32 unless said otherwise)."""
+    if dtype is None:
+        dtype = torch.float32 if y is None else y.dtype
+    if dtype not in RESULT_TYPES:
+        raise ValueError(f"result type {dtype}")
+    if y is not None:
+        _want(y, "y", shape, dtype)
+        return y
+    return x.new_empty(shape, dtype=dtype)
 
 
 def matmul_t_e4m3(x: torch.Tensor, xs: torch.Tensor, w: torch.Tensor, ws: torch.Tensor, y: torch.Tensor | None = None,
@@ -465,23 +504,16 @@ def matmul_t_e4m3(x: torch.Tensor, xs: torch.Tensor, w: torch.Tensor, ws: torch.
     a multiple of 16 bytes apart."""
     if w.dim() != 2:
         raise ValueError(f"w must be (O, K), got {tuple(w.shape)}")
-    if x.dtype != torch.float8_e4m3fn:
+    if x.dtype is not _E4M3:
         raise ValueError(f"matmul_t_e4m3 takes rows of e4m3, got {x.dtype}")
-    xr, xg = _operands(x, w, xs, ws, (_blocks(w.shape[0]), _blocks(w.shape[1])))
-    n, O = x.shape[0], w.shape[0]
-    dtype = (torch.float32 if y is None else y.dtype) if dtype is None else dtype
-    if dtype not in RESULT_TYPES:
-        raise ValueError(f"result type {dtype}")
-    if y is not None:
-        _want(y, "y", (n, O), (dtype,))
-        _rows_of(y, "y")
-    ldx, ldw = _row_stride(x, "x"), _row_stride(w, "w")
-    _status_word(status)
-    dev = _one_device(x, xs, w, ws, y, status)
-    with torch.cuda.device(dev):
-        y = torch.empty((n, O), dtype=dtype, device=dev) if y is None else y
-        check(lib().mb_matmul_t_e4m3(_p(x), ldx, _p(xs), xr, xg, n, _p(w), ldw, _p(ws), O, x.shape[1], _p(y),
-                                     _TYPES[dtype], _rows_of(y, "y"), _p(status), _stream()), "mb_matmul_t_e4m3")
+    O, K = w.shape
+    xsp, xr, xg, wsp = _operands(x, w, xs, ws, (_blocks(O), _blocks(K)))
+    n = x.shape[0]
+    y = _result(x, y, (n, O), dtype)
+    ldx, ldw = _operand_stride(x, "x"), _operand_stride(w, "w")
+    dev = _on(x, xs, w, ws, y, status)
+    _call("mb_matmul_t_e4m3", dev, x.data_ptr(), ldx, xsp, xr, xg, n, w.data_ptr(),
+          ldw, wsp, O, K, y.data_ptr(), _TYPES[y.dtype], _rows_of(y, "y"), _status_ptr(status))
     return y
 
 
@@ -497,22 +529,14 @@ def grouped_matmul_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs
     Offsets that decrease or pass P set bit 2 of ``status``."""
     _groups(w, offsets)
     E, O, K = w.shape
-    xr, xg = _operands(x, w, xs, ws, (E, _blocks(O), _blocks(K)))
+    xsp, xr, xg, wsp = _operands(x, w, xs, ws, (E, _blocks(O), _blocks(K)))
     P = x.shape[0]
-    dtype = (torch.float32 if y is None else y.dtype) if dtype is None else dtype
-    if dtype not in RESULT_TYPES:
-        raise ValueError(f"result type {dtype}")
-    if y is not None:
-        _want(y, "y", (P, O), (dtype,))
-        _rows_of(y, "y")
-    ldx, ldw = _row_stride(x, "x"), _row_stride(w, "w")
-    _status_word(status)
-    dev = _one_device(x, w, offsets, xs, ws, y, status)
-    with torch.cuda.device(dev):
-        y = torch.empty((P, O), dtype=dtype, device=dev) if y is None else y
-        check(lib().mb_grouped_matmul_t(_p(x), _TYPES[x.dtype], ldx, _p(xs), xr, xg, P, _p(w), w.stride(0), ldw,
-                                        _p(ws), E, O, K, _p(offsets), _p(y), _TYPES[dtype], _rows_of(y, "y"),
-                                        _p(status), _stream()), "mb_grouped_matmul_t")
+    y = _result(x, y, (P, O), dtype)
+    ldx, ldw = _operand_stride(x, "x"), _operand_stride(w, "w")
+    dev = _on(x, w, offsets, xs, ws, y, status)
+    _call("mb_grouped_matmul_t", dev, x.data_ptr(), _TYPES[x.dtype], ldx, xsp, xr, xg, P,
+          w.data_ptr(), w.stride(0), ldw, wsp, E, O, K, offsets.data_ptr(), y.data_ptr(),
+          _TYPES[y.dtype], _rows_of(y, "y"), _status_ptr(status))
     return y
 
 
@@ -529,27 +553,25 @@ def grouped_swiglu_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs
     if I2 % 2:
         raise ValueError(f"a gate|up matrix has an even number of rows, got {I2}")
     I = I2 // 2
-    e4m3 = x.dtype == torch.float8_e4m3fn
-    xr, xg = _operands(x, w, xs, ws, (E, 2, _blocks(I), _blocks(K)))
+    xsp, xr, xg, wsp = _operands(x, w, xs, ws, (E, 2, _blocks(I), _blocks(K)))
     P = x.shape[0]
     if q is not None:
-        _want(q, "q", (P, I), (x.dtype,))
-        _rows_of(q, "q")
+        _want(q, "q", (P, I), x.dtype)
     if scales is not None:
-        if not e4m3:
+        if x.dtype is not _E4M3:
             raise ValueError(f"{x.dtype} rows have no scales")
-        _want(scales, "scales", (P, _blocks(I)), (torch.float32,))
-    ldx, ldw = _row_stride(x, "x"), _row_stride(w, "w")
-    _status_word(status)
-    dev = _one_device(x, w, offsets, xs, ws, q, scales, status)
-    with torch.cuda.device(dev):
-        q = torch.empty((P, I), dtype=x.dtype, device=dev) if q is None else q
-        if e4m3 and scales is None:
-            scales = _new_scales(P, _blocks(I), dev)
-        sr, sg = scales.stride() if e4m3 else (0, 0)
-        check(lib().mb_grouped_swiglu_t(_p(x), _TYPES[x.dtype], ldx, _p(xs), xr, xg, P, _p(w), w.stride(0), ldw,
-                                        _p(ws), E, I, K, _p(offsets), _p(q), _rows_of(q, "q"), _p(scales), sr, sg,
-                                        _p(status), _stream()), "mb_grouped_swiglu_t")
+        _want(scales, "scales", (P, _blocks(I)), torch.float32)
+    ldx, ldw = _operand_stride(x, "x"), _operand_stride(w, "w")
+    dev = _on(x, w, offsets, xs, ws, q, scales, status)
+    if q is None:
+        q = x.new_empty((P, I))
+    s, sr, sg = None, 0, 0
+    if x.dtype is _E4M3:
+        scales = _new_scales(x, P, _blocks(I)) if scales is None else scales
+        s, (sr, sg) = scales.data_ptr(), scales.stride()
+    _call("mb_grouped_swiglu_t", dev, x.data_ptr(), _TYPES[x.dtype], ldx, xsp, xr, xg, P,
+          w.data_ptr(), w.stride(0), ldw, wsp, E, I, K, offsets.data_ptr(), q.data_ptr(),
+          _rows_of(q, "q"), s, sr, sg, _status_ptr(status))
     return q, scales
 
 
