@@ -30,7 +30,7 @@
 //    half of the columns: sums (e4m3: times their scale) into f32 registers
 //    while the next columns of K are multiplied, then the results, through
 //    shared memory of the warp's own so that they leave as 64-byte runs.  A
-//    quarter without rows is skipped.
+//    quarter without rows is skipped.  (Small passes: see Roles.)
 // Splitting K: with few items a cluster's CTAs take equal shares of one item's
 // groups and send their f32 partial sums through distributed shared memory to
 // the first of them, which adds them in rank order, so results do not depend on
@@ -40,6 +40,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "mb_common.cuh"
 #include "mb_float.cuh"
@@ -47,13 +48,21 @@
 
 namespace {
 
-constexpr int kWarps = 12;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kEpiWarp = 4;               // first of the eight epilogue warps
-// Registers: 168 a thread at launch; the epilogue warpgroups (up to 128 sums a thread) take theirs from the first
-// warpgroup: 128 * 72 + 256 * 216 = 64512 = the launch's 384 * 168.
+// Who does what.  Large passes: one CTA per SM, eight epilogue warps; 168 registers a thread at launch, of which the
+// epilogue warpgroups (up to 128 sums a thread) take their share from the first warpgroup: 128 * 72 + 256 * 216 = 64512 =
+// the launch's 384 * 168.  Small passes (at most 32 rows) use one quarter of the TMEM lanes, which the warps 0 and 4 can
+// read: six warps, half of the shared and the tensor memory, and so two CTAs per SM, one's hand-overs and prologue beside
+// the other's.
+template <bool SMALL>
+struct Roles {
+    static constexpr int kWarps = SMALL ? 6 : 12, kThreads = 32 * kWarps;
+    static constexpr int kEpiWarps = SMALL ? 2 : 8;
+    static constexpr int kLoad = SMALL ? 1 : 0, kMma = SMALL ? 2 : 1, kFind = SMALL ? 3 : 2, kScale = SMALL ? 5 : 3;
+    static constexpr int kTmemCols = SMALL ? 256 : 512;
+    static constexpr int kCtas = SMALL ? 2 : 1;            // per SM
+    static constexpr int kMaxSmem = SMALL ? 115712 : 232448;   // 227 KB of 228, or half of 228 less 1 KB
+};
 constexpr int kLoadRegs = 72, kEpiRegs = 216;
-constexpr int kEpiWarps = 8;
 constexpr int kBlock = 128;               // weight rows of a block
 constexpr int kTileW = kBlock * 128;      // bytes of a block's tile: 128 rows of 128 bytes
 constexpr int kMaxM = 128;                // rows of x per pass
@@ -63,11 +72,9 @@ constexpr int kScFloats = kUnit * (128 + 2);   // of each step: xs of the pass's
 constexpr int kItemSlots = 4;
 constexpr int kMaxAcc = 4;
 constexpr int kMaxStages = 16;
-constexpr int kTmemCols = 512;
 constexpr int kRowMaps = 4;               // boxes of 16, 32, 64, 128 rows of x
-constexpr int kMaxSmem = 232448;          // 227 KB
-constexpr int kMaxRed = 112 << 10;        // shared memory for partial sums of a split
-constexpr int kSplitRows = 32;            // a split item's rows, at most
+constexpr int kMaxRed = 48 << 10;         // shared memory for partial sums of a split
+constexpr int kSmallRows = 32;            // rows of a small pass, at most; only these are split
 constexpr int kRun = 64, kPitch = 80;     // results leave in runs of 64 bytes a row; rows 80 apart in shared memory
 
 __device__ unsigned g_no_status;          // where kernels report when the caller gives no status word
@@ -398,15 +405,17 @@ __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.
 template <int R>
 __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
-template <int TYPE, bool DUAL, bool WIDE, int OUT>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int TYPE, bool DUAL, bool WIDE, bool SMALL, int OUT>
+__global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
     grouped_kernel(const __grid_constant__ GroupedArgs a, const __grid_constant__ Maps maps)
 {
     using Epi = Epilogue<TYPE, DUAL, WIDE, OUT>;
+    using Role = Roles<SMALL>;
+    constexpr int kThreads = Role::kThreads, kWarps = Role::kWarps, kEpiWarps = Role::kEpiWarps;
     constexpr bool FP8 = TYPE == MB_T_E4M3;
     constexpr int KS = FP8 ? 128 : 64;    // columns of a K step
     constexpr int NB = WIDE ? 2 : 1;      // weight tiles of a step
-    constexpr int kAcc = kTmemCols / Epi::N;
+    constexpr int kAcc = Role::kTmemCols / Epi::N;
 
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -460,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         *abort_flag = 0;
         tma_prefetch_map(&maps.w);
     }
-    if (warp == 1) tc_alloc(tmem_slot, kTmemCols);
+    if (warp == Role::kMma) tc_alloc(tmem_slot, Role::kTmemCols);
     mb_pdl_wait();
 
     // The experts' rows and the first item of each: an exclusive scan over the experts, a run of them per thread.
@@ -530,8 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     ItemRing ring{items, item_full, item_empty, status, abort_flag, Ring(kItemSlots)};
     Item w;
 
-    if (warp < kEpiWarp) setmaxnreg_dec<kLoadRegs>();
-    if (warp == 0) {
+    if (!SMALL && warp < 4) setmaxnreg_dec<kLoadRegs>();
+    if (warp == Role::kLoad) {
         // ------------------------------------------------------------------ loads
         Ring st(a.stages);
         bool ok = true;
@@ -566,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
-    } else if (warp == 1) {
+    } else if (warp == Role::kMma) {
         // ------------------------------------------------------------------ tensor cores
         if (elect_one()) {
             Ring st(a.stages), ac(kAcc);
@@ -599,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 2) {
+    } else if (warp == Role::kFind) {
         // ------------------------------------------------------------------ items
         Finder find{a, meta, pstart, (int)blockIdx.x / split - (int)gridDim.x / split, (int)gridDim.x / split, 0};
         Ring r(kItemSlots);
@@ -613,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mb_mbar_arrive(&item_full[r.slot]);
             }
         }
-    } else if (warp == 3) {
+    } else if (warp == Role::kScale) {
         // ------------------------------------------------------------------ scales
         if (FP8) {
             const int Ob = (a.O + kScaleBlock - 1) / kScaleBlock;
@@ -656,10 +665,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ------------------------------------------------------------------ epilogue
-        setmaxnreg_inc<kEpiRegs>();
-        const int q = warp & 3, set = (warp - kEpiWarp) >> 2;
+        if (!SMALL) setmaxnreg_inc<kEpiRegs>();
+        const int q = warp & 3, set = SMALL ? warp >> 2 : (warp >> 2) - 1;
         Epi ep{a, status, abort_flag, tmem + ((uint32_t)(32 * q) << 16), acc_full, acc_empty, sc_full, sc_empty, sc, red,
-               red_full, red_empty, amax, runs + (warp - kEpiWarp) * 32 * kPitch, split, srank, cluster_rank() - srank,
+               red_full, red_empty, amax, runs + (SMALL ? set : warp - 4) * 32 * kPitch, split, srank, cluster_rank() - srank,
                q, set, lane, Ring(kAcc), Ring(kScSlots), 0, 0};
         while (ring.pop<true>(w)) ep.item(w, k0, k1);
     }
@@ -667,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == 1) tc_dealloc(tmem, kTmemCols);
+    if (warp == Role::kMma) tc_dealloc(tmem, Role::kTmemCols);
     if (csize > 1) cluster_sync();        // no CTA ends while another may still write to it
 }
 
@@ -753,12 +762,13 @@ int pow2_at_least(int64_t n, int lo, int hi)
     return p;
 }
 
-template <int TYPE, bool DUAL, bool WIDE, int OUT>
+template <int TYPE, bool DUAL, bool WIDE, bool SMALL, int OUT>
 int launch(GroupedArgs a, const char* what, cudaStream_t st)
 {
     constexpr bool FP8 = TYPE == MB_T_E4M3;
     constexpr int N = WIDE ? 256 : 128;
-    const int sms = mb_num_sms();
+    using Role = Roles<SMALL>;
+    const int slots = mb_num_sms() * Role::kCtas;
     const int64_t active = std::min<int64_t>(a.E, a.P);          // experts with rows, at most
     a.Kb = (a.K + (FP8 ? 127 : 63)) / (FP8 ? 128 : 64);
     a.Nb = DUAL ? (a.O + kBlock - 1) / kBlock : (a.O + N - 1) / N;
@@ -767,29 +777,42 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     const int64_t items = a.Nb * (active + a.P / a.MT);            // an upper bound
     MB_REQUIRE(items < (1ll << 30), "%s: %lld work items", what, (long long)items);
     int cluster = 1;
-    if (a.MT <= kSplitRows)
-        while (cluster < 8 && cluster * 2 <= a.Kb && (2 * cluster - 1) * N * 128 <= kMaxRed &&
-               a.Nb * active * cluster < 4 * sms)
-            cluster *= 2;
+    if (SMALL) {
+        // The split with the fewest K steps in turn on the busiest CTA, the launch of clusters counted as steps too (it
+        // measured 1, 3 and 6 us for 2, 4 and 8 CTAs, a step 0.35 us).  Experts with rows: those that P picks of E meet,
+        // each as likely as another.
+        const double meet = a.offsets ? a.E * (1.0 - std::pow(1.0 - 1.0 / a.E, (double)a.P)) : 1.0;
+        const int64_t likely = std::max<int64_t>(1, (int64_t)(a.Nb * meet + 0.5));
+        int64_t best = (int64_t)1 << 62;
+        for (int c = 1, extra = 0; c <= 8 && c <= a.Kb && (c - 1) * N * 128 <= kMaxRed; c *= 2) {
+            const int64_t groups = slots / c, cost = (likely + groups - 1) / groups * ((a.Kb + c - 1) / c + (c > 1 ? 2 : 0)) +
+                                                     extra;
+            if (cost < best) {
+                best = cost;
+                cluster = c;
+            }
+            extra = c == 1 ? 3 : 2 * extra + 3;
+        }
+    }
     const int stage = a.MT * 128 + N * 128;
     const int fixed = 1024 + (cluster - 1) * N * 128 + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM * 4 : 0) +
-                      (FP8 ? kScSlots * kScFloats * 4 : 0) + kEpiWarps * 32 * kPitch +
+                      (FP8 ? kScSlots * kScFloats * 4 : 0) + Role::kEpiWarps * 32 * kPitch +
                       (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2) * 8 + kItemSlots * 16 + 8 + 64 +
                       a.E * 8 + (a.E + 1) * 4 + 16;
-    a.stages = std::min(kMaxStages, (kMaxSmem - fixed) / stage);
+    a.stages = std::min(kMaxStages, (Role::kMaxSmem - fixed) / stage);
     const int smem = fixed + a.stages * stage;
 
-    auto kern = grouped_kernel<TYPE, DUAL, WIDE, OUT>;
+    auto kern = grouped_kernel<TYPE, DUAL, WIDE, SMALL, OUT>;
     static thread_local uint64_t ready = 0;                        // devices whose attribute is set
     int dev = 0;
     cudaGetDevice(&dev);
     if (!(ready >> (dev & 63) & 1)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Role::kMaxSmem);
         if (e != cudaSuccess) return mb_fail(MB_ECUDA, "%s: %s", what, cudaGetErrorString(e));
         ready |= 1ull << (dev & 63);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = kThreads;
+    cfg.blockDim = Role::kThreads;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -800,9 +823,9 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    int ctas = sms;
+    int ctas = slots;
     if (cluster > 1) {
-        // clusters that fit at the same time: a CTA takes an SM, and a cluster stays within one GPC
+        // clusters that fit at the same time: a cluster stays within one GPC
         static thread_local int fits[64][4] = {};
         int& f = fits[dev & 63][cluster == 2 ? 1 : cluster == 4 ? 2 : 3];
         if (f == 0) {
@@ -834,14 +857,24 @@ int pass_rows(const GroupedArgs& a)
 bool wide(const GroupedArgs& a)
 {
     const int64_t active = std::min<int64_t>(a.E, a.P);
-    return a.MT > kSplitRows && (a.O + 255) / 256 * (active + a.P / a.MT) >= mb_num_sms();
+    return (a.O + 255) / 256 * (active + a.P / a.MT) >= mb_num_sms();
 }
 
 template <int TYPE, int OUT>
 int launch_width(GroupedArgs a, const char* what, cudaStream_t st)
 {
     a.MT = pass_rows(a);
-    return wide(a) ? launch<TYPE, false, true, OUT>(a, what, st) : launch<TYPE, false, false, OUT>(a, what, st);
+    if (a.MT <= kSmallRows) return launch<TYPE, false, false, true, OUT>(a, what, st);
+    return wide(a) ? launch<TYPE, false, true, false, OUT>(a, what, st)
+                   : launch<TYPE, false, false, false, OUT>(a, what, st);
+}
+
+template <int TYPE>
+int launch_swiglu(GroupedArgs a, const char* what, cudaStream_t st)
+{
+    a.MT = pass_rows(a);
+    return a.MT <= kSmallRows ? launch<TYPE, true, true, true, TYPE>(a, what, st)
+                              : launch<TYPE, true, true, false, TYPE>(a, what, st);
 }
 
 template <int TYPE>
@@ -892,14 +925,13 @@ extern "C" int mb_grouped_swiglu_t(const void* x, int type, int64_t ldx, const f
 {
     const char* what = "mb_grouped_swiglu_t";
     MB_REQUIRE(offsets || P == 0, "%s: null pointer", what);
-    GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K,
-                  offsets, q, ldq, qs, qs_row, qs_group, status};
+    const GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K,
+                        offsets, q, ldq, qs, qs_row, qs_group, status};
     int rc = check_args(a, type, 2, what);
     if (rc || P == 0) return rc;
     MB_REQUIRE(type != MB_T_E4M3 || qs, "%s: e4m3 results need their scales", what);
     const cudaStream_t st = mb_stream(stream);
-    a.MT = pass_rows(a);
-    if (type == MB_T_E4M3) return launch<MB_T_E4M3, true, true, MB_T_E4M3>(a, what, st);
-    if (type == MB_T_BF16) return launch<MB_T_BF16, true, true, MB_T_BF16>(a, what, st);
-    return launch<MB_T_F16, true, true, MB_T_F16>(a, what, st);
+    if (type == MB_T_E4M3) return launch_swiglu<MB_T_E4M3>(a, what, st);
+    if (type == MB_T_BF16) return launch_swiglu<MB_T_BF16>(a, what, st);
+    return launch_swiglu<MB_T_F16>(a, what, st);
 }
