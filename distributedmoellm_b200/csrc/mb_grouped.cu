@@ -60,6 +60,11 @@ struct Roles {
     static constexpr int kLoad = SMALL ? 1 : 0, kMma = SMALL ? 2 : 1, kFind = SMALL ? 3 : 2, kScale = SMALL ? 5 : 3;
     static constexpr int kTmemCols = SMALL ? 256 : 512;
     static constexpr int kCtas = SMALL ? 2 : 1;            // per SM
+    // Tiles of results a warp has in flight.  e4m3 sums wait for the epilogue at every step, so large e4m3 passes send
+    // their results by TMA from four tiles a warp, at the price of the fourth stage (which measured nothing there, and
+    // 8% for 16-bit types).
+    template <bool FP8>
+    static constexpr int kTiles = !SMALL && FP8 ? 4 : 1;
     static constexpr int kMaxSmem = SMALL ? 115712 : 232448;   // 227 KB of 228, or half of 228 less 1 KB
 };
 constexpr int kLoadRegs = 72, kEpiRegs = 216;
@@ -75,7 +80,8 @@ constexpr int kMaxStages = 16;
 constexpr int kRowMaps = 4;               // boxes of 16, 32, 64, 128 rows of x
 constexpr int kMaxRed = 48 << 10;         // shared memory for partial sums of a split
 constexpr int kSmallRows = 32;            // rows of a small pass, at most; only these are split
-constexpr int kRun = 64, kPitch = 80;     // results leave in runs of 64 bytes a row; rows 80 apart in shared memory
+constexpr int kRun = 64;                  // results leave in runs of 64 bytes a row ..
+constexpr int kTile = 32 * kRun;          // .. and tiles of 32 rows
 
 __device__ unsigned g_no_status;          // where kernels report when the caller gives no status word
 
@@ -106,6 +112,7 @@ struct GroupedArgs {
 struct Maps {
     CUtensorMap w;
     CUtensorMap x[kRowMaps];
+    CUtensorMap y[2];          // tiles of results: runs of 32 rows, of 8 rows
 };
 
 // A work item: expert, block of weight rows, first row of x and how many (none: no more items).
@@ -180,13 +187,14 @@ __device__ __forceinline__ uint32_t round2(float lo, float hi)
 
 // WIDE: an item is two blocks of 128 weight rows, one per epilogue set (gate|up: the gate and the up rows of 128 columns,
 // of which each set takes 64); else one block, 64 columns per set.  OUT: the result type (gate|up: TYPE).
-template <int TYPE, bool DUAL, bool WIDE, int OUT>
+template <int TYPE, bool DUAL, bool WIDE, bool SMALL, int OUT>
 struct Epilogue {
     static constexpr bool FP8 = TYPE == MB_T_E4M3;
     static constexpr int H = DUAL ? 2 : 1;
     static constexpr int N = WIDE ? 256 : 128;             // accumulator columns of an item
     static constexpr int S = N / 2;                        // of them this thread's
     static constexpr int C = S / 16;                       // chunks of 16
+    static constexpr int kTiles = Roles<SMALL>::template kTiles<FP8>;
 
     const GroupedArgs& a;
     unsigned* status;
@@ -197,12 +205,13 @@ struct Epilogue {
     float4* red;               // partial sums: [sender][set][S / 4][32 lanes]
     uint64_t *red_full, *red_empty;
     float* amax;               // [2][2 sets][128 rows]
-    uint8_t* stage;            // the warp's 32 rows of kRun bytes
+    uint8_t* tiles;            // the warp's tiles of 32 rows of kRun bytes
+    const CUtensorMap* ymaps;
     int split, srank;
     uint32_t leader;
     int q, set, lane;
     Ring ac, scr;
-    int sent, abuf;
+    int sent, abuf, tile;
 
     // Accumulator column of this thread's chunk c.  Gate|up: its first half of chunks are gate columns, then the up
     // columns of the same place.
@@ -316,52 +325,80 @@ struct Epilogue {
             constexpr int RC = kRun / out_bytes(OUT);      // columns of a run: 16 of f32, 32 of 16 bits
 #pragma unroll
             for (int r = 0; r < (DUAL ? 64 : S) / RC; ++r) {
-                uint4* to = reinterpret_cast<uint4*>(stage + lane * kPitch);
+                begin();
 #pragma unroll
                 for (int j = 0; j < kRun / 16; ++j) {
                     constexpr int VC = 16 / out_bytes(OUT);
                     const int i = r * RC + j * VC;
                     const float* v = &sum[i / 16][i % 16];
                     if constexpr (OUT == MB_T_F32)
-                        to[j] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                                           __float_as_uint(v[3]));
+                        *run(lane, j) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                                   __float_as_uint(v[3]));
                     else
-                        to[j] = make_uint4(round2<OUT>(v[0], v[1]), round2<OUT>(v[2], v[3]), round2<OUT>(v[4], v[5]),
-                                           round2<OUT>(v[6], v[7]));
+                        *run(lane, j) = make_uint4(round2<OUT>(v[0], v[1]), round2<OUT>(v[2], v[3]),
+                                                   round2<OUT>(v[4], v[5]), round2<OUT>(v[6], v[7]));
                 }
                 send(row, n, col + r * RC);
             }
         }
     }
 
-    // The warp's 32 staged runs to rows row .. row + n - 1 of y, from column col on (not past column O).
+    // 16 bytes j of row r in the tile being filled: the four of a row change places every two rows (the 64-byte swizzle of
+    // the y maps), which keeps both the rows' and the runs' accesses on different banks.
+    __device__ __forceinline__ uint4* run(int r, int j) const
+    {
+        return reinterpret_cast<uint4*>(tiles + tile * kTile + r * kRun + ((j ^ (r >> 1 & 3)) << 4));
+    }
+
+    // The tile to be filled next has been read by whoever sent it.
+    __device__ __forceinline__ void begin()
+    {
+        if (kTiles > 1) {
+            tile = (tile + 1) % kTiles;
+            bulk_wait_read<kTiles - 1>();
+            __syncwarp();
+        }
+    }
+
+    // The tile's 32 runs to rows row .. row + n - 1 of y, from column col on (not past column O).
     __device__ __forceinline__ void send(int64_t row, int n, int col)
     {
         constexpr int B = out_bytes(OUT);
-        __syncwarp();
         uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row * a.ldy + col) * B;
+        int first = 0;                                     // rows before this one go by TMA, which knows where y ends
+        if (kTiles > 1) {
+            if (a.vec && col < a.O) {
+                first = max(n, 0) & ~7;
+                bulk_fence();
+                __syncwarp();
+                if (first == 32 && lane == 0)
+                    tma_store2(ymaps, tiles + tile * kTile, col, (int)row);
+                else if (first < 32 && lane < first / 8)
+                    tma_store2(ymaps + 1, tiles + tile * kTile + lane * 8 * kRun, col, (int)row + lane * 8);
+            }
+            bulk_commit();
+        }
+        __syncwarp();
         if (a.vec && col + kRun / B <= a.O) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 8 * i + (lane >> 2), s = 16 * (lane & 3);
-                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * kPitch + s);
-                if (r < n) *reinterpret_cast<uint4*>(dst + r * a.ldy * B + s) = v;
+            for (int i = 0; i < (kTiles > 1 ? 1 : 4); ++i) {
+                const int r = first + 8 * i + (lane >> 2), j = lane & 3;
+                if (r < n) *reinterpret_cast<uint4*>(dst + r * a.ldy * B + 16 * j) = *run(r, j);
             }
         } else {
             const int cols = min(kRun / B, a.O - col);
-            for (int r = 0; r < n; ++r)
+            for (int r = first; r < n; ++r)
                 for (int i = lane; i < cols; i += 32) {
+                    const uint8_t* from = reinterpret_cast<const uint8_t*>(run(r, i * B / 16)) + i * B % 16;
                     if (B == 4)
-                        reinterpret_cast<uint32_t*>(dst + r * a.ldy * B)[i] =
-                            reinterpret_cast<const uint32_t*>(stage + r * kPitch)[i];
+                        reinterpret_cast<uint32_t*>(dst + r * a.ldy * B)[i] = *reinterpret_cast<const uint32_t*>(from);
                     else if (B == 2)
-                        reinterpret_cast<uint16_t*>(dst + r * a.ldy * B)[i] =
-                            reinterpret_cast<const uint16_t*>(stage + r * kPitch)[i];
+                        reinterpret_cast<uint16_t*>(dst + r * a.ldy * B)[i] = *reinterpret_cast<const uint16_t*>(from);
                     else
-                        dst[r * a.ldy + i] = stage[r * kPitch + i];
+                        dst[r * a.ldy + i] = *from;
                 }
         }
-        __syncwarp();
+        if (kTiles == 1) __syncwarp();
     }
 
     // This thread's 64 activations of a row as e4m3, the row's scale over them and the other set's 64.
@@ -382,7 +419,7 @@ struct Epilogue {
         const Quotient qu(e4m3_scale(fmaxf(am[0], am[kMaxM])));
         const bool fast = __all_sync(0xffffffffu, qu.fast || lane >= n);
         if (set == 0 && lane < n) a.qs[(row + lane) * a.qs_row + nb * a.qs_group] = qu.s;
-        uint4* to = reinterpret_cast<uint4*>(stage + lane * kPitch);
+        begin();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             uint32_t u[4];
@@ -394,7 +431,7 @@ struct Epilogue {
                             : to_e4m3x2(__fdiv_rn(x[0], qu.s), __fdiv_rn(x[1], qu.s)) |
                                   to_e4m3x2(__fdiv_rn(x[2], qu.s), __fdiv_rn(x[3], qu.s)) << 16;
             }
-            to[j] = make_uint4(u[0], u[1], u[2], u[3]);
+            *run(lane, j) = make_uint4(u[0], u[1], u[2], u[3]);
         }
         send(row, n, col);
     }
@@ -409,7 +446,7 @@ template <int TYPE, bool DUAL, bool WIDE, bool SMALL, int OUT>
 __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
     grouped_kernel(const __grid_constant__ GroupedArgs a, const __grid_constant__ Maps maps)
 {
-    using Epi = Epilogue<TYPE, DUAL, WIDE, OUT>;
+    using Epi = Epilogue<TYPE, DUAL, WIDE, SMALL, OUT>;
     using Role = Roles<SMALL>;
     constexpr int kThreads = Role::kThreads, kWarps = Role::kWarps, kEpiWarps = Role::kEpiWarps;
     constexpr bool FP8 = TYPE == MB_T_E4M3;
@@ -425,10 +462,10 @@ __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
     const uint32_t csize = cluster_size();
     uint8_t* stage0 = smem;
     float4* red = reinterpret_cast<float4*>(stage0 + (size_t)a.stages * stage_bytes);
-    float* amax = reinterpret_cast<float*>(red + (csize - 1) * Epi::N / 4 * 32);
+    uint8_t* tiles = reinterpret_cast<uint8_t*>(red + (csize - 1) * Epi::N / 4 * 32);   // 1024-byte aligned
+    float* amax = reinterpret_cast<float*>(tiles + kEpiWarps * Epi::kTiles * kTile);
     float* sc = amax + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM : 0);
-    uint8_t* runs = reinterpret_cast<uint8_t*>(sc + (FP8 ? kScSlots * kScFloats : 0));
-    uint64_t* full = reinterpret_cast<uint64_t*>(runs + kEpiWarps * 32 * kPitch);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sc + (FP8 ? kScSlots * kScFloats : 0));
     uint64_t* empty = full + kMaxStages;
     uint64_t* acc_full = empty + kMaxStages;
     uint64_t* acc_empty = acc_full + kMaxAcc;
@@ -668,9 +705,10 @@ __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
         if (!SMALL) setmaxnreg_inc<kEpiRegs>();
         const int q = warp & 3, set = SMALL ? warp >> 2 : (warp >> 2) - 1;
         Epi ep{a, status, abort_flag, tmem + ((uint32_t)(32 * q) << 16), acc_full, acc_empty, sc_full, sc_empty, sc, red,
-               red_full, red_empty, amax, runs + (SMALL ? set : warp - 4) * 32 * kPitch, split, srank, cluster_rank() - srank,
-               q, set, lane, Ring(kAcc), Ring(kScSlots), 0, 0};
+               red_full, red_empty, amax, tiles + (SMALL ? set : warp - 4) * Epi::kTiles * kTile, maps.y, split, srank,
+               cluster_rank() - srank, q, set, lane, Ring(kAcc), Ring(kScSlots), 0, 0, 0};
         while (ring.pop<true>(w)) ep.item(w, k0, k1);
+        if (Epi::kTiles > 1) bulk_wait();
     }
 
     tc_before();
@@ -703,6 +741,7 @@ CUtensorMapDataType map_type(int type)
 {
     return type == MB_T_E4M3  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
            : type == MB_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+           : type == MB_T_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
@@ -732,7 +771,7 @@ int check_args(const GroupedArgs& a, int type, int halves, const char* what)
 }
 
 
-int make_maps(const GroupedArgs& a, int type, int halves, Maps* m, const char* what)
+int make_maps(const GroupedArgs& a, int type, int halves, int out, bool tiles, Maps* m, const char* what)
 {
     const EncodeTiledFn fn = encode_fn();
     if (!fn) return mb_fail(MB_ECUDA, "%s: cuTensorMapEncodeTiled unavailable", what);
@@ -750,6 +789,15 @@ int make_maps(const GroupedArgs& a, int type, int halves, Maps* m, const char* w
         const cuuint32_t xbox[2] = {inner, (cuuint32_t)(16 << i)};
         r = fn(&m->x[i], map_type(type), 2, const_cast<void*>(a.x), xd, xst, xbox, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    }
+    if (tiles && a.vec) {
+        const cuuint64_t ob = (cuuint64_t)out_bytes(out);
+        const cuuint64_t yd[2] = {(cuuint64_t)a.O, (cuuint64_t)a.P}, yst[1] = {(cuuint64_t)a.ldy * ob};
+        for (int i = 0; i < 2 && r == CUDA_SUCCESS; ++i) {
+            const cuuint32_t ybox[2] = {(cuuint32_t)(kRun / ob), i == 0 ? 32u : 8u};
+            r = fn(&m->y[i], map_type(out), 2, a.y, yd, yst, ybox, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        }
     }
     if (r != CUDA_SUCCESS) return mb_fail(MB_ECUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
     return MB_OK;
@@ -796,7 +844,7 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     }
     const int stage = a.MT * 128 + N * 128;
     const int fixed = 1024 + (cluster - 1) * N * 128 + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM * 4 : 0) +
-                      (FP8 ? kScSlots * kScFloats * 4 : 0) + Role::kEpiWarps * 32 * kPitch +
+                      (FP8 ? kScSlots * kScFloats * 4 : 0) + Role::kEpiWarps * Role::template kTiles<FP8> * kTile +
                       (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2) * 8 + kItemSlots * 16 + 8 + 64 +
                       a.E * 8 + (a.E + 1) * 4 + 16;
     a.stages = std::min(kMaxStages, (Role::kMaxSmem - fixed) / stage);
@@ -839,7 +887,7 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     }
     cfg.gridDim = (unsigned)std::min<int64_t>(ctas, items * cluster);
     Maps maps;
-    const int rc = make_maps(a, TYPE, DUAL ? 2 : 1, &maps, what);
+    const int rc = make_maps(a, TYPE, DUAL ? 2 : 1, OUT, Role::template kTiles<FP8> > 1, &maps, what);
     if (rc) return rc;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, maps);
     if (e != cudaSuccess) return mb_fail(MB_ECUDA, "%s: %s", what, cudaGetErrorString(e));

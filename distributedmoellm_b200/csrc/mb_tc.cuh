@@ -106,6 +106,25 @@ __device__ __forceinline__ void tma_load3(void* dst, const CUtensorMap* map, int
         : "memory");
 }
 
+// Shared -> global tile copies in the background: the writers of the shared tile fence, then (after a barrier) one thread
+// copies and commits, and waits for its copies to have read shared memory before the tile is written again.
+__device__ __forceinline__ void bulk_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tma_store2(const CUtensorMap* map, const void* src, int c0, int c1)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(c0), "r"(c1), "r"(mb_smem_addr(src))
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// At most N of this thread's committed groups have still to read shared memory.
+template <int N>
+__device__ __forceinline__ void bulk_wait_read()
+{
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ---- thread-block clusters -------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t cluster_size()
