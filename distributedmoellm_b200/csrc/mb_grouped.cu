@@ -195,6 +195,7 @@ struct Epilogue {
     static constexpr int S = N / 2;                        // of them this thread's
     static constexpr int C = S / 16;                       // chunks of 16
     static constexpr int kTiles = Roles<SMALL>::template kTiles<FP8>;
+    static constexpr int kBatch = kTiles > 1 ? kTiles / 2 : 1;   // tiles sent together, while the others are on their way
 
     const GroupedArgs& a;
     unsigned* status;
@@ -211,7 +212,7 @@ struct Epilogue {
     uint32_t leader;
     int q, set, lane;
     Ring ac, scr;
-    int sent, abuf, tile;
+    int sent, abuf, half;
 
     // Accumulator column of this thread's chunk c.  Gate|up: its first half of chunks are gate columns, then the up
     // columns of the same place.
@@ -323,73 +324,84 @@ struct Epilogue {
             encode(sum, row, n, w.nb, col);
         } else if (rows) {
             constexpr int RC = kRun / out_bytes(OUT);      // columns of a run: 16 of f32, 32 of 16 bits
+            constexpr int R = (DUAL ? 64 : S) / RC, B = R < kBatch ? R : kBatch;   // runs; a batch of them
 #pragma unroll
-            for (int r = 0; r < (DUAL ? 64 : S) / RC; ++r) {
+            for (int r0 = 0; r0 < R; r0 += B) {
                 begin();
 #pragma unroll
-                for (int j = 0; j < kRun / 16; ++j) {
-                    constexpr int VC = 16 / out_bytes(OUT);
-                    const int i = r * RC + j * VC;
-                    const float* v = &sum[i / 16][i % 16];
-                    if constexpr (OUT == MB_T_F32)
-                        *run(lane, j) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                                                   __float_as_uint(v[3]));
-                    else
-                        *run(lane, j) = make_uint4(round2<OUT>(v[0], v[1]), round2<OUT>(v[2], v[3]),
-                                                   round2<OUT>(v[4], v[5]), round2<OUT>(v[6], v[7]));
-                }
-                send(row, n, col + r * RC);
+                for (int r = r0; r < r0 + B; ++r)
+#pragma unroll
+                    for (int j = 0; j < kRun / 16; ++j) {
+                        constexpr int VC = 16 / out_bytes(OUT);
+                        const int i = r * RC + j * VC;
+                        const float* v = &sum[i / 16][i % 16];
+                        if constexpr (OUT == MB_T_F32)
+                            *run(r - r0, lane, j) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                                               __float_as_uint(v[2]), __float_as_uint(v[3]));
+                        else
+                            *run(r - r0, lane, j) = make_uint4(round2<OUT>(v[0], v[1]), round2<OUT>(v[2], v[3]),
+                                                               round2<OUT>(v[4], v[5]), round2<OUT>(v[6], v[7]));
+                    }
+                send<B>(row, n, col + r0 * RC);
             }
         }
     }
 
-    // 16 bytes j of row r in the tile being filled: the four of a row change places every two rows (the 64-byte swizzle of
-    // the y maps), which keeps both the rows' and the runs' accesses on different banks.
-    __device__ __forceinline__ uint4* run(int r, int j) const
+    // 16 bytes j of row r in tile t of the batch: the four of a row change places every two rows (the 64-byte swizzle of the y maps),
+    // which keeps both the rows' and the runs' accesses on different banks.
+    __device__ __forceinline__ uint4* run(int t, int r, int j) const
     {
-        return reinterpret_cast<uint4*>(tiles + tile * kTile + r * kRun + ((j ^ (r >> 1 & 3)) << 4));
+        return reinterpret_cast<uint4*>(tiles + (kTiles > 1 ? half * kBatch + t : t) * kTile + r * kRun + ((j ^ (r >> 1 & 3)) << 4));
     }
 
-    // The tile to be filled next has been read by whoever sent it.
+    // The next batch's tiles have been read by whoever sent them.
     __device__ __forceinline__ void begin()
     {
         if (kTiles > 1) {
-            tile = (tile + 1) % kTiles;
-            bulk_wait_read<kTiles - 1>();
-            __syncwarp();
-        }
-    }
-
-    // The tile's 32 runs to rows row .. row + n - 1 of y, from column col on (not past column O).
-    __device__ __forceinline__ void send(int64_t row, int n, int col)
-    {
-        constexpr int B = out_bytes(OUT);
-        uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row * a.ldy + col) * B;
-        int first = 0;                                     // rows before this one go by TMA, which knows where y ends
-        if (kTiles > 1) {
-            if (a.vec && col < a.O) {
-                first = max(n, 0) & ~7;
-                bulk_fence();
-                __syncwarp();
-                if (first == 32 && lane == 0)
-                    tma_store2(ymaps, tiles + tile * kTile, col, (int)row);
-                else if (first < 32 && lane < first / 8)
-                    tma_store2(ymaps + 1, tiles + tile * kTile + lane * 8 * kRun, col, (int)row + lane * 8);
-            }
-            bulk_commit();
+            half ^= 1;
+            bulk_wait_read<1>();
         }
         __syncwarp();
-        if (a.vec && col + kRun / B <= a.O) {
+    }
+
+    // The batch's first T tiles' runs, each run next to the one before, to rows row .. row + n - 1 of y, from column col on (not
+    // past column O).
+    template <int T>
+    __device__ __forceinline__ void send(int64_t row, int n, int col)
+    {
+        constexpr int B = out_bytes(OUT), RC = kRun / B;
+        uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row * a.ldy + col) * B;
+        int first = 0;                                     // rows before this one go by TMA, which knows where y ends
+        if (kTiles > 1 && a.vec) {
+            // a copy per lane: of 32 rows of a tile, or of 8 rows of as many as there are
+            first = max(n, 0) & ~7;
+            bulk_fence();
+            __syncwarp();
+            const int t = first == 32 ? lane : lane >> 2, r = first == 32 ? 0 : 8 * (lane & 3);
+            if (t < T && r < first && col + t * RC < a.O)
+                tma_store2(first == 32 ? ymaps : ymaps + 1, tiles + (half * kBatch + t) * kTile + r * kRun, col + t * RC,
+                           (int)row + r);
+        } else {
+            __syncwarp();
+        }
+        if (kTiles > 1) bulk_commit();
+        if (a.vec && col + T * RC <= a.O) {
+            if (first < n) {
 #pragma unroll
-            for (int i = 0; i < (kTiles > 1 ? 1 : 4); ++i) {
-                const int r = first + 8 * i + (lane >> 2), j = lane & 3;
-                if (r < n) *reinterpret_cast<uint4*>(dst + r * a.ldy * B + 16 * j) = *run(r, j);
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int i = 0; i < (kTiles > 1 ? 1 : 4); ++i) {
+                        const int r = first + 8 * i + (lane >> 2), j = lane & 3;
+                        if (r < n)
+                            *reinterpret_cast<uint4*>(dst + r * a.ldy * B + t * kRun + 16 * j) = *run(t, r, j);
+                    }
             }
         } else {
-            const int cols = min(kRun / B, a.O - col);
+            const int cols = min(T * RC, a.O - col);
             for (int r = first; r < n; ++r)
                 for (int i = lane; i < cols; i += 32) {
-                    const uint8_t* from = reinterpret_cast<const uint8_t*>(run(r, i * B / 16)) + i * B % 16;
+                    const uint8_t* from =
+                        reinterpret_cast<const uint8_t*>(run(i / RC, r, i % RC * B / 16)) + i * B % 16;
                     if (B == 4)
                         reinterpret_cast<uint32_t*>(dst + r * a.ldy * B)[i] = *reinterpret_cast<const uint32_t*>(from);
                     else if (B == 2)
@@ -398,7 +410,6 @@ struct Epilogue {
                         dst[r * a.ldy + i] = *from;
                 }
         }
-        if (kTiles == 1) __syncwarp();
     }
 
     // This thread's 64 activations of a row as e4m3, the row's scale over them and the other set's 64.
@@ -431,9 +442,9 @@ struct Epilogue {
                             : to_e4m3x2(__fdiv_rn(x[0], qu.s), __fdiv_rn(x[1], qu.s)) |
                                   to_e4m3x2(__fdiv_rn(x[2], qu.s), __fdiv_rn(x[3], qu.s)) << 16;
             }
-            *run(lane, j) = make_uint4(u[0], u[1], u[2], u[3]);
+            *run(0, lane, j) = make_uint4(u[0], u[1], u[2], u[3]);
         }
-        send(row, n, col);
+        send<1>(row, n, col);
     }
 };
 
