@@ -13,7 +13,8 @@ constexpr int kScaleBlock = MB_SCALE_BLOCK;
 // small that the quotient underflows), as mb_encode_rows does for int8.
 __device__ __forceinline__ float e4m3_scale(float m)
 {
-    const float s = __fdiv_rn(m, 448.0f);
+    const float r = 1.0f / 448.0f, q = m * r;              // see quotient()
+    const float s = m > 0x1p-100f && m < 0x1p120f ? fmaf(fmaf(-q, 448.0f, m), r, q) : __fdiv_rn(m, 448.0f);
     return s == 0.0f ? 1.0f : s;
 }
 
@@ -35,6 +36,26 @@ __device__ __forceinline__ float quotient(float x, float s, float r)
 {
     const float q = x * r;
     return copysignf(fmaf(fmaf(-q, s, x), r, q), x);       // the correction would turn -0 into +0
+}
+
+// quotient() of four values by one s, two at a time in packed arithmetic.
+__device__ __forceinline__ void quotient4(float (&x)[4], float s, float r)
+{
+    uint64_t s2, r2;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(-s));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r2) : "f"(r));
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        uint64_t v, q, e;
+        float lo, hi;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x[i]), "f"(x[i + 1]));
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(v), "l"(r2));
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e) : "l"(q), "l"(s2), "l"(v));
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(q) : "l"(e), "l"(r2), "l"(q));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(q));
+        x[i] = copysignf(lo, x[i]);
+        x[i + 1] = copysignf(hi, x[i + 1]);
+    }
 }
 
 // Nearest e4m3 of two values, as bytes lo, hi.

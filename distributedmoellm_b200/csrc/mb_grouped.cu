@@ -436,11 +436,14 @@ struct Epilogue {
             uint32_t u[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float* x = &v[j][4 * i];
-                u[i] = fast ? to_e4m3x2(quotient(x[0], qu.s, qu.r), quotient(x[1], qu.s, qu.r)) |
-                                  to_e4m3x2(quotient(x[2], qu.s, qu.r), quotient(x[3], qu.s, qu.r)) << 16
-                            : to_e4m3x2(__fdiv_rn(x[0], qu.s), __fdiv_rn(x[1], qu.s)) |
-                                  to_e4m3x2(__fdiv_rn(x[2], qu.s), __fdiv_rn(x[3], qu.s)) << 16;
+                float x[4] = {v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3]};
+                if (fast) {
+                    quotient4(x, qu.s, qu.r);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = __fdiv_rn(x[k], qu.s);
+                }
+                u[i] = to_e4m3x2(x[0], x[1]) | to_e4m3x2(x[2], x[3]) << 16;
             }
             *run(0, lane, j) = make_uint4(u[0], u[1], u[2], u[3]);
         }

@@ -112,9 +112,13 @@ __global__ void operand_rows_kernel(const SRC* __restrict__ x, int64_t ldx, int6
         for (int g = 0; g < kGroups; ++g) {
             const int c = c0 + g * kScaleBlock;
             const float s = __shfl_sync(0xffffffffu, mine.s, 8 * g), r = __shfl_sync(0xffffffffu, mine.r, 8 * g);
-            float t[4];
+            float t[4] = {v[g][0], v[g][1], v[g][2], v[g][3]};
+            if (fast) {
+                quotient4(t, s, r);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = fast ? quotient(v[g][i], s, r) : __fdiv_rn(v[g][i], s);
+                for (int i = 0; i < 4; ++i) t[i] = __fdiv_rn(t[i], s);
+            }
             const uint32_t u = to_e4m3x2(t[0], t[1]) | to_e4m3x2(t[2], t[3]) << 16;
             if (VEC) {
                 if (c < d) *reinterpret_cast<uint32_t*>(dst + c) = u;
