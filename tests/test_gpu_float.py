@@ -617,3 +617,35 @@ def test_layer_equals_packed_experts_of_the_same_weights(D):
     assert torch.equal(a.buffers(T).idx, b.buffers(T).idx)
     # rows off by 2^-11 move gate and up by 2^-11 sum |x w|; bounded here through the largest output of the row
     assert float(((ya - yb).abs().amax(1) / ya.abs().amax(1)).max()) < 1e-2
+
+
+# ---- operand rows of many picks (each row of x made once, then copied to its picks) ------------------
+
+@pytest.mark.parametrize("src,dst,T,k,d", [(F32, E4M3, 1200, 8, 512), (F32, E4M3, 1187, 5, 400), (BF16, E4M3, 1300, 4, 2048),
+                                           (F32, BF16, 1200, 6, 768), (F16, F16, 1250, 4, 1032)])
+def test_operand_rows_of_many_picks(D, src, dst, T, k, d):
+    """Every token k times in random order, one token another 5000 times, and some indices outside x."""
+    g = gen(T + k + d)
+    x = (torch.randn((T, d), generator=g, device="cuda") * 3).to(src)
+    rows = torch.arange(T, device="cuda", dtype=torch.int32).repeat(k)
+    rows = torch.cat([rows, torch.full((5000,), 7, dtype=torch.int32, device="cuda")])
+    rows = rows[torch.randperm(rows.numel(), generator=g, device="cuda")].contiguous()
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q, s = D.operand_rows(x, dst, rows=rows, status=st)
+    assert int(st) == 0
+
+    def want(r):
+        return plain_e4m3(x[r.long()]) if dst == E4M3 else (x[r.long()].float().to(dst), None)
+    wq, ws = want(rows)
+    assert same_bits(q, wq) and (s is None or torch.equal(s, ws))
+    bad = torch.tensor([0, 4100, rows.numel() - 1], device="cuda")
+    rows[bad] = torch.tensor([-1, T, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    q, s = D.operand_rows(x, dst, rows=rows, status=st)
+    assert int(st) == 2
+    rows[bad] = 0
+    wq, ws = want(rows)
+    wq[bad] = torch.zeros((3, d), device="cuda").to(dst)
+    assert same_bits(q, wq)
+    if s is not None:
+        ws[bad] = 1.0
+        assert torch.equal(s, ws)
