@@ -48,26 +48,27 @@
 
 namespace {
 
-// Who does what.  Large passes: one CTA per SM, eight epilogue warps; 168 registers a thread at launch, of which the
-// epilogue warpgroups (up to 128 sums a thread) take their share from the first warpgroup: 128 * 72 + 256 * 216 = 64512 =
-// the launch's 384 * 168.  Small passes (at most 32 rows) use one quarter of the TMEM lanes, which the warps 0 and 4 can
-// read: six warps, half of the shared and the tensor memory, and so two CTAs per SM, one's hand-overs and prologue beside
-// the other's.
-template <bool SMALL>
+// Who does what.  Small passes (at most 32 rows) use one quarter of the TMEM lanes, which the warps 0 and 4 can read: six
+// warps, half of the shared and the tensor memory, and so two CTAs per SM, one's hand-overs and prologue beside the
+// other's.  Large passes: one CTA per SM, eight epilogue warps; 168 registers a thread at launch, of which the epilogue
+// warpgroups (up to 128 sums a thread) take their share from the first: 128 * 72 + 256 * 216 = 64512 = 384 * 168.
+// (Sixteen epilogue warps with half the columns each measured the same: a step's length is the round trip from the
+// products to the sums and back over the two accumulators that TMEM holds, about 900 cycles.)
+template <bool SMALL, bool FP8>
 struct Roles {
-    static constexpr int kWarps = SMALL ? 6 : 12, kThreads = 32 * kWarps;
     static constexpr int kEpiWarps = SMALL ? 2 : 8;
+    static constexpr int kWarps = SMALL ? 6 : 12, kThreads = 32 * kWarps;
     static constexpr int kLoad = SMALL ? 1 : 0, kMma = SMALL ? 2 : 1, kFind = SMALL ? 3 : 2, kScale = SMALL ? 5 : 3;
     static constexpr int kTmemCols = SMALL ? 256 : 512;
     static constexpr int kCtas = SMALL ? 2 : 1;            // per SM
     // Tiles of results a warp has in flight.  e4m3 sums wait for the epilogue at every step, so large e4m3 passes send
-    // their results by TMA from four tiles a warp, at the price of the fourth stage (which measured nothing there, and
-    // 8% for 16-bit types).
-    template <bool FP8>
+    // their results by TMA, two tiles while the next two are filled, at the price of the fourth stage (which measured
+    // nothing there, and 8% for 16-bit types).
     static constexpr int kTiles = !SMALL && FP8 ? 4 : 1;
     static constexpr int kMaxSmem = SMALL ? 115712 : 232448;   // 227 KB of 228, or half of 228 less 1 KB
 };
 constexpr int kLoadRegs = 72, kEpiRegs = 216;
+constexpr int kSets = 2;                  // of epilogue warps, each with half of an item's columns
 constexpr int kBlock = 128;               // weight rows of a block
 constexpr int kTileW = kBlock * 128;      // bytes of a block's tile: 128 rows of 128 bytes
 constexpr int kMaxM = 128;                // rows of x per pass
@@ -192,21 +193,25 @@ struct Epilogue {
     static constexpr bool FP8 = TYPE == MB_T_E4M3;
     static constexpr int H = DUAL ? 2 : 1;
     static constexpr int N = WIDE ? 256 : 128;             // accumulator columns of an item
-    static constexpr int S = N / 2;                        // of them this thread's
+    using Role = Roles<SMALL, FP8>;
+    static constexpr int kTiles = Role::kTiles;
+    static constexpr int kBatch = kTiles > 1 && OUT != MB_T_E4M3 ? 2 : 1;   // tiles sent together
+    static constexpr int S = N / kSets;                    // of them this thread's
     static constexpr int C = S / 16;                       // chunks of 16
-    static constexpr int kTiles = Roles<SMALL>::template kTiles<FP8>;
-    static constexpr int kBatch = kTiles > 1 ? kTiles / 2 : 1;   // tiles sent together, while the others are on their way
+    static constexpr int R = S / H;                        // results of this thread
+    static constexpr int B = out_bytes(OUT);
+    static constexpr int RC = kRun / B;                    // columns of a run
 
     const GroupedArgs& a;
     unsigned* status;
     volatile int* abort_flag;
     uint32_t tl;               // TMEM address of the warp's lane quarter
-    uint64_t *acc_full, *acc_empty, *sc_full, *sc_empty;
+    uint32_t acc_full, acc_empty, sc_full, sc_empty;       // shared-memory addresses
     const float* sc;
     float4* red;               // partial sums: [sender][set][S / 4][32 lanes]
     uint64_t *red_full, *red_empty;
-    float* amax;               // [2][2 sets][128 rows]
-    uint8_t* tiles;            // the warp's tiles of 32 rows of kRun bytes
+    float* amax;               // [2][sets][128 rows]
+    uint8_t* tiles;            // the warp's tiles of results
     const CUtensorMap* ymaps;
     int split, srank;
     uint32_t leader;
@@ -218,7 +223,7 @@ struct Epilogue {
     // columns of the same place.
     __device__ __forceinline__ int column(int c) const
     {
-        if (DUAL) return (c >= C / 2 ? kBlock : 0) + 64 * set + 16 * (c % (C / 2));
+        if (DUAL) return (c >= C / 2 ? kBlock : 0) + R * set + 16 * (c % (C / 2));
         return S * set + 16 * c;
     }
 
@@ -232,43 +237,31 @@ struct Epilogue {
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sum[c][i] = 0.0f;
-        for (int kb = k0, us = 0; kb < k1; kb += a.prom) {
-            float s[H];
-            if (FP8) {
-                if (us == 0) ok = mb_mbar_wait_spin(&sc_full[scr.slot], scr.full_parity(), status, abort_flag) && ok;
-                const float* from = sc + scr.slot * kScFloats + us * 130;
-                const float x = from[32 * q + lane];
-                const float2 b = *reinterpret_cast<const float2*>(from + 128);
-                s[0] = x * (!DUAL && WIDE && set ? b.y : b.x);
-                if (DUAL) s[H - 1] = x * b.y;
-            }
-            ok = mb_mbar_wait_spin(&acc_full[ac.slot], ac.full_parity(), status, abort_flag) && ok;
-            tc_after();
-            if (rows) {
-                const uint32_t from = tl + ac.slot * N;
-                float d[2][16];                            // the next chunk is on its way while this one is added
-                tc_ld16(from + column(0), d[0]);
-                tc_wait_ld(d[0]);
+        if constexpr (FP8) {
+            for (int kb = k0; kb < k1; kb += kUnit) {
+                // the scales of up to kUnit steps at once, so that a step has little but its sums
+                ok = bar_wait(sc_full + 8 * scr.slot, scr.full_parity(), status, abort_flag) && ok;
+                const float* from = sc + scr.slot * kScFloats;
+                float s[kUnit][H];
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    if (c + 1 < C) tc_ld16(from + column(c + 1), d[(c + 1) & 1]);
-                    const float f = s[DUAL && c >= C / 2 ? H - 1 : 0];
+                for (int u = 0; u < kUnit; ++u) {
+                    const float x = from[130 * u + 32 * q + lane];
+                    const float2 b = *reinterpret_cast<const float2*>(from + 130 * u + 128);
+                    s[u][0] = x * (!DUAL && WIDE && set >= kSets / 2 ? b.y : b.x);
+                    if (DUAL) s[u][H - 1] = x * b.y;
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(sc_empty + 8 * scr.slot);
+                scr.next();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        sum[c][i] = FP8 ? fmaf(d[c & 1][i], f, sum[c][i]) : sum[c][i] + d[c & 1][i];
-                    if (c + 1 < C) tc_wait_ld(d[(c + 1) & 1]);
+                for (int u = 0; u < kUnit; ++u) {
+                    if (kb + u >= k1) break;
+                    step(sum, s[u], rows, ok);
                 }
             }
-            const bool unit_done = FP8 && (us == kUnit - 1 || kb + 1 == k1);
-            us = unit_done ? 0 : us + 1;
-            tc_before();
-            __syncwarp();
-            if (lane == 0) {
-                mb_mbar_arrive(&acc_empty[ac.slot]);
-                if (unit_done) mb_mbar_arrive(&sc_empty[scr.slot]);
-            }
-            ac.next();
-            if (unit_done) scr.next();
+        } else {
+            const float one[H] = {};
+            for (int kb = k0; kb < k1; kb += a.prom) step(sum, one, rows, ok);
         }
 
         if (split > 1) {
@@ -308,6 +301,7 @@ struct Epilogue {
                 for (int r = 1; r < split; ++r) cluster_arrive(cluster_map(mb_smem_addr(red_empty), leader + r));
         }
 
+        if (!rows) return;
         if constexpr (DUAL) {
 #pragma unroll
             for (int c = 0; c < C / 2; ++c)
@@ -319,42 +313,65 @@ struct Epilogue {
         }
         const int n = ok ? min(32, w.nrows - 32 * q) : 0;  // rows of this quarter to write
         const int64_t row = (int64_t)w.row0 + 32 * q;
-        const int col = DUAL ? w.nb * kBlock + 64 * set : w.nb * N + S * set;
+        const int col = (DUAL ? w.nb * kBlock : w.nb * N) + R * set;
         if constexpr (OUT == MB_T_E4M3) {
             encode(sum, row, n, w.nb, col);
-        } else if (rows) {
-            constexpr int RC = kRun / out_bytes(OUT);      // columns of a run: 16 of f32, 32 of 16 bits
-            constexpr int R = (DUAL ? 64 : S) / RC, B = R < kBatch ? R : kBatch;   // runs; a batch of them
+        } else {
 #pragma unroll
-            for (int r0 = 0; r0 < R; r0 += B) {
+            for (int r0 = 0; r0 < R / RC; r0 += kBatch) {
                 begin();
 #pragma unroll
-                for (int r = r0; r < r0 + B; ++r)
+                for (int r = 0; r < kBatch; ++r)
 #pragma unroll
                     for (int j = 0; j < kRun / 16; ++j) {
-                        constexpr int VC = 16 / out_bytes(OUT);
-                        const int i = r * RC + j * VC;
+                        const int i = (r0 + r) * RC + j * (16 / B);
                         const float* v = &sum[i / 16][i % 16];
                         if constexpr (OUT == MB_T_F32)
-                            *run(r - r0, lane, j) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
-                                                               __float_as_uint(v[2]), __float_as_uint(v[3]));
+                            *run(r, lane, j) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                                          __float_as_uint(v[2]), __float_as_uint(v[3]));
                         else
-                            *run(r - r0, lane, j) = make_uint4(round2<OUT>(v[0], v[1]), round2<OUT>(v[2], v[3]),
-                                                               round2<OUT>(v[4], v[5]), round2<OUT>(v[6], v[7]));
+                            *run(r, lane, j) = make_uint4(round2<OUT>(v[0], v[1]), round2<OUT>(v[2], v[3]),
+                                                          round2<OUT>(v[4], v[5]), round2<OUT>(v[6], v[7]));
                     }
-                send<B>(row, n, col + r0 * RC);
+                send(row, n, col + r0 * RC);
             }
         }
     }
 
-    // 16 bytes j of row r in tile t of the batch: the four of a row change places every two rows (the 64-byte swizzle of the y maps),
+    // One accumulator: its sums, times s for e4m3, to the thread's.
+    __device__ __forceinline__ void step(float (&sum)[C][16], const float (&s)[H], bool rows, bool& ok)
+    {
+        ok = bar_wait(acc_full + 8 * ac.slot, ac.full_parity(), status, abort_flag) && ok;
+        tc_after();
+        if (rows) {
+            const uint32_t from = tl + ac.slot * N;
+            float d[2][16];                                // the next chunk is on its way while this one is added
+            tc_ld16(from + column(0), d[0]);
+            tc_wait_ld(d[0]);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float(&v)[16] = d[c & 1], (&next)[16] = d[(c + 1) & 1];
+                if (c + 1 < C) tc_ld16(from + column(c + 1), next);
+                const float f = s[DUAL && c >= C / 2 ? H - 1 : 0];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum[c][i] = FP8 ? fmaf(v[i], f, sum[c][i]) : sum[c][i] + v[i];
+                if (c + 1 < C) tc_wait_ld(next);
+            }
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(acc_empty + 8 * ac.slot);
+        ac.next();
+    }
+
+    // 16 bytes j of row r in tile t of the batch: a row's change places every two rows (the 64-byte swizzle of the y maps),
     // which keeps both the rows' and the runs' accesses on different banks.
     __device__ __forceinline__ uint4* run(int t, int r, int j) const
     {
-        return reinterpret_cast<uint4*>(tiles + (kTiles > 1 ? half * kBatch + t : t) * kTile + r * kRun + ((j ^ (r >> 1 & 3)) << 4));
+        return reinterpret_cast<uint4*>(tiles + (2 * half + t) * kTile + r * kRun + ((j ^ (r >> 1 & 3)) << 4));
     }
 
-    // The next batch's tiles have been read by whoever sent them.
+    // The tiles to be filled next have been read by whoever sent them.
     __device__ __forceinline__ void begin()
     {
         if (kTiles > 1) {
@@ -364,40 +381,36 @@ struct Epilogue {
         __syncwarp();
     }
 
-    // The batch's first T tiles' runs, each run next to the one before, to rows row .. row + n - 1 of y, from column col on (not
-    // past column O).
-    template <int T>
+    // The batch's tiles, a run next to a run, to rows row .. row + n - 1 of y, from column col on (not past column O).
     __device__ __forceinline__ void send(int64_t row, int n, int col)
     {
-        constexpr int B = out_bytes(OUT), RC = kRun / B;
         uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + (row * a.ldy + col) * B;
         int first = 0;                                     // rows before this one go by TMA, which knows where y ends
-        if (kTiles > 1 && a.vec) {
-            // a copy per lane: of 32 rows of a tile, or of 8 rows of as many as there are
-            first = max(n, 0) & ~7;
-            bulk_fence();
-            __syncwarp();
-            const int t = first == 32 ? lane : lane >> 2, r = first == 32 ? 0 : 8 * (lane & 3);
-            if (t < T && r < first && col + t * RC < a.O)
-                tma_store2(first == 32 ? ymaps : ymaps + 1, tiles + (half * kBatch + t) * kTile + r * kRun, col + t * RC,
-                           (int)row + r);
-        } else {
-            __syncwarp();
-        }
-        if (kTiles > 1) bulk_commit();
-        if (a.vec && col + T * RC <= a.O) {
-            if (first < n) {
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-#pragma unroll
-                    for (int i = 0; i < (kTiles > 1 ? 1 : 4); ++i) {
-                        const int r = first + 8 * i + (lane >> 2), j = lane & 3;
-                        if (r < n)
-                            *reinterpret_cast<uint4*>(dst + r * a.ldy * B + t * kRun + 16 * j) = *run(t, r, j);
-                    }
+        if (kTiles > 1) {
+            if (a.vec) {
+                // a copy per lane: of a tile's 32 rows, or of 8 rows of as many as there are
+                first = max(n, 0) & ~7;
+                bulk_fence();
+                __syncwarp();
+                const int t = first == 32 ? lane : lane >> 2, r = first == 32 ? 0 : 8 * (lane & 3);
+                if (t < kBatch && r < first && col + t * RC < a.O)
+                    tma_store2(first == 32 ? ymaps : ymaps + 1, tiles + (2 * half + t) * kTile + r * kRun, col + t * RC,
+                               (int)row + r);
             }
+            bulk_commit();
+        }
+        __syncwarp();
+        if (first >= n) return;
+        if (a.vec && col + kBatch * RC <= a.O) {
+#pragma unroll
+            for (int t = 0; t < kBatch; ++t)
+#pragma unroll
+                for (int i = 0; i < (kTiles > 1 ? 1 : 4); ++i) {
+                    const int r = first + 8 * i + (lane >> 2), j = lane & 3;
+                    if (r < n) *reinterpret_cast<uint4*>(dst + r * a.ldy * B + t * kRun + 16 * j) = *run(t, r, j);
+                }
         } else {
-            const int cols = min(T * RC, a.O - col);
+            const int cols = min(kBatch * RC, a.O - col);
             for (int r = first; r < n; ++r)
                 for (int i = lane; i < cols; i += 32) {
                     const uint8_t* from =
@@ -412,27 +425,29 @@ struct Epilogue {
         }
     }
 
-    // This thread's 64 activations of a row as e4m3, the row's scale over them and the other set's 64.
+    // This thread's R activations of a row as e4m3, the row's scale over them and the other sets'.
     __device__ __forceinline__ void encode(const float (&v)[C][16], int64_t row, int n, int nb, int col)
     {
         float m = 0.0f;
-        if (col + 64 <= a.O) {
+        if (col + R <= a.O) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) m = fmaxf(m, fabsf(v[i / 16][i % 16]));
+            for (int i = 0; i < R; ++i) m = fmaxf(m, fabsf(v[i / 16][i % 16]));
         } else {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) m = col + i < a.O ? fmaxf(m, fabsf(v[i / 16][i % 16])) : m;
+            for (int i = 0; i < R; ++i) m = col + i < a.O ? fmaxf(m, fabsf(v[i / 16][i % 16])) : m;
         }
-        float* am = amax + abuf * 2 * kMaxM + 32 * q + lane;
+        float* am = amax + abuf * kSets * kMaxM + 32 * q + lane;
         abuf ^= 1;
         am[set * kMaxM] = m;
-        mb_named_barrier(1 + q, 64);
-        const Quotient qu(e4m3_scale(fmaxf(am[0], am[kMaxM])));
+        mb_named_barrier(1 + q, 32 * kSets);
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) m = fmaxf(m, am[s * kMaxM]);
+        const Quotient qu(e4m3_scale(m));
         const bool fast = __all_sync(0xffffffffu, qu.fast || lane >= n);
         if (set == 0 && lane < n) a.qs[(row + lane) * a.qs_row + nb * a.qs_group] = qu.s;
         begin();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < R / 16; ++j) {
             uint32_t u[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -447,7 +462,7 @@ struct Epilogue {
             }
             *run(0, lane, j) = make_uint4(u[0], u[1], u[2], u[3]);
         }
-        send<1>(row, n, col);
+        send(row, n, col);
     }
 };
 
@@ -457,11 +472,11 @@ template <int R>
 __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
 template <int TYPE, bool DUAL, bool WIDE, bool SMALL, int OUT>
-__global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
+__global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Roles<SMALL, TYPE == MB_T_E4M3>::kCtas)
     grouped_kernel(const __grid_constant__ GroupedArgs a, const __grid_constant__ Maps maps)
 {
     using Epi = Epilogue<TYPE, DUAL, WIDE, SMALL, OUT>;
-    using Role = Roles<SMALL>;
+    using Role = typename Epi::Role;
     constexpr int kThreads = Role::kThreads, kWarps = Role::kWarps, kEpiWarps = Role::kEpiWarps;
     constexpr bool FP8 = TYPE == MB_T_E4M3;
     constexpr int KS = FP8 ? 128 : 64;    // columns of a K step
@@ -478,7 +493,7 @@ __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
     float4* red = reinterpret_cast<float4*>(stage0 + (size_t)a.stages * stage_bytes);
     uint8_t* tiles = reinterpret_cast<uint8_t*>(red + (csize - 1) * Epi::N / 4 * 32);   // 1024-byte aligned
     float* amax = reinterpret_cast<float*>(tiles + kEpiWarps * Epi::kTiles * kTile);
-    float* sc = amax + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM : 0);
+    float* sc = amax + (OUT == MB_T_E4M3 ? 2 * kSets * kMaxM : 0);
     uint64_t* full = reinterpret_cast<uint64_t*>(sc + (FP8 ? kScSlots * kScFloats : 0));
     uint64_t* empty = full + kMaxStages;
     uint64_t* acc_full = empty + kMaxStages;
@@ -492,8 +507,8 @@ __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
     Item* items = reinterpret_cast<Item*>(red_empty + 1);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kItemSlots);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [kWarps], [15]: split
-    int2* meta = reinterpret_cast<int2*>(wsum + 16);                   // [E]
+    int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [kWarps], [31]: split
+    int2* meta = reinterpret_cast<int2*>(wsum + 32);                   // [E]
     int* pstart = reinterpret_cast<int*>(meta + a.E);                  // [E + 1]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -572,7 +587,7 @@ __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
                     split = s;
                 }
             }
-            wsum[15] = split;
+            wsum[31] = split;
             mb_mbar_init(red_full, kEpiWarps * max(split - 1, 1));
             mb_mbar_init(red_empty, kEpiWarps);
             mb_fence_mbar_init();
@@ -584,7 +599,7 @@ __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
     tc_after();
 
     const uint32_t tmem = *tmem_slot;
-    const int split = wsum[15];
+    const int split = wsum[31];
     const int srank = (int)blockIdx.x % split;                          // rank among the CTAs of an item
     const int k0 = (int)((int64_t)a.Kb * srank / split), k1 = (int)((int64_t)a.Kb * (srank + 1) / split);
     ItemRing ring{items, item_full, item_empty, status, abort_flag, Ring(kItemSlots)};
@@ -593,39 +608,44 @@ __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
     if (!SMALL && warp < 4) setmaxnreg_dec<kLoadRegs>();
     if (warp == Role::kLoad) {
         // ------------------------------------------------------------------ loads
-        Ring st(a.stages);
-        bool ok = true;
-        int issued = 0;
-        while (ok && ring.pop<true>(w)) {
-            const int r16 = (w.nrows + 15) >> 4;
-            // lanes 0, 1: weight tiles; lane 2 + b: a box of 16 << b rows, the larger boxes first
-            const int b = lane - 2;
-            const bool box = b >= 0 && b < kRowMaps && ((r16 >> b) & 1);
-            const int brow = b >= 0 && b < kRowMaps ? ((r16 >> (b + 1)) << (b + 1)) * 16 : 0;
-            const int wrow = DUAL ? lane * a.O + w.nb * kBlock : (w.nb * NB + lane) * kBlock;
-            for (int kb = k0; kb < k1; ++kb, st.next()) {
-                ok = __all_sync(0xffffffffu, mb_mbar_wait_spin(&empty[st.slot], st.empty_parity(), status, abort_flag));
-                if (!ok) break;
-                uint8_t* dst = stage0 + (size_t)st.slot * stage_bytes;
-                if (lane == 0) mb_mbar_arrive_expect_tx(&full[st.slot], NB * kTileW + r16 * 16 * 128);
-                __syncwarp();
-                if (lane < NB)
-                    tma_load3(dst + a.MT * 128 + lane * kTileW, &maps.w, kb * KS, wrow, w.e, &full[st.slot]);
-                else if (box)
-                    tma_load2(dst + brow * 128, &maps.x[b], kb * KS, w.row0 + brow, &full[st.slot]);
-                ++issued;
-            }
-        }
-        if (!ok || *abort_flag) {   // wait (bounded) for the copies still in flight before the CTA may end
-            for (int i = 0; i < min(issued, a.stages); ++i) {
-                if (--st.slot < 0) {
-                    st.slot = a.stages - 1;
-                    st.phase ^= 1;
-                }
-                for (int n = 0; n < 100000 && !mb_mbar_try_wait(&full[st.slot], st.full_parity()); ++n) {
+        if (elect_one()) {
+            Ring st(a.stages);
+            bool ok = true;
+            int issued = 0;
+            const uint32_t stage0s = mb_smem_addr(stage0), fullb = mb_smem_addr(full), emptyb = mb_smem_addr(empty);
+            while (ok && ring.pop<false>(w)) {
+                const int r16 = (w.nrows + 15) >> 4;
+                const uint32_t bytes = NB * kTileW + r16 * 16 * 128;
+                for (int kb = k0; kb < k1; ++kb, st.next()) {
+                    ok = bar_wait(emptyb + 8 * st.slot, st.empty_parity(), status, abort_flag);
+                    if (!ok) break;
+                    const uint32_t dst = stage0s + st.slot * stage_bytes, bar = fullb + 8 * st.slot;
+                    bar_expect(bar, bytes);
+                    tma_load3(dst + a.MT * 128, &maps.w, kb * KS, DUAL ? w.nb * kBlock : w.nb * Epi::N, w.e, bar);
+                    if (DUAL)
+                        tma_load3(dst + a.MT * 128 + kTileW, &maps.w, kb * KS, a.O + w.nb * kBlock, w.e, bar);
+                    int row = 0;                           // boxes of 128, 64, 32, 16 rows: those that add up to the pass's
+#pragma unroll
+                    for (int b = kRowMaps - 1; b >= 0; --b)
+                        if (r16 >> b & 1) {
+                            tma_load2(dst + row * 128, &maps.x[b], kb * KS, w.row0 + row, bar);
+                            row += 16 << b;
+                        }
+                    ++issued;
                 }
             }
+            if (!ok || *abort_flag) {   // wait (bounded) for the copies still in flight before the CTA may end
+                for (int i = 0; i < min(issued, a.stages); ++i) {
+                    if (--st.slot < 0) {
+                        st.slot = a.stages - 1;
+                        st.phase ^= 1;
+                    }
+                    for (int n = 0; n < 100000 && !bar_try(fullb + 8 * st.slot, st.full_parity()); ++n) {
+                    }
+                }
+            }
         }
+        __syncwarp();
     } else if (warp == Role::kMma) {
         // ------------------------------------------------------------------ tensor cores
         if (elect_one()) {
@@ -635,22 +655,22 @@ __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
             constexpr uint32_t idesc = (1u << 4) | (TYPE == MB_T_BF16 ? (1u << 7) | (1u << 10) : 0u) |
                                        ((uint32_t)(Epi::N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             const uint64_t desc0 = tc_desc_sw128(mb_smem_addr(stage0));
+            const uint32_t fullb = mb_smem_addr(full), accb = mb_smem_addr(acc_empty);
+            const uint32_t step_w = a.MT * 128 >> 4, step_stage = stage_bytes >> 4;
             while (ok && ring.pop<false>(w)) {
                 int part = 0;                              // K steps already in the accumulator
                 for (int kb = k0; kb < k1; ++kb, st.next()) {
-                    if (part == 0)
-                        ok = mb_mbar_wait_spin(&acc_empty[ac.slot], ac.empty_parity(), status, abort_flag);
-                    ok = ok && mb_mbar_wait_spin(&full[st.slot], st.full_parity(), status, abort_flag);
+                    if (part == 0) ok = bar_wait(accb + 8 * ac.slot, ac.empty_parity(), status, abort_flag);
+                    ok = ok && bar_wait(fullb + 8 * st.slot, st.full_parity(), status, abort_flag);
                     if (!ok) break;
                     tc_after();
-                    const uint64_t dx = desc0 + (uint64_t)((st.slot * stage_bytes) >> 4);
-                    const uint64_t dw = dx + (uint64_t)(a.MT * 128 >> 4);
+                    const uint64_t dx = desc0 + st.slot * step_stage, dw = dx + step_w;
+                    const uint32_t d = tmem + ac.slot * Epi::N;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        tc_mma_ss<FP8>(tmem + ac.slot * Epi::N, dx + 2 * j, dw + 2 * j, idesc,
-                                       (j > 0 || part > 0) ? 1u : 0u);
+                        tc_mma_ss<FP8>(d, dx + 2 * j, dw + 2 * j, idesc, (j > 0 || part > 0) ? 1u : 0u);
                     tc_commit(&empty[st.slot]);
-                    if (++part == a.prom || kb + 1 == k1) {
+                    if (FP8 || ++part == a.prom || kb + 1 == k1) {
                         tc_commit(&acc_full[ac.slot]);
                         ac.next();
                         part = 0;
@@ -718,7 +738,8 @@ __global__ void __launch_bounds__(Roles<SMALL>::kThreads, Roles<SMALL>::kCtas)
         // ------------------------------------------------------------------ epilogue
         if (!SMALL) setmaxnreg_inc<kEpiRegs>();
         const int q = warp & 3, set = SMALL ? warp >> 2 : (warp >> 2) - 1;
-        Epi ep{a, status, abort_flag, tmem + ((uint32_t)(32 * q) << 16), acc_full, acc_empty, sc_full, sc_empty, sc, red,
+        Epi ep{a, status, abort_flag, tmem + ((uint32_t)(32 * q) << 16), mb_smem_addr(acc_full),
+               mb_smem_addr(acc_empty), mb_smem_addr(sc_full), mb_smem_addr(sc_empty), sc, red,
                red_full, red_empty, amax, tiles + (SMALL ? set : warp - 4) * Epi::kTiles * kTile, maps.y, split, srank,
                cluster_rank() - srank, q, set, lane, Ring(kAcc), Ring(kScSlots), 0, 0, 0};
         while (ring.pop<true>(w)) ep.item(w, k0, k1);
@@ -785,7 +806,7 @@ int check_args(const GroupedArgs& a, int type, int halves, const char* what)
 }
 
 
-int make_maps(const GroupedArgs& a, int type, int halves, int out, bool tiles, Maps* m, const char* what)
+int make_maps(const GroupedArgs& a, int type, int halves, int wrows, int out, bool tiles, Maps* m, const char* what)
 {
     const EncodeTiledFn fn = encode_fn();
     if (!fn) return mb_fail(MB_ECUDA, "%s: cuTensorMapEncodeTiled unavailable", what);
@@ -794,7 +815,7 @@ int make_maps(const GroupedArgs& a, int type, int halves, int out, bool tiles, M
     const cuuint64_t wd[3] = {(cuuint64_t)a.K, (cuuint64_t)a.O * halves, (cuuint64_t)a.E};
     const cuuint64_t wst[2] = {(cuuint64_t)a.ldw * b,
                                (cuuint64_t)(a.E > 1 ? a.w_expert : (int64_t)a.O * halves * a.ldw) * b};
-    const cuuint32_t wbox[3] = {inner, kBlock, 1};
+    const cuuint32_t wbox[3] = {inner, (cuuint32_t)wrows, 1};
     CUresult r = fn(&m->w, map_type(type), 3, const_cast<void*>(a.w), wd, wst, wbox, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     const cuuint64_t xd[2] = {(cuuint64_t)a.K, (cuuint64_t)a.P};
@@ -829,7 +850,7 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
 {
     constexpr bool FP8 = TYPE == MB_T_E4M3;
     constexpr int N = WIDE ? 256 : 128;
-    using Role = Roles<SMALL>;
+    using Role = Roles<SMALL, FP8>;
     const int slots = mb_num_sms() * Role::kCtas;
     const int64_t active = std::min<int64_t>(a.E, a.P);          // experts with rows, at most
     a.Kb = (a.K + (FP8 ? 127 : 63)) / (FP8 ? 128 : 64);
@@ -857,9 +878,9 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
         }
     }
     const int stage = a.MT * 128 + N * 128;
-    const int fixed = 1024 + (cluster - 1) * N * 128 + (OUT == MB_T_E4M3 ? 2 * 2 * kMaxM * 4 : 0) +
-                      (FP8 ? kScSlots * kScFloats * 4 : 0) + Role::kEpiWarps * Role::template kTiles<FP8> * kTile +
-                      (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2) * 8 + kItemSlots * 16 + 8 + 64 +
+    const int fixed = 1024 + (cluster - 1) * N * 128 + (OUT == MB_T_E4M3 ? 2 * kSets * kMaxM * 4 : 0) +
+                      (FP8 ? kScSlots * kScFloats * 4 : 0) + Role::kEpiWarps * Role::kTiles * kTile +
+                      (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2) * 8 + kItemSlots * 16 + 8 + 128 +
                       a.E * 8 + (a.E + 1) * 4 + 16;
     a.stages = std::min(kMaxStages, (Role::kMaxSmem - fixed) / stage);
     const int smem = fixed + a.stages * stage;
@@ -901,7 +922,7 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     }
     cfg.gridDim = (unsigned)std::min<int64_t>(ctas, items * cluster);
     Maps maps;
-    const int rc = make_maps(a, TYPE, DUAL ? 2 : 1, OUT, Role::template kTiles<FP8> > 1, &maps, what);
+    const int rc = make_maps(a, TYPE, DUAL ? 2 : 1, DUAL ? kBlock : N, OUT, Role::kTiles > 1, &maps, what);
     if (rc) return rc;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, maps);
     if (e != cudaSuccess) return mb_fail(MB_ECUDA, "%s: %s", what, cudaGetErrorString(e));
