@@ -41,6 +41,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "mb_common.cuh"
 #include "mb_float.cuh"
@@ -208,7 +209,7 @@ struct Epilogue {
     uint32_t tl;               // TMEM address of the warp's lane quarter
     uint32_t acc_full, acc_empty, sc_full, sc_empty;       // shared-memory addresses
     const float* sc;
-    float4* red;               // partial sums: [sender][set][S / 4][32 lanes]
+    float4* red;               // partial sums: [sender][set][S / 4][MT lanes]
     uint64_t *red_full, *red_empty;
     float* amax;               // [2][sets][128 rows]
     uint8_t* tiles;            // the warp's tiles of results
@@ -272,11 +273,13 @@ struct Epilogue {
                 ++sent;
                 if (rows && ok) {
                     const uint32_t to =
-                        cluster_map(mb_smem_addr(red + ((srank - 1) * 2 + set) * (S / 4) * 32 + lane), leader);
+                        cluster_map(mb_smem_addr(red + ((srank - 1) * 2 + set) * (S / 4) * a.MT + lane), leader);
+                    if (lane < a.MT) {
 #pragma unroll
-                    for (int j = 0; j < S / 4; ++j) {
-                        const float* v = &sum[j / 4][4 * (j % 4)];
-                        cluster_st4(to + j * 512, v[0], v[1], v[2], v[3]);
+                        for (int j = 0; j < S / 4; ++j) {
+                            const float* v = &sum[j / 4][4 * (j % 4)];
+                            cluster_st4(to + j * a.MT * 16, v[0], v[1], v[2], v[3]);
+                        }
                     }
                 }
                 __syncwarp();
@@ -285,12 +288,12 @@ struct Epilogue {
             }
             ok = mbar_wait_cluster(red_full, sent & 1, status, abort_flag) && ok;
             ++sent;
-            if (rows) {
+            if (rows && lane < a.MT) {
                 for (int r = 0; r < split - 1; ++r) {
-                    const float4* from = red + (r * 2 + set) * (S / 4) * 32 + lane;
+                    const float4* from = red + (r * 2 + set) * (S / 4) * a.MT + lane;
 #pragma unroll
                     for (int j = 0; j < S / 4; ++j) {
-                        const float4 v = from[j * 32];
+                        const float4 v = from[j * a.MT];
                         float* to = &sum[j / 4][4 * (j % 4)];
                         to[0] += v.x, to[1] += v.y, to[2] += v.z, to[3] += v.w;
                     }
@@ -410,18 +413,17 @@ struct Epilogue {
                     if (r < n) *reinterpret_cast<uint4*>(dst + r * a.ldy * B + t * kRun + 16 * j) = *run(t, r, j);
                 }
         } else {
-            const int cols = min(kBatch * RC, a.O - col);
-            for (int r = first; r < n; ++r)
-                for (int i = lane; i < cols; i += 32) {
-                    const uint8_t* from =
-                        reinterpret_cast<const uint8_t*>(run(i / RC, r, i % RC * B / 16)) + i * B % 16;
-                    if (B == 4)
-                        reinterpret_cast<uint32_t*>(dst + r * a.ldy * B)[i] = *reinterpret_cast<const uint32_t*>(from);
-                    else if (B == 2)
-                        reinterpret_cast<uint16_t*>(dst + r * a.ldy * B)[i] = *reinterpret_cast<const uint16_t*>(from);
-                    else
-                        dst[r * a.ldy + i] = *from;
-                }
+            // one result at a time, neighbours of a row next to each other
+            constexpr int W = kBatch * RC;
+            using U = typename std::conditional<B == 4, uint32_t, typename std::conditional<B == 2, uint16_t, uint8_t>::type>::type;
+            const int cols = min(W, a.O - col);
+#pragma unroll 8
+            for (int k = lane; k < 32 * W; k += 32) {
+                const int r = k / W, i = k % W;
+                if (r >= first && r < n && i < cols)
+                    reinterpret_cast<U*>(dst + r * a.ldy * B)[i] =
+                        reinterpret_cast<const U*>(run(i / RC, r, i % RC * B / 16))[i % (16 / B)];
+            }
         }
     }
 
@@ -491,7 +493,7 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
     const uint32_t csize = cluster_size();
     uint8_t* stage0 = smem;
     float4* red = reinterpret_cast<float4*>(stage0 + (size_t)a.stages * stage_bytes);
-    uint8_t* tiles = reinterpret_cast<uint8_t*>(red + (csize - 1) * Epi::N / 4 * 32);   // 1024-byte aligned
+    uint8_t* tiles = reinterpret_cast<uint8_t*>(red + (csize - 1) * Epi::N / 4 * a.MT);   // 1024-byte aligned
     float* amax = reinterpret_cast<float*>(tiles + kEpiWarps * Epi::kTiles * kTile);
     float* sc = amax + (OUT == MB_T_E4M3 ? 2 * kSets * kMaxM : 0);
     uint64_t* full = reinterpret_cast<uint64_t*>(sc + (FP8 ? kScSlots * kScFloats : 0));
@@ -533,8 +535,9 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
             mb_mbar_init(&item_empty[i], kEpiWarps + (FP8 ? 3 : 2));
         }
         *abort_flag = 0;
-        tma_prefetch_map(&maps.w);
     }
+    if (warp == Role::kLoad && lane < 1 + kRowMaps && (lane == 0 || 8 << lane <= a.MT))
+        tma_prefetch_map(lane == 0 ? &maps.w : &maps.x[lane - 1]);
     if (warp == Role::kMma) tc_alloc(tmem_slot, Role::kTmemCols);
     mb_pdl_wait();
 
@@ -867,7 +870,7 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
         const double meet = a.offsets ? a.E * (1.0 - std::pow(1.0 - 1.0 / a.E, (double)a.P)) : 1.0;
         const int64_t likely = std::max<int64_t>(1, (int64_t)(a.Nb * meet + 0.5));
         int64_t best = (int64_t)1 << 62;
-        for (int c = 1, extra = 0; c <= 8 && c <= a.Kb && (c - 1) * N * 128 <= kMaxRed; c *= 2) {
+        for (int c = 1, extra = 0; c <= 8 && c <= a.Kb && (c - 1) * N * a.MT * 4 <= kMaxRed; c *= 2) {
             const int64_t groups = slots / c, cost = (likely + groups - 1) / groups * ((a.Kb + c - 1) / c + (c > 1 ? 2 : 0)) +
                                                      extra;
             if (cost < best) {
@@ -878,7 +881,7 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
         }
     }
     const int stage = a.MT * 128 + N * 128;
-    const int fixed = 1024 + (cluster - 1) * N * 128 + (OUT == MB_T_E4M3 ? 2 * kSets * kMaxM * 4 : 0) +
+    const int fixed = 1024 + (cluster - 1) * N * a.MT * 4 + (OUT == MB_T_E4M3 ? 2 * kSets * kMaxM * 4 : 0) +
                       (FP8 ? kScSlots * kScFloats * 4 : 0) + Role::kEpiWarps * Role::kTiles * kTile +
                       (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2) * 8 + kItemSlots * 16 + 8 + 128 +
                       a.E * 8 + (a.E + 1) * 4 + 16;

@@ -649,3 +649,22 @@ def test_operand_rows_of_many_picks(D, src, dst, T, k, d):
     if s is not None:
         ws[bad] = 1.0
         assert torch.equal(s, ws)
+
+
+# ---- results whose rows no vector fits, and splits of every size ---------------------------------------
+
+@pytest.mark.parametrize("dtype", [E4M3, F16])
+@pytest.mark.parametrize("out", [F32, BF16, F16])
+def test_grouped_unaligned_rows_of_results(D, dtype, out):
+    """Odd O: rows of y start anywhere; large passes and small ones, full quarters and rests of them."""
+    check_grouped(D, [160, 35, 8, 1, 77], 1001, 272, dtype, out, 101, first=1, tail=3)
+    check_grouped(D, [3, 0, 17], 333, 144, dtype, out, 102, tail=2)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 32])
+def test_few_rows_long_columns_are_split(D, dtype, n):
+    """One expert's few rows over long columns: the K split, for passes of 16 and of 32 rows, and gate|up."""
+    check_grouped(D, [n], 130, 7168, dtype, F32, 110 + n)
+    check_grouped(D, [0, n, 0], 600, 2064, dtype, BF16, 111 + n)
+    check_swiglu(D, [n], 200, 4112, dtype, 112 + n)
