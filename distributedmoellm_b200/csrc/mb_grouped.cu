@@ -893,7 +893,10 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     int dev = 0;
     cudaGetDevice(&dev);
     if (!(ready >> (dev & 63) & 1)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Role::kMaxSmem);
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Role::kMaxSmem);
+        if (e == cudaSuccess)             // two small CTAs per SM, clusters of them included, need all of it
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                     cudaSharedmemCarveoutMaxShared);
         if (e != cudaSuccess) return mb_fail(MB_ECUDA, "%s: %s", what, cudaGetErrorString(e));
         ready |= 1ull << (dev & 63);
     }
