@@ -66,6 +66,7 @@ struct Roles {
     // their results by TMA, two tiles while the next two are filled, at the price of the fourth stage (which measured
     // nothing there, and 8% for 16-bit types).
     static constexpr int kTiles = !SMALL && FP8 ? 4 : 1;
+    static constexpr int kMaxRed = SMALL ? 48 << 10 : 32 << 10;   // shared memory for partial sums of a split
     static constexpr int kMaxSmem = SMALL ? 115712 : 232448;   // 227 KB of 228, or half of 228 less 1 KB
 };
 constexpr int kLoadRegs = 72, kEpiRegs = 216;
@@ -80,8 +81,7 @@ constexpr int kItemSlots = 4;
 constexpr int kMaxAcc = 4;
 constexpr int kMaxStages = 16;
 constexpr int kRowMaps = 4;               // boxes of 16, 32, 64, 128 rows of x
-constexpr int kMaxRed = 48 << 10;         // shared memory for partial sums of a split
-constexpr int kSmallRows = 32;            // rows of a small pass, at most; only these are split
+constexpr int kSmallRows = 32;            // rows of a small pass, at most
 constexpr int kRun = 64;                  // results leave in runs of 64 bytes a row ..
 constexpr int kTile = 32 * kRun;          // .. and tiles of 32 rows
 
@@ -209,7 +209,7 @@ struct Epilogue {
     uint32_t tl;               // TMEM address of the warp's lane quarter
     uint32_t acc_full, acc_empty, sc_full, sc_empty;       // shared-memory addresses
     const float* sc;
-    float4* red;               // partial sums: [sender][set][S / 4][MT lanes]
+    float4* red;               // partial sums: [sender][set][S / 4][MT rows]
     uint64_t *red_full, *red_empty;
     float* amax;               // [2][sets][128 rows]
     uint8_t* tiles;            // the warp's tiles of results
@@ -266,15 +266,15 @@ struct Epilogue {
         }
 
         if (split > 1) {
-            // at most 32 rows: the first lane quarter's two warps
+            const int me = 32 * q + lane;
             if (srank > 0) {
                 // the receiver has read the previous item's sums (the first wait passes at once)
                 ok = mbar_wait_cluster(red_empty, (sent & 1) ^ 1, status, abort_flag) && ok;
                 ++sent;
                 if (rows && ok) {
                     const uint32_t to =
-                        cluster_map(mb_smem_addr(red + ((srank - 1) * 2 + set) * (S / 4) * a.MT + lane), leader);
-                    if (lane < a.MT) {
+                        cluster_map(mb_smem_addr(red + ((srank - 1) * 2 + set) * (S / 4) * a.MT + me), leader);
+                    if (me < a.MT) {
 #pragma unroll
                         for (int j = 0; j < S / 4; ++j) {
                             const float* v = &sum[j / 4][4 * (j % 4)];
@@ -288,9 +288,9 @@ struct Epilogue {
             }
             ok = mbar_wait_cluster(red_full, sent & 1, status, abort_flag) && ok;
             ++sent;
-            if (rows && lane < a.MT) {
+            if (rows && me < a.MT) {
                 for (int r = 0; r < split - 1; ++r) {
-                    const float4* from = red + (r * 2 + set) * (S / 4) * a.MT + lane;
+                    const float4* from = red + (r * 2 + set) * (S / 4) * a.MT + me;
 #pragma unroll
                     for (int j = 0; j < S / 4; ++j) {
                         const float4 v = from[j * a.MT];
@@ -863,21 +863,24 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     const int64_t items = a.Nb * (active + a.P / a.MT);            // an upper bound
     MB_REQUIRE(items < (1ll << 30), "%s: %lld work items", what, (long long)items);
     int cluster = 1;
-    if (SMALL) {
+    if (!(WIDE && !SMALL)) {
         // The split with the fewest K steps in turn on the busiest CTA, the launch of clusters counted as steps too (it
-        // measured 1, 3 and 6 us for 2, 4 and 8 CTAs, a step 0.35 us).  Experts with rows: those that P picks of E meet,
-        // each as likely as another.
+        // measured 1, 3 and 6 us for 2, 4 and 8 CTAs of small passes, a step 0.35 us; passes of 64 rows have more sums to
+        // send, and with 128 rows the split lost: 17.8 us against 16.0 at 128 x 4096 x 4096).  Clusters get one CTA per
+        // SM, which is what the occupancy query grants them.  Experts with rows: those that P picks of E meet, each as
+        // likely as another.
         const double meet = a.offsets ? a.E * (1.0 - std::pow(1.0 - 1.0 / a.E, (double)a.P)) : 1.0;
-        const int64_t likely = std::max<int64_t>(1, (int64_t)(a.Nb * meet + 0.5));
+        const double passes = std::max(meet, (double)((a.P + a.MT - 1) / a.MT));
+        const int64_t likely = std::max<int64_t>(1, (int64_t)(a.Nb * passes + 0.5));
         int64_t best = (int64_t)1 << 62;
-        for (int c = 1, extra = 0; c <= 8 && c <= a.Kb && (c - 1) * N * a.MT * 4 <= kMaxRed; c *= 2) {
-            const int64_t groups = slots / c, cost = (likely + groups - 1) / groups * ((a.Kb + c - 1) / c + (c > 1 ? 2 : 0)) +
-                                                     extra;
+        for (int c = 1, extra = 0; c <= 8 && c <= a.Kb && (c - 1) * N * a.MT * 4 <= Role::kMaxRed; c *= 2) {
+            const int64_t groups = (c == 1 ? slots : slots / Role::kCtas) / c;
+            const int64_t cost = (likely + groups - 1) / groups * ((a.Kb + c - 1) / c + (c > 1 ? 2 : 0)) + extra;
             if (cost < best) {
                 best = cost;
                 cluster = c;
             }
-            extra = c == 1 ? 3 : 2 * extra + 3;
+            extra = c == 1 ? (SMALL ? 3 : 9) : 2 * extra + 3;
         }
     }
     const int stage = a.MT * 128 + N * 128;

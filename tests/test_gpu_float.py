@@ -668,3 +668,11 @@ def test_few_rows_long_columns_are_split(D, dtype, n):
     check_grouped(D, [n], 130, 7168, dtype, F32, 110 + n)
     check_grouped(D, [0, n, 0], 600, 2064, dtype, BF16, 111 + n)
     check_swiglu(D, [n], 200, 4112, dtype, 112 + n)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("n", [33, 64, 65, 100, 128, 200])
+def test_ordinary_rows_long_columns_are_split(D, dtype, n):
+    """Large passes on few items: clusters of two over K, every lane quarter full, ragged or empty."""
+    check_grouped(D, [n], 300, 4096, dtype, F32, 130 + n, tail=1)
+    check_grouped(D, [0, n, 3], 260, 2064, dtype, BF16, 131 + n, first=2)
