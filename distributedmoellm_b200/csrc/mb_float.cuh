@@ -13,13 +13,10 @@ constexpr int kScaleBlock = MB_SCALE_BLOCK;
 // small that the quotient underflows), as mb_encode_rows does for int8.
 __device__ __forceinline__ float e4m3_scale(float m)
 {
-    const float r = 1.0f / 448.0f, q = m * r;              // see quotient()
+    const float r = 1.0f / 448.0f, q = m * r;              // see Quotient
     const float s = m > 0x1p-100f && m < 0x1p120f ? fmaf(fmaf(-q, 448.0f, m), r, q) : __fdiv_rn(m, 448.0f);
     return s == 0.0f ? 1.0f : s;
 }
-
-// Nearest e4m3 (ties to even).  Saturation matters only where s is subnormal: x / s may then round to above 448.
-__device__ __forceinline__ uint8_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 
 // x / s, correctly rounded, for many x and one s: r = 1 / s correctly rounded, then one correction of x * r by its
 // remainder (Markstein, IBM J. Res. Dev. 34, 1990).  Holds while nothing leaves the normal range, which `fast` says: with
@@ -32,13 +29,8 @@ struct Quotient {
     {
     }
 };
-__device__ __forceinline__ float quotient(float x, float s, float r)
-{
-    const float q = x * r;
-    return copysignf(fmaf(fmaf(-q, s, x), r, q), x);       // the correction would turn -0 into +0
-}
 
-// quotient() of four values by one s, two at a time in packed arithmetic.
+// x[i] / s for four values, two at a time in packed arithmetic.
 __device__ __forceinline__ void quotient4(float (&x)[4], float s, float r)
 {
     uint64_t s2, r2;
@@ -53,12 +45,13 @@ __device__ __forceinline__ void quotient4(float (&x)[4], float s, float r)
         asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e) : "l"(q), "l"(s2), "l"(v));
         asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(q) : "l"(e), "l"(r2), "l"(q));
         asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(q));
-        x[i] = copysignf(lo, x[i]);
+        x[i] = copysignf(lo, x[i]);                        // the correction turns -0 into +0
         x[i + 1] = copysignf(hi, x[i + 1]);
     }
 }
 
-// Nearest e4m3 of two values, as bytes lo, hi.
+// Nearest e4m3 (ties to even) of two values, as bytes lo, hi.  Saturation matters only where s is subnormal: x / s may
+// then round to above 448.
 __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi)
 {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);

@@ -884,12 +884,15 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
         }
     }
     const int stage = a.MT * 128 + N * 128;
-    const int fixed = 1024 + (cluster - 1) * N * a.MT * 4 + (OUT == MB_T_E4M3 ? 2 * kSets * kMaxM * 4 : 0) +
-                      (FP8 ? kScSlots * kScFloats * 4 : 0) + Role::kEpiWarps * Role::kTiles * kTile +
+    const int fixed = 1024 + (OUT == MB_T_E4M3 ? 2 * kSets * kMaxM * 4 : 0) + (FP8 ? kScSlots * kScFloats * 4 : 0) +
+                      Role::kEpiWarps * Role::kTiles * kTile +
                       (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2) * 8 + kItemSlots * 16 + 8 + 128 +
                       a.E * 8 + (a.E + 1) * 4 + 16;
-    a.stages = std::min(kMaxStages, (Role::kMaxSmem - fixed) / stage);
-    const int smem = fixed + a.stages * stage;
+    // a split's partial sums may leave too few stages beside the tables of very many experts: then a smaller split
+    while (cluster > 1 && (Role::kMaxSmem - fixed - (cluster - 1) * N * a.MT * 4) / stage < 2) cluster /= 2;
+    const int used = fixed + (cluster - 1) * N * a.MT * 4;
+    a.stages = std::min(kMaxStages, (Role::kMaxSmem - used) / stage);
+    const int smem = used + a.stages * stage;
 
     auto kern = grouped_kernel<TYPE, DUAL, WIDE, SMALL, OUT>;
     static thread_local uint64_t ready = 0;                        // devices whose attribute is set

@@ -676,3 +676,84 @@ def test_ordinary_rows_long_columns_are_split(D, dtype, n):
     """Large passes on few items: clusters of two over K, every lane quarter full, ragged or empty."""
     check_grouped(D, [n], 300, 4096, dtype, F32, 130 + n, tail=1)
     check_grouped(D, [0, n, 3], 260, 2064, dtype, BF16, 131 + n, first=2)
+
+
+# ---- slices of a layer, captured splits, other streams ---------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [E4M3, F16])
+def test_slices_of_experts_add_up_to_the_layer(D, dtype):
+    """run_experts over a slice of the experts and the matching slice of the routing (expert parallelism): the slices write
+    their own picks' rows only, and together every row as the whole layer has it."""
+    from distributedmoellm_b200 import layer as Lyr
+    from distributedmoellm_b200.store import FloatExperts
+    E, H, I, k, T = 8, 272, 144, 3, 40
+    layer, _ = float_layer(dtype, E, H, I, k, 93)
+    x = torch.randn((T, H), generator=gen(7), device="cuda")
+    layer(x)
+    b = layer.buffers(T)
+    P = T * k
+    whole = b.y[:P].clone()
+    off = b.routing.offsets.tolist()
+    y = torch.full((P, H), 5.0, device="cuda")
+    bufs = {}
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for e0, e1 in ((0, 3), (3, 8)):
+        ex = FloatExperts(e1 - e0, H, I, dtype, "cuda")
+        ex.gu, ex.down = layer.experts.gu[e0:e1], layer.experts.down[e0:e1]
+        if dtype == E4M3:
+            ex.gu_s, ex.dn_s = layer.experts.gu_s[e0:e1], layer.experts.dn_s[e0:e1]
+        r = D.Routing.from_plan(b.routing.counts[e0:e1], b.routing.offsets[e0:e1 + 1], b.routing.sorted_rows[:P])
+        Lyr.run_experts(ex, x, b.row_exp, r, y,
+                        lambda name, n: bufs.setdefault((name, n), torch.empty(n, dtype=torch.uint8, device="cuda")),
+                        st, 12)
+        assert torch.equal(y[off[e0]:off[e1]], whole[off[e0]:off[e1]])
+        if e1 < E:
+            assert (y[off[e1]:] == 5.0).all()
+    assert torch.equal(y, whole) and int(st) == 0
+
+
+def test_captured_split_replays_on_several_streams(D):
+    """A call split over K (clusters), captured without a call before it at this size, replayed on two streams at once."""
+    x, w, off, xs, ws = _product_inputs(E4M3, seed=95, counts=(3, 0, 2), O=392, K=5008)
+    y = [torch.zeros((5, 392), device="cuda") for _ in range(2)]
+    graphs = []
+    for o in y:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            D.grouped_matmul_t(x, w, off, xs, ws, y=o)
+        graphs.append(g)
+    want = D.grouped_matmul_t(x, w, off, xs, ws)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y[0], want) and torch.equal(y[1], want)
+
+
+def test_one_row_may_be_asked_for_twice_and_rows_shared(D):
+    """The same pick several times, and x's rows taken from an expanded row: every copy is the same."""
+    x = torch.randn((1, 256), generator=gen(96), device="cuda").expand(6, 256)
+    q, s = D.operand_rows(x.contiguous(), E4M3, rows=torch.tensor([5, 5, 0, 5], dtype=torch.int32, device="cuda"))
+    assert all(same_bits(q[i], q[0]) and torch.equal(s[i], s[0]) for i in range(4))
+    with pytest.raises(RuntimeError, match="closer"):
+        D.operand_rows(x, E4M3)                    # a row distance of 0 is refused
+    w = torch.zeros((1, 64, 256), dtype=BF16, device="cuda").expand(3, 64, 256)
+    with pytest.raises(RuntimeError, match="overlap"):
+        D.grouped_matmul_t(x.to(BF16).contiguous(), w, offsets_of([2, 2, 2]))
+    with pytest.raises(RuntimeError, match="16 bytes"):
+        D.grouped_matmul_t(torch.zeros((6, 100), dtype=BF16, device="cuda"), torch.zeros((3, 64, 100), dtype=BF16,
+                                                                                      device="cuda"), offsets_of([2, 2, 2]))
+
+
+def test_1024_experts_with_long_columns(D):
+    """Large tables beside the stages and a split's partial sums."""
+    counts = [0] * 1024
+    counts[3], counts[1023] = 2, 20
+    for dtype in (E4M3, BF16):
+        check_grouped(D, counts, 40, 2064, dtype, F32, 141)
+        check_swiglu(D, counts, 40, 1040, dtype, 142)
+        counts[5] = 300
+        check_swiglu(D, counts, 40, 528, dtype, 143)
