@@ -254,7 +254,7 @@ int launch(const SRC* x, int64_t ldx, int64_t n_src, const int32_t* rows, int64_
     const int ng = (d + kScaleBlock - 1) / kScaleBlock;
     const int64_t smem = (int64_t)kSpreadRows * (d * B + ng * 4);
     if (rows && vec && n >= 4 * n_src && n_src >= kSpreadRows * mb_num_sms() && n_src <= 4 * (int64_t)d &&
-        smem <= 40 << 10 && d * B % 16 == 0 && ldq * B % 16 == 0 && (uintptr_t)q % 16 == 0) {
+        smem <= 39 << 10 && d * B % 16 == 0 && ldq * B % 16 == 0 && (uintptr_t)q % 16 == 0) {
         const cudaError_t e = mb_launch_pdl(spread_rows_kernel<SRC, TYPE>,
                                             dim3((unsigned)((n_src + kSpreadRows - 1) / kSpreadRows)), dim3(256),
                                             (size_t)smem, st, x, ldx, (int)n_src, rows, (int)n, d, (uint8_t*)q, ldq * B,

@@ -369,6 +369,9 @@ def _rows_of(t, name):
 
 def _operand_stride(t, name):
     """As :func:`_rows_of`; a single row's distance is rounded up to 16 bytes, since nothing lies behind it."""
+    st = t.stride()
+    if st[-1] == 1 and t.shape[-2] > 1:
+        return st[-2]
     ld = _rows_of(t, name)
     if t.shape[-2] <= 1:
         step = 16 // t.element_size()

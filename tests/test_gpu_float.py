@@ -757,3 +757,11 @@ def test_1024_experts_with_long_columns(D):
         check_swiglu(D, counts, 40, 1040, dtype, 142)
         counts[5] = 300
         check_swiglu(D, counts, 40, 528, dtype, 143)
+
+
+@pytest.mark.parametrize("d", [2480, 2496, 2504, 2520, 2536])
+def test_operand_rows_of_many_picks_at_the_shared_memory_limit(D, d):
+    x = torch.randn((1200, d), generator=gen(d), device="cuda")
+    rows = torch.arange(1200, device="cuda", dtype=torch.int32).repeat(4)
+    q, _ = D.operand_rows(x, BF16, rows=rows)
+    assert torch.equal(q, x[rows.long()].to(BF16))
