@@ -11,8 +11,8 @@
 // Two kernels.  operand_rows_kernel makes each row of the result from its row of x; bound by instructions (about 200 a
 // warp) when tokens have many picks, since every pick of a token repeats the work.  spread_rows_kernel makes each row
 // of x once, into shared memory, looks through `rows` for its picks and copies the row to them.  Looking costs
-// n * 4 bytes per eight rows of x, which pays for many picks of not too many rows: 32768 rows of 2048 columns from 4096
-// rows of f32 take 43 us the first way and 34 the second.
+// n * 4 bytes per sixteen rows of x, which pays for many picks of not too many rows: 32768 rows of 2048 columns from 4096
+// rows of f32 take 43 us the first way and 29 the second.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -153,13 +153,15 @@ __global__ void operand_rows_kernel(const SRC* __restrict__ x, int64_t ldx, int6
     }
 }
 
-constexpr int kSpreadRows = 8;            // rows of x of a block, one per warp
-constexpr int kSegment = 4096;            // picks looked through at a time: 12 bits, next to 4 of the row found
+constexpr int kSpreadRows = 16;           // rows of x of a block, one per warp
+constexpr int kSpreadThreads = 32 * kSpreadRows;
+constexpr int kSegment = 4 * kSpreadThreads;   // picks looked through at a time
+constexpr int kSpreadSmem = 88 << 10;     // for the rows, at most: two blocks per SM
 
-// Eight rows of x, each put into operand form once and copied to its picks.  Block 0 takes the picks of no row of x.
+// Sixteen rows of x, each put into operand form once and copied to its picks.  Block 0 takes the picks of no row of x.
 // Needs 16 bytes at a time to be aligned in q, four columns in x, and d * bytes a multiple of 16.
 template <typename SRC, int TYPE>
-__global__ void __launch_bounds__(256) spread_rows_kernel(const SRC* __restrict__ x, int64_t ldx, int n_src,
+__global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const SRC* __restrict__ x, int64_t ldx, int n_src,
                                                           const int32_t* __restrict__ rows, int n, int d,
                                                           uint8_t* __restrict__ q, int64_t ldq_bytes,
                                                           float* __restrict__ scales, int64_t s_row, int64_t s_group,
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const SRC* __restrict_
 {
     constexpr int B = TYPE == MB_T_E4M3 ? 1 : 2;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint16_t found[kSegment];
+    __shared__ uint16_t found[kSegment], slots[kSegment];
     __shared__ int count;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ng = (d + kScaleBlock - 1) / kScaleBlock, bytes = d * B;
@@ -176,12 +178,13 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const SRC* __restrict_
     mb_pdl_trigger();
     mb_pdl_wait();
 
-    int idx[kSegment / 256];                               // the next segment, on its way
-    auto load = [&](int base) {
+    int idx[kSegment / kSpreadThreads];                    // the next segment, on its way
+    const int none = blockIdx.x == 0 ? kSpreadRows : 0;    // a row of x that is not this block's (there are more than 16)
+    auto load = [&](int64_t base) {
 #pragma unroll
-        for (int j = 0; j < kSegment / 256; ++j) {
-            const int p = base + 256 * j + threadIdx.x;
-            idx[j] = p < n ? rows[p] : r0 + kSpreadRows;   // (another block's row, or none: see below)
+        for (int j = 0; j < kSegment / kSpreadThreads; ++j) {
+            const int64_t p = base + kSpreadThreads * j + threadIdx.x;
+            idx[j] = p < n ? rows[p] : none;
         }
     };
     load(0);
@@ -208,27 +211,26 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const SRC* __restrict_
             }
         }
     }
-    for (int base = 0; base < n; base += kSegment) {
+    const unsigned mine = min(kSpreadRows, n_src - r0);
+    for (int64_t base = 0; base < n; base += kSegment) {
         if (threadIdx.x == 0) count = 0;
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < kSegment / 256; ++j) {
-            const int i = 256 * j + threadIdx.x, p = base + i;
-            int slot = -1;
-            if (p < n) {
-                if (idx[j] < 0 || idx[j] >= n_src)
-                    slot = blockIdx.x == 0 ? kSpreadRows : -1;
-                else if (idx[j] >= r0 && idx[j] < r0 + kSpreadRows)
-                    slot = idx[j] - r0;
+        for (int j = 0; j < kSegment / kSpreadThreads; ++j) {
+            unsigned slot = (unsigned)idx[j] - (unsigned)r0;
+            if (blockIdx.x == 0 && (unsigned)idx[j] >= (unsigned)n_src) slot = kSpreadRows;
+            if (slot < mine || (blockIdx.x == 0 && slot == kSpreadRows && idx[j] != kSpreadRows)) {
+                const int k = atomicAdd(&count, 1);        // (their order varies; every pick is one row's copy)
+                found[k] = (uint16_t)(kSpreadThreads * j + threadIdx.x);
+                slots[k] = (uint16_t)slot;
             }
-            if (slot >= 0) found[atomicAdd(&count, 1)] = (uint16_t)(i | slot << 12);
         }
         __syncthreads();
         const int c = count;
         if (base + kSegment < n) load(base + kSegment);
-        for (int k = warp; k < c; k += 8) {                // (the order of `found` varies; every pick is one row's copy)
-            const int slot = found[k] >> 12;
-            const int64_t p = base + (found[k] & (kSegment - 1));
+        for (int k = warp; k < c; k += kSpreadRows) {
+            const int slot = slots[k];
+            const int64_t p = base + found[k];
             const bool real = slot < kSpreadRows;
             if (!real && lane == 0 && status) atomicOr(status, MB_STATUS_BADARG);
             uint8_t* dst = q + p * ldq_bytes;
@@ -249,16 +251,25 @@ int launch(const SRC* x, int64_t ldx, int64_t n_src, const int32_t* rows, int64_
     constexpr int B = TYPE == MB_T_E4M3 ? 1 : 2;
     const bool vec = d % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 && (uintptr_t)x % (4 * sizeof(SRC)) == 0 &&
                      (uintptr_t)q % (4 * B) == 0;
-    // Worth it from four picks a row on, with enough rows for every SM, and few enough that looking through the picks
-    // (4 n bytes for each eight rows) stays below reading x for each pick.
+    // Worth it from four picks a row on, with enough rows for half of the SMs, and few enough that looking through the
+    // picks (4 n bytes for each 16 rows) stays below reading x for each pick.
     const int ng = (d + kScaleBlock - 1) / kScaleBlock;
     const int64_t smem = (int64_t)kSpreadRows * (d * B + ng * 4);
-    if (rows && vec && n >= 4 * n_src && n_src >= kSpreadRows * mb_num_sms() && n_src <= 4 * (int64_t)d &&
-        smem <= 39 << 10 && d * B % 16 == 0 && ldq * B % 16 == 0 && (uintptr_t)q % 16 == 0) {
-        const cudaError_t e = mb_launch_pdl(spread_rows_kernel<SRC, TYPE>,
-                                            dim3((unsigned)((n_src + kSpreadRows - 1) / kSpreadRows)), dim3(256),
-                                            (size_t)smem, st, x, ldx, (int)n_src, rows, (int)n, d, (uint8_t*)q, ldq * B,
-                                            scales, s_row, s_group, status);
+    if (rows && vec && n >= 4 * n_src && n_src >= kSpreadRows / 2 * mb_num_sms() && n_src <= 8 * (int64_t)d &&
+        smem <= kSpreadSmem && d * B % 16 == 0 && ldq * B % 16 == 0 && (uintptr_t)q % 16 == 0) {
+        static thread_local uint64_t ready = 0;            // devices whose attribute is set
+        int dev = 0;
+        cudaGetDevice(&dev);
+        cudaError_t e = cudaSuccess;
+        if (!(ready >> (dev & 63) & 1))
+            e = cudaFuncSetAttribute(spread_rows_kernel<SRC, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     kSpreadSmem);
+        if (e == cudaSuccess) {
+            ready |= 1ull << (dev & 63);
+            e = mb_launch_pdl(spread_rows_kernel<SRC, TYPE>, dim3((unsigned)((n_src + kSpreadRows - 1) / kSpreadRows)),
+                              dim3(kSpreadThreads), (size_t)smem, st, x, ldx, (int)n_src, rows, (int)n, d, (uint8_t*)q,
+                              ldq * B, scales, s_row, s_group, status);
+        }
         if (e != cudaSuccess) return mb_fail(MB_ECUDA, "mb_operand_rows: %s", cudaGetErrorString(e));
         return MB_OK;
     }
