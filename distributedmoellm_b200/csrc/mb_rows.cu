@@ -11,8 +11,9 @@
 // Two kernels.  operand_rows_kernel makes each row of the result from its row of x; bound by instructions (about 200 a
 // warp) when tokens have many picks, since every pick of a token repeats the work.  spread_rows_kernel makes each row
 // of x once, into shared memory, looks through `rows` for its picks and copies the row to them.  Looking costs
-// n * 4 bytes per sixteen rows of x, which pays for many picks of not too many rows: 32768 rows of 2048 columns from 4096
-// rows of f32 take 43 us the first way and 29 the second.
+// n * 4 bytes per sixteen rows of x, which pays for many picks of not too many rows.  us, first way / second, rows of
+// 2048 columns from f32: 32768 from 4096 44.9 / 31 (3.3 TB/s), 16384 from 4096 23.8 / 19, 18944 from 2368 26.1 / 19.2,
+// 9472 from 2368 13.7 / 11.8.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -251,11 +252,12 @@ int launch(const SRC* x, int64_t ldx, int64_t n_src, const int32_t* rows, int64_
     constexpr int B = TYPE == MB_T_E4M3 ? 1 : 2;
     const bool vec = d % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 && (uintptr_t)x % (4 * sizeof(SRC)) == 0 &&
                      (uintptr_t)q % (4 * B) == 0;
-    // Worth it from four picks a row on, with enough rows for half of the SMs, and few enough that looking through the
-    // picks (4 n bytes for each 16 rows) stays below reading x for each pick.
+    // Worth it from four picks a row on, with a block of rows for every SM (16384 from 2048 rows: 23.7 us, made for each
+    // pick 22.5; 9600 from 1200: 19.1 and 13.2), and few enough rows that looking through the picks (4 n bytes for each
+    // 16 rows) stays below reading x for each pick.
     const int ng = (d + kScaleBlock - 1) / kScaleBlock;
     const int64_t smem = (int64_t)kSpreadRows * (d * B + ng * 4);
-    if (rows && vec && n >= 4 * n_src && n_src >= kSpreadRows / 2 * mb_num_sms() && n_src <= 8 * (int64_t)d &&
+    if (rows && vec && n >= 4 * n_src && n_src >= kSpreadRows * mb_num_sms() && n_src <= 8 * (int64_t)d &&
         smem <= kSpreadSmem && d * B % 16 == 0 && ldq * B % 16 == 0 && (uintptr_t)q % 16 == 0) {
         static thread_local uint64_t ready = 0;            // devices whose attribute is set
         int dev = 0;

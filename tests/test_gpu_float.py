@@ -765,3 +765,18 @@ def test_operand_rows_of_many_picks_at_the_shared_memory_limit(D, d):
     rows = torch.arange(1200, device="cuda", dtype=torch.int32).repeat(4)
     q, _ = D.operand_rows(x, BF16, rows=rows)
     assert torch.equal(q, x[rows.long()].to(BF16))
+
+
+@pytest.mark.parametrize("src,dst,T,k,d", [(F32, E4M3, 2368, 8, 512), (F32, E4M3, 2367, 8, 512), (F32, E4M3, 2371, 5, 400),
+                                           (BF16, E4M3, 2500, 4, 2048), (F32, BF16, 2400, 6, 768), (F16, F16, 2433, 4, 1032)])
+def test_operand_rows_of_many_picks_of_many_rows(D, src, dst, T, k, d):
+    """Rows for every SM's blocks of sixteen, the last block ragged, and one row fewer than that."""
+    test_operand_rows_of_many_picks(D, src, dst, T, k, d)
+
+
+@pytest.mark.parametrize("d", [2752, 2760, 2768, 2776, 2784])
+def test_operand_rows_of_many_rows_at_the_shared_memory_limit(D, d):
+    x = torch.randn((2400, d), generator=gen(d), device="cuda")
+    rows = torch.arange(2400, device="cuda", dtype=torch.int32).repeat(4)
+    q, _ = D.operand_rows(x, BF16, rows=rows)
+    assert torch.equal(q, x[rows.long()].to(BF16))
