@@ -8,6 +8,9 @@ and bound with ctypes) for:
   weighted combine;
 * fused decode mat-vecs over packed experts (gate|up, SiLU, down);
 * grouped GEMMs on the tcgen05 tensor cores for prefill-sized batches;
+* experts in float8 e4m3 with block scales, bf16 or f16: operand rows and
+  grouped products (device.operand_rows, grouped_swiglu_t, grouped_matmul_t,
+  matmul_t_e4m3; store.FloatExperts);
 * expert parallelism over NCCL (ep.py).
 
 ``install()`` swaps them in behind moelan's own entry points (its kernels
