@@ -780,3 +780,52 @@ def test_operand_rows_of_many_rows_at_the_shared_memory_limit(D, d):
     rows = torch.arange(2400, device="cuda", dtype=torch.int32).repeat(4)
     q, _ = D.operand_rows(x, BF16, rows=rows)
     assert torch.equal(q, x[rows.long()].to(BF16))
+
+
+# ---- results of more than 2^31 values -----------------------------------------------------------------
+
+ENDS = (slice(0, 130), slice(-130, None))
+
+
+@pytest.mark.parametrize("T,P", [(100, 1_060_000), (2400, 1_060_000)])
+def test_operand_rows_past_32_bits(D, T, P):
+    """Made for each pick, and made once and copied."""
+    x = torch.randn((T, 2048), generator=gen(T), device="cuda")
+    rows = torch.randint(0, T, (P,), generator=gen(P), device="cuda", dtype=torch.int32)
+    q, s = D.operand_rows(x, E4M3, rows=rows)
+    assert q.numel() > 2 ** 31
+    for r in ENDS:
+        wq, ws = plain_e4m3(x[rows[r].long()])
+        assert same_bits(q[r], wq) and torch.equal(s[r], ws)
+
+
+@pytest.mark.parametrize("dtype,O", [(E4M3, 14336), (E4M3, 14337), (F16, 14336)])
+def test_grouped_past_32_bits(D, dtype, O):
+    """Results by TMA, one at a time, and by vectors."""
+    g = gen(O)
+    P, K, E = 151_000, 64, 2
+    x, xs, xw = rand_rows((P, K), dtype, g)
+    w, ws, ww = rand_weights((E, O, K), dtype, g)
+    off = offsets_of([70_001, P - 70_001])
+    y = D.grouped_matmul_t(x, w, off, xs, ws, dtype=BF16)
+    assert y.numel() > 2 ** 31
+    for e, r in enumerate(ENDS):
+        want, S = xw[r] @ ww[e].t(), xw[r].abs() @ ww[e].abs().t()
+        close(y[r], want, sum_tol(K, S) + round_tol(want, BF16), str(r))
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+def test_swiglu_past_32_bits(D, dtype):
+    g = gen(81)
+    P, K, I = 151_000, 64, 14336
+    x, xs, xw = rand_rows((P, K), dtype, g)
+    w, ws, ww = rand_weights((1, 2, I, K), dtype, g, scale=3.0 / K ** 0.5)
+    q, s = D.grouped_swiglu_t(x, w.view(1, 2 * I, K), offsets_of([P]), xs, ws)
+    assert q.numel() > 2 ** 31
+    for r in ENDS:
+        a, tol, _ = want_swiglu(xw[r], ww.view(1, 2 * I, K), offsets_of([130]), I, K)
+        if dtype != E4M3:
+            close(q[r], a, tol + round_tol(a, dtype), str(r))
+            continue
+        sw = s[r].double().repeat_interleave(G, 1)
+        close(q[r].double() * sw, a, tol * 17 / 16 + 2.0 ** -4 * a.abs() * (1 + 2.0 ** -20) + 2.0 ** -10 * sw, str(r))
