@@ -421,7 +421,8 @@ struct Epilogue {
         } else {
             // one result at a time, neighbours of a row next to each other
             constexpr int W = kBatch * RC;
-            using U = typename std::conditional<B == 4, uint32_t, typename std::conditional<B == 2, uint16_t, uint8_t>::type>::type;
+            using U16 = typename std::conditional<B == 2, uint16_t, uint8_t>::type;
+            using U = typename std::conditional<B == 4, uint32_t, U16>::type;
             const int cols = min(W, a.O - col);
 #pragma unroll 8
             for (int k = lane; k < 32 * W; k += 32) {
@@ -813,7 +814,6 @@ int check_args(const GroupedArgs& a, int type, int halves, const char* what)
     MB_REQUIRE(type != MB_T_E4M3 || (a.xs && a.ws), "%s: e4m3 operands need their scales", what);
     return MB_OK;
 }
-
 
 int make_maps(const GroupedArgs& a, int type, int halves, int wrows, int out, bool tiles, Maps* m, const char* what)
 {

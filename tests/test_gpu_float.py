@@ -829,3 +829,55 @@ def test_swiglu_past_32_bits(D, dtype):
             continue
         sw = s[r].double().repeat_interleave(G, 1)
         close(q[r].double() * sw, a, tol * 17 / 16 + 2.0 ** -4 * a.abs() * (1 + 2.0 ** -20) + 2.0 ** -10 * sw, str(r))
+
+
+FIRST_CALL = """
+import torch
+from distributedmoellm_b200 import device as D
+torch.manual_seed(0)
+x = torch.randn(40, 2048, device="cuda")
+w = torch.randn(4, 1536, 2048, device="cuda").to(torch.float8_e4m3fn)
+ws = torch.rand(4, 2, 6, 16, device="cuda")
+wd = torch.randn(4, 2048, 768, device="cuda").to(torch.float8_e4m3fn)
+wds = torch.rand(4, 16, 6, device="cuda")
+off = torch.tensor([0, 1, 9, 9, 40], dtype=torch.int32, device="cuda")
+one = torch.randn(1, 2048, device="cuda")
+torch.cuda.synchronize()
+
+def run():
+    q, s = D.operand_rows(x, torch.float8_e4m3fn)
+    a, t = D.grouped_swiglu_t(q, w, off, s, ws)
+    y = D.grouped_matmul_t(a, wd, off, t, wds)
+    q1, s1 = D.operand_rows(one, torch.float8_e4m3fn)
+    return y, D.matmul_t_e4m3(q1, s1, w[0], ws[0].reshape(12, 16))
+
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    captured = run()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(captured, run()))
+
+# several threads, each on a stream of its own
+import threading
+want, bad = run(), []
+def work():
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for _ in range(50):
+            got = run()
+        torch.cuda.current_stream().synchronize()
+        if not all(torch.equal(a, b) for a, b in zip(got, want)):
+            bad.append(1)
+torch.cuda.synchronize()
+ts = [threading.Thread(target=work) for _ in range(4)]
+[t.start() for t in ts]; [t.join() for t in ts]
+assert not bad
+print("fine")
+"""
+
+
+def test_first_calls_of_a_process_captured_and_from_threads(D):
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stderr[-2000:]
