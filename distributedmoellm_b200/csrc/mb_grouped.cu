@@ -35,7 +35,8 @@
 // groups and send their f32 partial sums through distributed shared memory to
 // the first of them, which adds them in rank order, so results do not depend on
 // timing.
-// Every wait is bounded (status word + abort flag).
+// Every wait of a role is bounded (status word + abort flag), so each reaches the
+// CTA's (and cluster's) barriers at the end, which have no limit of their own.
 //
 // Few rows an expert: bound by memory (512 picks of 128 e4m3 experts of 2048 x
 // 768: 33-34 us, operands and results at 5.9-6.1 TB/s).  Many: products and epilogue each take 160-180 us of
@@ -80,6 +81,7 @@ constexpr int kSets = 2;                  // of epilogue warps, each with half o
 constexpr int kBlock = 128;               // weight rows of a block
 constexpr int kTileW = kBlock * 128;      // bytes of a block's tile: 128 rows of 128 bytes
 constexpr int kMaxM = 128;                // rows of x per pass
+constexpr int kQuarters = 4;              // of the TMEM lanes, 32 rows each
 constexpr int kUnit = 4;                  // K steps whose scales are handed over together
 constexpr int kScSlots = 3;               // ring of such units
 constexpr int kScFloats = kUnit * (128 + 2);   // of each step: xs of the pass's rows, ws of the item's (up to) two blocks
@@ -170,7 +172,9 @@ struct ItemRing {
     template <bool WARP>
     __device__ __forceinline__ bool pop(Item& v)
     {
-        if (!mb_mbar_wait_spin(&full[r.slot], r.full_parity(), status, abort_flag)) return false;
+        bool got = mb_mbar_wait_spin(&full[r.slot], r.full_parity(), status, abort_flag);
+        if (WARP) got = __all_sync(0xffffffffu, got);      // lanes give up together
+        if (!got) return false;
         v = slots[r.slot];
         if (WARP) __syncwarp();
         if (!WARP || (threadIdx.x & 31) == 0) mb_mbar_arrive(&empty[r.slot]);
@@ -218,6 +222,7 @@ struct Epilogue {
     float4* red;               // partial sums: [sender][set][S / 4][MT rows]
     uint64_t *red_full, *red_empty;
     float* amax;               // [2][sets][128 rows]
+    uint32_t max_full;         // of each quarter: both sets' maxima are there (shared-memory address)
     uint8_t* tiles;            // the warp's tiles of results
     const CUtensorMap* ymaps;
     int split, srank;
@@ -320,7 +325,7 @@ struct Epilogue {
                     sum[c][i] = __fdividef(g, 1.0f + __expf(-g)) * sum[c + C / 2][i];
                 }
         }
-        const int n = ok ? min(32, w.nrows - 32 * q) : 0;  // rows of this quarter to write
+        const int n = __all_sync(0xffffffffu, ok) ? min(32, w.nrows - 32 * q) : 0;  // rows of this quarter to write
         const int64_t row = (int64_t)w.row0 + 32 * q;
         const int col = (DUAL ? w.nb * kBlock : w.nb * N) + R * set;
         if constexpr (OUT == MB_T_E4M3) {
@@ -445,10 +450,14 @@ struct Epilogue {
 #pragma unroll
             for (int i = 0; i < R; ++i) m = col + i < a.O ? fmaxf(m, fabsf(v[i / 16][i % 16])) : m;
         }
+        // The sets meet at an mbarrier, whose waits are bounded: after a wait that ran out one set may have left already.  A
+        // set is at most one item ahead of the other, so two buffers do.
         float* am = amax + abuf * kSets * kMaxM + 32 * q + lane;
-        abuf ^= 1;
         am[set * kMaxM] = m;
-        mb_named_barrier(1 + q, 32 * kSets);
+        __syncwarp();
+        if (lane == 0) bar_arrive(max_full + 8 * q);
+        if (!__all_sync(0xffffffffu, bar_wait(max_full + 8 * q, abuf, status, abort_flag))) n = 0;
+        abuf ^= 1;
 #pragma unroll
         for (int s = 0; s < kSets; ++s) m = fmaxf(m, am[s * kMaxM]);
         const Quotient qu(e4m3_scale(m));
@@ -513,7 +522,8 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
     uint64_t* item_empty = item_full + kItemSlots;
     uint64_t* red_full = item_empty + kItemSlots;
     uint64_t* red_empty = red_full + 1;
-    Item* items = reinterpret_cast<Item*>(red_empty + 1);
+    uint64_t* max_full = red_empty + 1;
+    Item* items = reinterpret_cast<Item*>(max_full + kQuarters);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kItemSlots);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [kWarps], [31]: split
@@ -541,6 +551,7 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
             mb_mbar_init(&item_full[i], 1);
             mb_mbar_init(&item_empty[i], kEpiWarps + (FP8 ? 3 : 2));
         }
+        for (int i = 0; i < kQuarters; ++i) mb_mbar_init(&max_full[i], kSets);
         *abort_flag = 0;
     }
     if (warp == Role::kLoad && lane < 1 + kRowMaps && (lane == 0 || 8 << lane <= a.MT))
@@ -750,7 +761,7 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
         const int q = warp & 3, set = SMALL ? warp >> 2 : (warp >> 2) - 1;
         Epi ep{a, status, abort_flag, tmem + ((uint32_t)(32 * q) << 16), mb_smem_addr(acc_full),
                mb_smem_addr(acc_empty), mb_smem_addr(sc_full), mb_smem_addr(sc_empty), sc, red,
-               red_full, red_empty, amax, tiles + (SMALL ? set : warp - 4) * Epi::kTiles * kTile, maps.y, split, srank,
+               red_full, red_empty, amax, mb_smem_addr(max_full), tiles + (SMALL ? set : warp - 4) * Epi::kTiles * kTile, maps.y, split, srank,
                cluster_rank() - srank, q, set, lane, Ring(kAcc), Ring(kScSlots), 0, 0, 0};
         while (ring.pop<true>(w)) ep.item(w, k0, k1);
         if (Epi::kTiles > 1) bulk_wait();
@@ -892,7 +903,7 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     const int stage = a.MT * 128 + N * 128;
     const int fixed = 1024 + (OUT == MB_T_E4M3 ? 2 * kSets * kMaxM * 4 : 0) + (FP8 ? kScSlots * kScFloats * 4 : 0) +
                       Role::kEpiWarps * Role::kTiles * kTile +
-                      (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2) * 8 + kItemSlots * 16 + 8 + 128 +
+                      (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2 + kQuarters) * 8 + kItemSlots * 16 + 8 + 128 +
                       a.E * 8 + (a.E + 1) * 4 + 16;
     // a split's partial sums may leave too few stages beside the tables of very many experts: then a smaller split
     while (cluster > 1 && (Role::kMaxSmem - fixed - (cluster - 1) * N * a.MT * 4) / stage < 2) cluster /= 2;
