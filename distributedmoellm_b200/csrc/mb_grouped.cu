@@ -92,6 +92,7 @@ constexpr int kRowMaps = 4;               // boxes of 16, 32, 64, 128 rows of x
 constexpr int kSmallRows = 32;            // rows of a small pass, at most
 constexpr int kRun = 64;                  // results leave in runs of 64 bytes a row ..
 constexpr int kTile = 32 * kRun;          // .. and tiles of 32 rows
+constexpr int kDrainTries = 100000;       // polls for work in flight at a role's end, at most
 
 __device__ unsigned g_no_status;          // where kernels report when the caller gives no status word
 
@@ -523,7 +524,8 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
     uint64_t* red_full = item_empty + kItemSlots;
     uint64_t* red_empty = red_full + 1;
     uint64_t* max_full = red_empty + 1;
-    Item* items = reinterpret_cast<Item*>(max_full + kQuarters);
+    uint64_t* mma_done = max_full + kQuarters;
+    Item* items = reinterpret_cast<Item*>(mma_done + 2);               // 16-byte aligned
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kItemSlots);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [kWarps], [31]: split
@@ -552,6 +554,7 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
             mb_mbar_init(&item_empty[i], kEpiWarps + (FP8 ? 3 : 2));
         }
         for (int i = 0; i < kQuarters; ++i) mb_mbar_init(&max_full[i], kSets);
+        mb_mbar_init(mma_done, 1);
         *abort_flag = 0;
     }
     if (warp == Role::kLoad && lane < 1 + kRowMaps && (lane == 0 || 8 << lane <= a.MT))
@@ -655,14 +658,14 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
                     ++issued;
                 }
             }
-            if (!ok || *abort_flag) {   // wait (bounded) for the copies still in flight before the CTA may end
-                for (int i = 0; i < min(issued, a.stages); ++i) {
-                    if (--st.slot < 0) {
-                        st.slot = a.stages - 1;
-                        st.phase ^= 1;
-                    }
-                    for (int n = 0; n < 100000 && !bar_try(fullb + 8 * st.slot, st.full_parity()); ++n) {
-                    }
+            // The last copies land (bounded) before the CTA may end, whoever gave up and whenever: without that they are what
+            // the products have waited for anyway.
+            for (int i = 0; i < min(issued, a.stages); ++i) {
+                if (--st.slot < 0) {
+                    st.slot = a.stages - 1;
+                    st.phase ^= 1;
+                }
+                for (int n = 0; n < kDrainTries && !bar_try(fullb + 8 * st.slot, st.full_parity()); ++n) {
                 }
             }
         }
@@ -697,6 +700,10 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
                         part = 0;
                     }
                 }
+            }
+            // so do the products, before TMEM and the barriers that they arrive on go
+            tc_commit(mma_done);
+            for (int n = 0; n < kDrainTries && !bar_try(mb_smem_addr(mma_done), 0); ++n) {
             }
         }
         __syncwarp();
@@ -903,7 +910,7 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
     const int stage = a.MT * 128 + N * 128;
     const int fixed = 1024 + (OUT == MB_T_E4M3 ? 2 * kSets * kMaxM * 4 : 0) + (FP8 ? kScSlots * kScFloats * 4 : 0) +
                       Role::kEpiWarps * Role::kTiles * kTile +
-                      (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2 + kQuarters) * 8 + kItemSlots * 16 + 8 + 128 +
+                      (2 * kMaxStages + 2 * kMaxAcc + 2 * kScSlots + 2 * kItemSlots + 2 + kQuarters + 2) * 8 + kItemSlots * 16 + 8 + 128 +
                       a.E * 8 + (a.E + 1) * 4 + 16;
     // a split's partial sums may leave too few stages beside the tables of very many experts: then a smaller split
     while (cluster > 1 && (Role::kMaxSmem - fixed - (cluster - 1) * N * a.MT * 4) / stage < 2) cluster /= 2;

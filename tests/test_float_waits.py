@@ -35,3 +35,15 @@ def test_lanes_of_a_warp_give_up_together():
     """A whole warp's wait for an item ends in one vote: lanes that leave a loop alone would miss the others' warp-wide steps."""
     pop = section(code(SOURCE.read_text()), "bool pop(Item& v)", "return v.nrows > 0;")
     assert re.search(r"if \(WARP\) got = __all_sync\(0xffffffffu, got\);\s+if \(!got\) return false;", pop)
+
+
+def test_work_in_flight_ends_before_the_cta():
+    """The loads and the products wait, with a limit, for what they issued last, whatever made them stop: a copy, or a
+    product's arrival, behind the CTA's end would reach the shared memory of the next one."""
+    text = code(SOURCE.read_text())
+    loads = section(text, "if (warp == Role::kLoad) {", "} else if (warp == Role::kMma) {")
+    mma = section(text, "} else if (warp == Role::kMma) {", "} else if (warp == Role::kFind) {")
+    for part, bar in ((loads, r"fullb \+ 8 \* st\.slot, st\.full_parity\(\)"), (mma, r"mb_smem_addr\(mma_done\), 0")):
+        loop = section(part, "while (ok && ring.pop<false>(w))", "__syncwarp();")
+        end = re.search(r"n < kDrainTries && !bar_try\(" + bar, loop)
+        assert end and "abort_flag)" not in loop[loop.rindex("++issued;" if part is loads else "part = 0;"):end.start()]
