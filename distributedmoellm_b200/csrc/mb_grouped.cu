@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
     {
         const int per = (a.E + kThreads - 1) / kThreads;
         const int e0 = min(a.E, (int)threadIdx.x * per), e1 = min(a.E, e0 + per);
-        int mine = 0;
+        int mine = 0, bad = 0;
         for (int e = e0; e < e1; ++e) {
             int lo = 0, n = (int)a.P;
             if (a.offsets) {
@@ -575,6 +575,7 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
                 n = hi - lo;
                 if (lo < 0 || hi < lo || hi > a.P) {
                     atomicOr(status, MB_STATUS_BADARG);
+                    bad = 1;
                     lo = n = 0;
                 }
             }
@@ -589,14 +590,31 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
             if (lane >= o) run += t;
         }
         if (lane == 31) wsum[warp] = run;
-        __syncthreads();
+        // Where no pair of offsets decreases, the ranges are disjoint.  Else what is left of them may overlap: a range that
+        // starts before the end of an earlier one is left out too, so that no row has two writers and the items stay within
+        // the count that the launch allowed for.
+        bad = __syncthreads_or(bad);
         int before = run - mine, total = 0;
         for (int w = 0; w < kWarps; ++w) {
             const int s = wsum[w];
             if (w < warp) before += s;
             total += s;
         }
-        for (int e = e0; e < e1; ++e) pstart[e] += before;
+        if (bad) {
+            if (threadIdx.x == 0) {
+                total = 0;
+                for (int e = 0, end = 0; e < a.E; ++e) {
+                    const int2 m = meta[e];
+                    const int n = m.x < end ? 0 : m.y;
+                    if (n < m.y) meta[e].y = 0;
+                    if (n > 0) end = m.x + n;
+                    pstart[e] = total;
+                    total += a.Nb * ((n + a.MT - 1) / a.MT);
+                }
+            }
+        } else {
+            for (int e = e0; e < e1; ++e) pstart[e] += before;
+        }
         if (threadIdx.x == 0) {
             pstart[a.E] = total;
             // How many CTAs share an item: the split whose longest CTA has the fewest K steps, two more for each

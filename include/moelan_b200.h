@@ -390,8 +390,9 @@ int mb_operand_rows(const void *x, int x_type, int64_t ldx, int64_t n_src, const
  * expert e (ragged; an expert may have no rows), f32 sums, rounded once to
  * y_type (MB_T_F32, MB_T_BF16 or MB_T_F16).  offsets (E + 1) int32 on the
  * device, non-decreasing within 0 .. P (else MB_STATUS_BADARG is set and the
- * offending experts' rows are left); rows of y before offsets[0] and from
- * offsets[E] on are left as they are.
+ * offending experts are left out: those whose range decreases or leaves 0 .. P,
+ * and those whose range starts before the end of an earlier one that counts);
+ * rows of y before offsets[0] and from offsets[E] on are left as they are.
  *   x (P, K) and w (E, O, K) of one type: MB_T_E4M3, MB_T_BF16 or MB_T_F16.
  *   ldx, ldw: elements between rows; w_expert: between experts' matrices.  x,
  *   w and these distances in bytes must be multiples of 16.  y rows are ldy
