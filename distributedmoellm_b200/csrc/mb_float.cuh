@@ -19,13 +19,14 @@ __device__ __forceinline__ float e4m3_scale(float m)
 }
 
 // x / s, correctly rounded, for many x and one s: r = 1 / s correctly rounded, then one correction of x * r by its
-// remainder (Markstein, IBM J. Res. Dev. 34, 1990).  Holds while nothing leaves the normal range, which `fast` says: with
-// |x| <= 449 s only remainders of quotients below 2^-20 can, and those round to e4m3's zero either way.
+// remainder x - q s (Markstein, IBM J. Res. Dev. 34, 1990), which has to be exact.  It is a multiple of ulp(q) ulp(s); for
+// quotients q from 2^-20 on, ulp(q) >= 2^-43, and s >= 2^-80 has ulp(s) >= 2^-103: at least 2^-146, which f32 holds, as a
+// subnormal if need be.  Smaller quotients round to e4m3's zero whatever their last bits.  Scales outside `fast` divide.
 struct Quotient {
     float s, r;
     bool fast;
     __device__ __forceinline__ explicit Quotient(float scale)
-        : s(scale), r(1.0f / scale), fast(scale > 0x1p-100f && scale < 0x1p100f)
+        : s(scale), r(1.0f / scale), fast(scale > 0x1p-80f && scale < 0x1p100f)
     {
     }
 };

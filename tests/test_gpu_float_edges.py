@@ -46,3 +46,43 @@ def test_overlapping_offsets_leave_later_ranges_out(D, dtype, offs):
     D.grouped_matmul_t(x, w, off, xs, ws, y=y, status=st)
     assert int(st) == 2
     close(y, want, sum_tol(K, S) + round_tol(want, F32), str(offs))
+
+
+# ---- quotients of very small scales ------------------------------------------------------
+
+# (largest value of a group, a value of it): next to a border of e4m3 with scales of 2^-97 and below, where the remainder
+# of an f32 division has bits below the smallest f32
+NEXT_TO_BORDERS = [("0x1.c0000ap-89", "0x1.800008p-106"), ("0x1.c00010p-90", "0x1.80000ep-107"),
+                   ("0x1.bfffd8p-90", "0x1.ffffd4p-109"), ("0x1.bfffeap-90", "0x1.ffffe8p-109"),
+                   ("0x1.500004p-89", "0x1.b00006p-105"), ("0x1.500002p-90", "0x1.e00004p-107"),
+                   ("0x1.500002p-89", "0x1.e00004p-106")]
+
+
+def test_operand_rows_quotients_of_small_scales_bit_exact(D):
+    x = torch.zeros((len(NEXT_TO_BORDERS), 256), dtype=torch.float64)
+    for i, (m, v) in enumerate(NEXT_TO_BORDERS):
+        x[i, 0], x[i, 1:128] = float.fromhex(m), float.fromhex(v)
+        x[i, 128], x[i, 129:] = -float.fromhex(m), -float.fromhex(v)
+    x = x.float().cuda()
+    q, s = D.operand_rows(x, E4M3)
+    wq, ws = plain_e4m3(x)
+    assert torch.equal(s, ws) and same_bits(q, wq)
+
+
+@pytest.mark.parametrize("low,high", [(-126, -76), (-80, -70), (-10, 10), (90, 110)])
+def test_operand_rows_next_to_every_border_bit_exact(D, low, high):
+    """Values whose quotients lie half an f32 step from a border between two e4m3 values, for scales of every size."""
+    g = gen(low + 1000)
+    n = 20000
+    m = torch.rand(n, generator=g, device="cuda") + 1
+    m = m * torch.exp2(torch.randint(low + 9, high + 9, (n,), generator=g, device="cuda").float())
+    s = (m / torch.full_like(m, 448.0)).double()
+    k = torch.arange(128, device="cuda")
+    borders = torch.where(k < 16, (k // 2 + 0.5) * 2.0 ** -9, (8 + (k // 2) % 8 + 0.5) / 8 * 2.0 ** (-6 + (k - 16) // 16))
+    step = torch.nextafter(borders.float(), torch.full_like(k, 1000.0, dtype=F32)).double() - borders.double()
+    mid = borders.double() + (k % 2 - 0.5) * step
+    x = (s[:, None] * mid).float()
+    x[:, 0] = m
+    q, sc = D.operand_rows(x, E4M3)
+    wq, ws = plain_e4m3(x)
+    assert torch.equal(sc, ws) and same_bits(q, wq)
