@@ -10,9 +10,11 @@
 constexpr int kScaleBlock = MB_SCALE_BLOCK;
 
 // The scale of a group whose largest magnitude is m: m / 448, and 1 where that is 0 (a group of zeros, or of values so
-// small that the quotient underflows), as mb_encode_rows does for int8.
+// small that the quotient underflows), as mb_encode_rows does for int8.  NaN counts as no value: m, a maximum by fmaxf, is
+// NaN only for a group of nothing else, which has scale 1 then.
 __device__ __forceinline__ float e4m3_scale(float m)
 {
+    m = fmaxf(m, 0.0f);
     const float r = 1.0f / 448.0f, q = m * r;              // see Quotient
     const float s = m > 0x1p-100f && m < 0x1p120f ? fmaf(fmaf(-q, 448.0f, m), r, q) : __fdiv_rn(m, 448.0f);
     return s == 0.0f ? 1.0f : s;

@@ -377,7 +377,8 @@ enum { MB_T_F32 = 0, MB_T_BF16 = 1, MB_T_F16 = 2, MB_T_E4M3 = 3 };
  *   type MB_T_E4M3: for each group g of 128 columns (the last may be shorter)
  *     scales[p, g] = max|x| / 448 (1 when that is 0), q = e4m3(x / scale) with
  *     both divisions and the final rounding to nearest even.  A NaN stays a
- *     NaN; a group that holds an infinity gets an infinite scale.
+ *     NaN and counts for nothing in its group's max (a group of nothing but
+ *     NaN has scale 1); a group that holds an infinity gets an infinite scale.
  * x_type: MB_T_F32, MB_T_BF16 or MB_T_F16.  Rows of x and q are ldx / ldq
  * elements apart; scales[p, g] is at scales[p * s_row + g * s_group].  An
  * index outside x sets MB_STATUS_BADARG (2) in *status (when not NULL) and its

@@ -86,3 +86,38 @@ def test_operand_rows_next_to_every_border_bit_exact(D, low, high):
     q, sc = D.operand_rows(x, E4M3)
     wq, ws = plain_e4m3(x)
     assert torch.equal(sc, ws) and same_bits(q, wq)
+
+
+# ---- groups of NaN ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T,k", [(6, 0), (0, 4)], ids=["each pick", "made once"])
+@pytest.mark.parametrize("d", [256, 200, 513])
+def test_operand_rows_groups_of_nothing_but_nan_have_scale_one(D, T, k, d):
+    """Whole groups of NaN (the last, shorter one too), groups with one value among NaN, and rows beside them; k: so many
+    rows and picks that each row is made once."""
+    if k:
+        T = 16 * torch.cuda.get_device_properties(0).multi_processor_count
+        d = ceil(d, 16) * 16
+    g = gen(d)
+    x = torch.randn((T, d), generator=g, device="cuda")
+    x[0] = float("nan")
+    x[2, :128] = float("nan")
+    x[3, 128:] = float("nan")
+    x[4, 1:] = float("nan")
+    x[4, 0] = -3.0
+    rows = torch.arange(T, device="cuda", dtype=torch.int32).repeat(max(k, 1))
+    q, s = D.operand_rows(x, E4M3, rows=rows)
+    wq, ws = plain_e4m3(x[rows.long()])
+    assert (ws[0] == 1).all() and ws[2, 0] == 1 and (ws[3, 1:] == 1).all()
+    assert torch.equal(s, ws) and same_bits(q, wq)
+
+
+def test_swiglu_nan_groups_have_the_same_scale_as_operand_rows(D):
+    """The activation of a NaN row, put into operand form, is what operand_rows makes of a row of NaN."""
+    g = gen(5)
+    x, xs, _ = rand_rows((20, 128), E4M3, g)
+    x[5] = float("nan")
+    w, ws, _ = rand_weights((1, 2, 200, 128), E4M3, g)
+    q, s = D.grouped_swiglu_t(x, w.reshape(1, 400, 128), offsets_of([20]), xs, ws)
+    q2, s2 = D.operand_rows(torch.full((1, 200), float("nan"), device="cuda"), E4M3)
+    assert same_bits(q[5:6], q2) and torch.equal(s[5:6], s2)
