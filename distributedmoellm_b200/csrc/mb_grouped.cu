@@ -198,6 +198,17 @@ __device__ __forceinline__ uint32_t round2(float lo, float hi)
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// g / (1 + exp(-g)), by the fast exponential and division (a few units of f32 each, |g| 2^-22 of the exponential's argument
+// on top: far below the rounding of any result type).  The fast division gives 0 for divisors from 2^126 on, that is below
+// -87.3, where the quotient is still a normal number; from -64 down 1 + exp(-g) is exp(-g) to the last bit, and g exp(g) the
+// same quotient.
+__device__ __forceinline__ float silu(float g)
+{
+    const bool low = g < -64.0f;
+    const float t = __expf(low ? g : -g);
+    return low ? g * t : __fdividef(g, 1.0f + t);
+}
+
 // WIDE: an item is two blocks of 128 weight rows, one per epilogue set (gate|up: the gate and the up rows of 128 columns,
 // of which each set takes 64); else one block, 64 columns per set.  OUT: the result type (gate|up: TYPE).
 template <int TYPE, bool DUAL, bool WIDE, bool SMALL, int OUT>
@@ -322,8 +333,7 @@ struct Epilogue {
             for (int c = 0; c < C / 2; ++c)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float g = sum[c][i];
-                    sum[c][i] = __fdividef(g, 1.0f + __expf(-g)) * sum[c + C / 2][i];
+                    sum[c][i] = silu(sum[c][i]) * sum[c + C / 2][i];
                 }
         }
         const int n = __all_sync(0xffffffffu, ok) ? min(32, w.nrows - 32 * q) : 0;  // rows of this quarter to write

@@ -409,7 +409,8 @@ int mb_grouped_matmul_t(const void *x, int type, int64_t ldx, const float *xs, i
 /* mb_grouped_matmul_t for gate|up matrices w (E, 2I, K), the I gate rows and
  * then the I up rows (moelan/experts.py:247-263 Expert), with the activation:
  *   a[p, j] = g / (1 + exp(-g)) * u,  g = x[p] @ w[e][j], u = x[p] @ w[e][I + j]
- * in f32, then put into operand form of x's type as mb_operand_rows does: q
+ * in f32, the exponential and the quotient by the device's fast functions (off
+ * by at most (|g| + 8) 2^-22 of a, and by |g u| 2^-149), then put into operand form of x's type as mb_operand_rows does: q
  * (P, I) of `type`, and for MB_T_E4M3 its scales qs[p, g] at
  * qs[p * qs_row + g * qs_group].  ws (E, 2, ceil(I/128), ceil(K/128)): the gate
  * rows' blocks and the up rows' blocks, each half with its own grid. */

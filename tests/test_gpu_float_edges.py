@@ -13,6 +13,10 @@ from test_gpu_float import D  # noqa: F401  (fixture)
 pytestmark = pytest.mark.gpu
 
 
+def padded_ones(n, d, dtype):
+    return torch.ones((n, d), device="cuda").to(dtype)
+
+
 # ---- offsets ----------------------------------------------------------------------------
 
 def ranges_that_count(offs, P):
@@ -121,3 +125,56 @@ def test_swiglu_nan_groups_have_the_same_scale_as_operand_rows(D):
     q, s = D.grouped_swiglu_t(x, w.reshape(1, 400, 128), offsets_of([20]), xs, ws)
     q2, s2 = D.operand_rows(torch.full((1, 200), float("nan"), device="cuda"), E4M3)
     assert same_bits(q[5:6], q2) and torch.equal(s[5:6], s2)
+
+
+# ---- gates far below zero -------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_swiglu_gates_far_below_zero(D, dtype, rows):
+    """Gates of -112 .. 112 with ups of 2^60 and 2^-60: below -87.3 the activation is tiny, but no zero once the up is
+    large.  Tolerance: as want_swiglu's, and exp(g) off by a step of the smallest f32 (2^-149), times |g u|; one product per
+    sum, which is exact."""
+    v = torch.arange(-448, 449, 1, device="cuda").float().to(E4M3).float().unique() / 4          # exact in both types
+    v = torch.cat([v, torch.linspace(-112, -80, 65, device="cuda")]) if dtype == BF16 else v
+    v = v.to(BF16).float()
+    I = v.numel()
+    x = padded_ones(rows, 128, dtype)
+    for up in (60, -60):
+        w = torch.zeros((1, 2, I, 128), device="cuda")
+        w[0, 0, :, 0] = v * (4 if dtype == E4M3 else 1)
+        w[0, 1, :, 0] = 1.0 if dtype == E4M3 else 2.0 ** up
+        xs = ws = None
+        if dtype == E4M3:
+            xs = torch.ones((rows, 1), device="cuda")
+            ws = torch.full((1, 2, ceil(I, G), 1), 0.25, device="cuda")
+            ws[0, 1] = 2.0 ** up
+        q, s = D.grouped_swiglu_t(x, w.to(dtype).view(1, 2 * I, 128), offsets_of([rows]), xs, ws)
+        g64, u = v.double(), 2.0 ** up
+        a = g64 / (1 + torch.exp(-g64)) * u
+        tol = (g64.abs() + 8) * 2.0 ** -22 * a.abs() + g64.abs() * u * 2.0 ** -149 + 2.0 ** -149
+        a, tol = a.expand(rows, I), tol.expand(rows, I)
+        if dtype != E4M3:
+            close(q, a, tol + round_tol(a, dtype), f"up 2^{up}")
+            continue
+        sw = s.double().repeat_interleave(G, 1)[:, :I]
+        close(q.double() * sw, a, tol * 17 / 16 + 2.0 ** -4 * a.abs() * (1 + 2.0 ** -20) + 2.0 ** -10 * sw, f"up 2^{up}")
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_swiglu_groups_of_tiny_activations(D, rows):
+    """A whole group of gates near -88 with ups of 1: its scale follows the activations, which are normal numbers."""
+    gate = torch.tensor([-87.0, -87.5, -88.0, -88.5], device="cuda").repeat(32)
+    x = padded_ones(rows, 128, E4M3)
+    w = torch.zeros((1, 2, 128, 128), device="cuda")
+    w[0, 0, :, 0], w[0, 0, :, 1], w[0, 1, :, 0] = -352.0, (gate * 4 + 352.0), 1.0     # -352 + (4, 2, 0, -2)
+    ws = torch.ones((1, 2, 1, 1), device="cuda")
+    ws[0, 0] = 0.25
+    q, s = D.grouped_swiglu_t(x, w.to(E4M3).view(1, 256, 128), offsets_of([rows]), torch.ones((rows, 1), device="cuda"), ws)
+    g64 = gate.double()
+    a = (g64 / (1 + torch.exp(-g64))).expand(rows, 128)
+    tol = (g64.abs() + 8) * 2.0 ** -22 * a.abs() + g64.abs() * 2.0 ** -149
+    m = a.abs().amax(1, keepdim=True) / 448
+    close(s, m, tol.amax(1, keepdim=True) / 448 + 2.0 ** -23 * m + 2.0 ** -149, "scales")
+    close(q.double() * s.double(), a, tol * 17 / 16 + 2.0 ** -4 * a.abs() * (1 + 2.0 ** -20) + 2.0 ** -10 * s.double()
+          + 448 * 2.0 ** -149, "values")
