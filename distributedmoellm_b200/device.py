@@ -419,6 +419,14 @@ def _new_scales(like: torch.Tensor, n: int, groups: int):
     return torch.empty_strided((n, groups), (1, n), dtype=torch.float32, device=like.device)
 
 
+def _new_operand(like: torch.Tensor, n: int, d: int, dtype):
+    """Operand rows (n, d) that the products take: a multiple of 16 bytes apart."""
+    step = 16 // dtype.itemsize
+    if d % step == 0:
+        return like.new_empty((n, d), dtype=dtype)
+    return like.new_empty((n, -(-d // step) * step), dtype=dtype)[:, :d]
+
+
 def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None = None, q: torch.Tensor | None = None,
                  scales: torch.Tensor | None = None, status: torch.Tensor | None = None):
     """Rows of x (T, d) f32 / bf16 / f16 in the form the grouped products take:
@@ -426,7 +434,8 @@ def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None 
     rounded to ``dtype``.  torch.float8_e4m3fn: each group of 128 columns over
     its scale max|x| / 448.  Returns (q (n, d), scales (n, ceil(d / 128)) f32
     or None); rows of q and the scales may have any strides, columns of x and q
-    must be adjacent.  An index outside x sets bit 2 of ``status`` and gives a row
+    must be adjacent.  A new q has rows a multiple of 16 bytes apart, as the
+    products take them.  An index outside x sets bit 2 of ``status`` and gives a row
     of zeros."""
     if x.dim() != 2 or x.dtype not in RESULT_TYPES:
         raise ValueError(f"operand_rows takes (rows, columns) of f32, bf16 or f16, got {tuple(x.shape)} {x.dtype}")
@@ -446,7 +455,7 @@ def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None 
     st = _status_ptr(status)
     dev = _on(x, rows, q, scales, status)
     if q is None:
-        q = x.new_empty((n, d), dtype=dtype)
+        q = _new_operand(x, n, d, dtype)
     s, sr, sg = None, 0, 0
     if dtype is _E4M3:
         scales = _new_scales(x, n, _blocks(d)) if scales is None else scales
@@ -549,8 +558,8 @@ def grouped_swiglu_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs
     """The grouped product with gate|up matrices w (E, 2I, K) (I gate rows, then
     I up rows; ws (E, 2, ceil(I/128), ceil(K/128)) for e4m3), SiLU(gate) * up
     in f32, and its rows in operand form of x's type: returns (q (P, I), scales
-    (P, ceil(I/128)) or None), what the down product takes.  Otherwise as
-    grouped_matmul_t."""
+    (P, ceil(I/128)) or None), what the down product takes (a new q has rows a
+    multiple of 16 bytes apart).  Otherwise as grouped_matmul_t."""
     _groups(w, offsets)
     E, I2, K = w.shape
     if I2 % 2:
@@ -567,7 +576,7 @@ def grouped_swiglu_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs
     ldx, ldw = _operand_stride(x, "x"), _operand_stride(w, "w")
     dev = _on(x, w, offsets, xs, ws, q, scales, status)
     if q is None:
-        q = x.new_empty((P, I))
+        q = _new_operand(x, P, I, x.dtype)
     s, sr, sg = None, 0, 0
     if x.dtype is _E4M3:
         scales = _new_scales(x, P, _blocks(I)) if scales is None else scales

@@ -178,3 +178,35 @@ def test_swiglu_groups_of_tiny_activations(D, rows):
     close(s, m, tol.amax(1, keepdim=True) / 448 + 2.0 ** -23 * m + 2.0 ** -149, "scales")
     close(q.double() * s.double(), a, tol * 17 / 16 + 2.0 ** -4 * a.abs() * (1 + 2.0 ** -20) + 2.0 ** -10 * s.double()
           + 448 * 2.0 ** -149, "values")
+
+
+# ---- rows taken from one operator by the next ---------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16, F16])
+@pytest.mark.parametrize("H,I", [(1000, 715), (24, 1), (129, 4), (272, 208)])
+def test_operators_take_each_others_rows_at_any_width(D, dtype, H, I):
+    """Operand rows, gate|up and down with the results that the operators make themselves, widths that are no multiple of
+    16 bytes among them."""
+    g = gen(H + I)
+    off = offsets_of([3, 0, 40])
+    x = torch.randn((43, H), generator=g, device="cuda")
+    q, s = D.operand_rows(x, dtype)
+    w, ws, ww = rand_weights((3, 2, I, H), dtype, g, scale=2.0 / H ** 0.5)
+    wv = torch.as_strided(w, (3, 2 * I, H), (2 * I * w.stride(2), w.stride(2), 1), w.storage_offset())
+    a, as_ = D.grouped_swiglu_t(q, wv, off, s, ws)
+    d, ds, dw = rand_weights((3, H, I), dtype, g)
+    y = D.grouped_matmul_t(a, d, off, as_, ds)
+
+    def wide(v, sc):
+        return v.double() if sc is None else v.double() * sc.double().repeat_interleave(G, 1)[:, :v.shape[1]]
+    want, S, _ = want_grouped(wide(a, as_), dw, off)
+    close(y, want, sum_tol(I, S) + round_tol(want, F32))
+    act, tol, _ = want_swiglu(wide(q, s), ww.reshape(3, 2 * I, H), off, I, H)
+    if dtype != E4M3:
+        close(a, act, tol + round_tol(act, dtype))
+    else:
+        sw = as_.double().repeat_interleave(G, 1)[:, :I]
+        close(a.double() * sw, act, tol * 17 / 16 + 2.0 ** -4 * act.abs() * (1 + 2.0 ** -20) + 2.0 ** -10 * sw)
+        m, ms, mw = rand_weights((I, H), E4M3, g)
+        want, S = wide(q, s) @ mw.t(), wide(q, s).abs() @ mw.abs().t()
+        close(D.matmul_t_e4m3(q, s, m, ms), want, sum_tol(H, S) + round_tol(want, F32))
