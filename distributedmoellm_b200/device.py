@@ -338,9 +338,9 @@ RESULT_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 # Small calls cost what their checks cost on the host: shapes are compared whole, the device is an index, the stream comes
-# as a raw handle, and the messages are put together only when something is wrong.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# as a raw handle, and the messages are put together only when something is wrong.  torch's two functions for that are
+# looked up at the first call: a torch without CUDA does not have them.
+_raw_stream = _current_device = None
 _fns: dict = {}
 _E4M3 = torch.float8_e4m3fn
 
@@ -402,8 +402,10 @@ def _on(t, *others):
 
 def _call(name, dev, *args):
     """The library's ``name`` on device ``dev``'s current stream, which is the last argument."""
+    global _raw_stream, _current_device
     fn = _fns.get(name)
     if fn is None:
+        _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
         fn = _fns[name] = getattr(lib(), name)
     if _current_device() == dev:
         rc = fn(*args, _raw_stream(dev))
