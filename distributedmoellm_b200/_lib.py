@@ -64,6 +64,12 @@ SIGNATURES = {
                                    _vp, _vp, _int, _i64, _vp, _vp]),
     "mb_grouped_swiglu_t": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _int, _int, _int,
                                    _vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp]),
+    "mb_operand_rows_slice": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _int, _int, _vp, _i64, _vp, _i64, _i64, _vp, _vp,
+                                     _vp, _vp]),
+    "mb_grouped_matmul_t_slice": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _int, _int, _int,
+                                         _vp, _vp, _int, _i64, _i64, _vp, _vp]),
+    "mb_grouped_swiglu_t_slice": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _int, _int, _int,
+                                         _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp]),
     "mb_matmul_t_e4m3": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _int, _int, _vp, _int, _i64, _vp,
                                 _vp]),
 }

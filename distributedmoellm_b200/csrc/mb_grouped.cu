@@ -112,6 +112,7 @@ struct GroupedArgs {
     float* qs;
     int64_t qs_row, qs_group;
     unsigned* status;
+    int64_t likely;            // rows within the offsets, as far as the host knows: what sizes and splits go by
     int Kb;                    // K steps (128 bytes of a row each)
     int Nb;                    // column blocks of an item's width
     int MT;                    // rows of x per pass, at most
@@ -846,6 +847,7 @@ int check_args(const GroupedArgs& a, int type, int halves, const char* what)
     MB_REQUIRE(a.E >= 1 && a.E <= 1024 && a.O >= 1 && a.O <= (1 << 24) && a.K >= 1 && a.K <= (1 << 24) && a.P >= 0 &&
                    a.P < (1ll << 31),
                "%s: E=%d O=%d K=%d P=%lld", what, a.E, a.O, a.K, (long long)a.P);
+    MB_REQUIRE(a.likely >= 0 && a.likely <= a.P, "%s: %lld picks of %lld rows", what, (long long)a.likely, (long long)a.P);
     const int64_t b = elem_bytes(type);
     MB_REQUIRE(a.ldx >= a.K && a.ldw >= a.K && a.ldy >= a.O, "%s: rows closer than their width (%lld, %lld, %lld)",
                what, (long long)a.ldx, (long long)a.ldw, (long long)a.ldy);
@@ -919,10 +921,10 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
         // The split with the fewest K steps in turn on the busiest CTA, the launch of clusters counted as steps too (it
         // measured 1, 3 and 6 us for 2, 4 and 8 CTAs of small passes, a step 0.35 us; passes of 64 rows have more sums to
         // send, and with 128 rows the split lost: 17.8 us against 16.0 at 128 x 4096 x 4096).  Clusters get one CTA per
-        // SM, which is what the occupancy query grants them.  Experts with rows: those that P picks of E meet, each as
+        // SM, which is what the occupancy query grants them.  Experts with rows: those that the picks meet, each expert as
         // likely as another.
-        const double meet = a.offsets ? a.E * (1.0 - std::pow(1.0 - 1.0 / a.E, (double)a.P)) : 1.0;
-        const double passes = std::max(meet, (double)((a.P + a.MT - 1) / a.MT));
+        const double meet = a.offsets ? a.E * (1.0 - std::pow(1.0 - 1.0 / a.E, (double)a.likely)) : 1.0;
+        const double passes = std::max(meet, (double)((a.likely + a.MT - 1) / a.MT));
         const int64_t likely = std::max<int64_t>(1, (int64_t)(a.Nb * passes + 0.5));
         int64_t best = (int64_t)1 << 62;
         for (int c = 1, extra = 0; c <= 8 && c <= a.Kb && (c - 1) * N * a.MT * 4 <= Role::kMaxRed; c *= 2) {
@@ -998,7 +1000,7 @@ int launch(GroupedArgs a, const char* what, cudaStream_t st)
 // 15.7 / 14.9).
 int pass_rows(const GroupedArgs& a)
 {
-    return pow2_at_least(a.offsets ? (a.P * 3 / 2 + a.E - 1) / a.E : a.P, 16, kMaxM);
+    return pow2_at_least(a.offsets ? (a.likely * 3 / 2 + a.E - 1) / a.E : a.P, 16, kMaxM);
 }
 
 // Blocks of 256 weight rows where that still gives every SM an item, else of 128: the wider items move fewer bytes of x
@@ -1006,8 +1008,8 @@ int pass_rows(const GroupedArgs& a)
 // calls over more SMs.
 bool wide(const GroupedArgs& a)
 {
-    const int64_t active = std::min<int64_t>(a.E, a.P);
-    return (a.O + 255) / 256 * (active + a.P / a.MT) >= mb_num_sms();
+    const int64_t active = std::min<int64_t>(a.E, a.likely);
+    return (a.O + 255) / 256 * (active + a.likely / a.MT) >= mb_num_sms();
 }
 
 template <int TYPE, int OUT>
@@ -1048,15 +1050,24 @@ int matmul(const GroupedArgs& a, int type, int y_type, const char* what, void* s
 
 }  // namespace
 
+extern "C" int mb_grouped_matmul_t_slice(const void* x, int type, int64_t ldx, const float* xs, int64_t xs_row,
+                                         int64_t xs_group, int64_t P, const void* w, int64_t w_expert, int64_t ldw,
+                                         const float* ws, int E, int O, int K, const int32_t* offsets, void* y,
+                                         int y_type, int64_t ldy, int64_t picks, unsigned* status, void* stream)
+{
+    MB_REQUIRE(offsets || P == 0, "mb_grouped_matmul_t: null pointer");
+    const GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, O, K,
+                        offsets, y, ldy, nullptr, 0, 0, status, picks};
+    return matmul(a, type, y_type, "mb_grouped_matmul_t", stream);
+}
+
 extern "C" int mb_grouped_matmul_t(const void* x, int type, int64_t ldx, const float* xs, int64_t xs_row,
                                    int64_t xs_group, int64_t P, const void* w, int64_t w_expert, int64_t ldw,
                                    const float* ws, int E, int O, int K, const int32_t* offsets, void* y, int y_type,
                                    int64_t ldy, unsigned* status, void* stream)
 {
-    MB_REQUIRE(offsets || P == 0, "mb_grouped_matmul_t: null pointer");
-    const GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, O, K,
-                        offsets, y, ldy, nullptr, 0, 0, status};
-    return matmul(a, type, y_type, "mb_grouped_matmul_t", stream);
+    return mb_grouped_matmul_t_slice(x, type, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, O, K, offsets, y,
+                                     y_type, ldy, P, status, stream);
 }
 
 extern "C" int mb_matmul_t_e4m3(const void* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_group,
@@ -1064,19 +1075,20 @@ extern "C" int mb_matmul_t_e4m3(const void* x, int64_t ldx, const float* xs, int
                                 int y_type, int64_t ldy, unsigned* status, void* stream)
 {
     const GroupedArgs a{x, ldx, xs, xs_row, xs_group, n, w, 0, ldw, ws, 1, O, K,
-                        nullptr, y, ldy, nullptr, 0, 0, status};
+                        nullptr, y, ldy, nullptr, 0, 0, status, n};
     return matmul(a, MB_T_E4M3, y_type, "mb_matmul_t_e4m3", stream);
 }
 
-extern "C" int mb_grouped_swiglu_t(const void* x, int type, int64_t ldx, const float* xs, int64_t xs_row,
-                                   int64_t xs_group, int64_t P, const void* w, int64_t w_expert, int64_t ldw,
-                                   const float* ws, int E, int I, int K, const int32_t* offsets, void* q, int64_t ldq,
-                                   float* qs, int64_t qs_row, int64_t qs_group, unsigned* status, void* stream)
+extern "C" int mb_grouped_swiglu_t_slice(const void* x, int type, int64_t ldx, const float* xs, int64_t xs_row,
+                                         int64_t xs_group, int64_t P, const void* w, int64_t w_expert, int64_t ldw,
+                                         const float* ws, int E, int I, int K, const int32_t* offsets, void* q,
+                                         int64_t ldq, float* qs, int64_t qs_row, int64_t qs_group, int64_t picks,
+                                         unsigned* status, void* stream)
 {
     const char* what = "mb_grouped_swiglu_t";
     MB_REQUIRE(offsets || P == 0, "%s: null pointer", what);
     const GroupedArgs a{x, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K,
-                        offsets, q, ldq, qs, qs_row, qs_group, status};
+                        offsets, q, ldq, qs, qs_row, qs_group, status, picks};
     int rc = check_args(a, type, 2, what);
     if (rc || P == 0) return rc;
     MB_REQUIRE(type != MB_T_E4M3 || qs, "%s: e4m3 results need their scales", what);
@@ -1084,4 +1096,13 @@ extern "C" int mb_grouped_swiglu_t(const void* x, int type, int64_t ldx, const f
     if (type == MB_T_E4M3) return launch_swiglu<MB_T_E4M3>(a, what, st);
     if (type == MB_T_BF16) return launch_swiglu<MB_T_BF16>(a, what, st);
     return launch_swiglu<MB_T_F16>(a, what, st);
+}
+
+extern "C" int mb_grouped_swiglu_t(const void* x, int type, int64_t ldx, const float* xs, int64_t xs_row,
+                                   int64_t xs_group, int64_t P, const void* w, int64_t w_expert, int64_t ldw,
+                                   const float* ws, int E, int I, int K, const int32_t* offsets, void* q, int64_t ldq,
+                                   float* qs, int64_t qs_row, int64_t qs_group, unsigned* status, void* stream)
+{
+    return mb_grouped_swiglu_t_slice(x, type, ldx, xs, xs_row, xs_group, P, w, w_expert, ldw, ws, E, I, K, offsets, q,
+                                     ldq, qs, qs_row, qs_group, P, status, stream);
 }

@@ -104,18 +104,36 @@ __device__ __forceinline__ uint2 round4(const float (&v)[4])
     return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
+struct RowsArgs {
+    const void* x;
+    int64_t ldx, n_src;
+    const int32_t* rows;
+    int64_t n;
+    int d;
+    void* q;
+    int64_t ldq;
+    float* scales;
+    int64_t s_row, s_group;
+    const int32_t *first, *last;           // null: every row
+    unsigned* status;
+};
+
 // VEC: four columns at a time are aligned in x and q, and d is a multiple of 4.
 template <typename SRC, int TYPE, bool VEC>
-__global__ void operand_rows_kernel(const SRC* __restrict__ x, int64_t ldx, int64_t n_src,
-                                    const int32_t* __restrict__ rows, int64_t n, int d, void* __restrict__ q,
-                                    int64_t ldq, float* __restrict__ scales, int64_t s_row, int64_t s_group,
-                                    unsigned* status)
+__global__ void operand_rows_kernel(const __grid_constant__ RowsArgs a)
 {
+    const SRC* __restrict__ x = reinterpret_cast<const SRC*>(a.x);
+    const int32_t* __restrict__ rows = a.rows;
+    void* __restrict__ q = a.q;
+    float* __restrict__ scales = a.scales;
+    unsigned* const status = a.status;
+    const int64_t ldx = a.ldx, n_src = a.n_src, n = a.n, ldq = a.ldq, s_row = a.s_row, s_group = a.s_group;
+    const int d = a.d;
     mb_pdl_trigger();
     mb_pdl_wait();
     const int lane = threadIdx.x & 31;
     const int64_t p = (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x >> 5);
-    if (p >= n) return;
+    if (p >= n || (a.first && (p < *a.first || p >= *a.last))) return;
     const int64_t src = rows ? rows[p] : p;
     const bool ok = src >= 0 && src < n_src;
     if (!ok && blockIdx.y == 0 && lane == 0 && status) atomicOr(status, MB_STATUS_BADARG);
@@ -247,17 +265,19 @@ __global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const SRC* 
 
 template <typename SRC, int TYPE>
 int launch(const SRC* x, int64_t ldx, int64_t n_src, const int32_t* rows, int64_t n, int d, void* q, int64_t ldq,
-           float* scales, int64_t s_row, int64_t s_group, unsigned* status, cudaStream_t st)
+           float* scales, int64_t s_row, int64_t s_group, const int32_t* first, const int32_t* last, unsigned* status,
+           cudaStream_t st)
 {
     constexpr int B = TYPE == MB_T_E4M3 ? 1 : 2;
     const bool vec = d % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 && (uintptr_t)x % (4 * sizeof(SRC)) == 0 &&
                      (uintptr_t)q % (4 * B) == 0;
     // Worth it from four picks a row on, with a block of rows for every SM (16384 from 2048 rows: 23.7 us, made for each
     // pick 22.5; 9600 from 1200: 19.1 and 13.2), and few enough rows that looking through the picks (4 n bytes for each
-    // 16 rows) stays below reading x for each pick.
+    // 16 rows) stays below reading x for each pick.  A slice of the experts is made for each pick: it has 1 / ranks of them
+    // (the bounds of its rows in the kernel cost every call 1.1 of 29.4 us at 32768 from 4096).
     const int ng = (d + kScaleBlock - 1) / kScaleBlock;
     const int64_t smem = (int64_t)kSpreadRows * (d * B + ng * 4);
-    if (rows && vec && n >= 4 * n_src && n_src >= kSpreadRows * mb_num_sms() && n_src <= 8 * (int64_t)d &&
+    if (rows && !first && vec && n >= 4 * n_src && n_src >= kSpreadRows * mb_num_sms() && n_src <= 8 * (int64_t)d &&
         smem <= kSpreadSmem && d * B % 16 == 0 && ldq * B % 16 == 0 && (uintptr_t)q % 16 == 0) {
         static thread_local uint64_t ready = 0;            // devices whose attribute is set
         int dev = 0;
@@ -277,46 +297,57 @@ int launch(const SRC* x, int64_t ldx, int64_t n_src, const int32_t* rows, int64_
     }
     const int cols = kGroups * kScaleBlock;
     const dim3 grid((unsigned)((n + kRowsPerBlock - 1) / kRowsPerBlock), (unsigned)((d + cols - 1) / cols));
-    const cudaError_t e =
-        vec ? mb_launch_pdl(operand_rows_kernel<SRC, TYPE, true>, grid, dim3(32 * kRowsPerBlock), 0, st, x, ldx, n_src,
-                            rows, n, d, q, ldq, scales, s_row, s_group, status)
-            : mb_launch_pdl(operand_rows_kernel<SRC, TYPE, false>, grid, dim3(32 * kRowsPerBlock), 0, st, x, ldx, n_src,
-                            rows, n, d, q, ldq, scales, s_row, s_group, status);
+    const RowsArgs a{x, ldx, n_src, rows, n, d, q, ldq, scales, s_row, s_group, first, last, status};
+    const cudaError_t e = mb_launch_pdl(vec ? operand_rows_kernel<SRC, TYPE, true> : operand_rows_kernel<SRC, TYPE, false>,
+                                        grid, dim3(32 * kRowsPerBlock), 0, st, a);
     if (e != cudaSuccess) return mb_fail(MB_ECUDA, "mb_operand_rows: %s", cudaGetErrorString(e));
     return MB_OK;
 }
 
 template <typename SRC>
 int launch_as(const SRC* x, int64_t ldx, int64_t n_src, const int32_t* rows, int64_t n, int d, int type, void* q,
-              int64_t ldq, float* scales, int64_t s_row, int64_t s_group, unsigned* status, cudaStream_t st)
+              int64_t ldq, float* scales, int64_t s_row, int64_t s_group, const int32_t* first, const int32_t* last,
+              unsigned* status, cudaStream_t st)
 {
     if (type == MB_T_E4M3)
-        return launch<SRC, MB_T_E4M3>(x, ldx, n_src, rows, n, d, q, ldq, scales, s_row, s_group, status, st);
+        return launch<SRC, MB_T_E4M3>(x, ldx, n_src, rows, n, d, q, ldq, scales, s_row, s_group, first, last, status, st);
     if (type == MB_T_BF16)
-        return launch<SRC, MB_T_BF16>(x, ldx, n_src, rows, n, d, q, ldq, scales, s_row, s_group, status, st);
-    return launch<SRC, MB_T_F16>(x, ldx, n_src, rows, n, d, q, ldq, scales, s_row, s_group, status, st);
+        return launch<SRC, MB_T_BF16>(x, ldx, n_src, rows, n, d, q, ldq, scales, s_row, s_group, first, last, status, st);
+    return launch<SRC, MB_T_F16>(x, ldx, n_src, rows, n, d, q, ldq, scales, s_row, s_group, first, last, status, st);
 }
 
 }  // namespace
 
-extern "C" int mb_operand_rows(const void* x, int x_type, int64_t ldx, int64_t n_src, const int32_t* rows, int64_t n,
-                               int d, int type, void* q, int64_t ldq, float* scales, int64_t s_row, int64_t s_group,
-                               unsigned* status, void* stream)
+extern "C" int mb_operand_rows_slice(const void* x, int x_type, int64_t ldx, int64_t n_src, const int32_t* rows,
+                                     int64_t n, int d, int type, void* q, int64_t ldq, float* scales, int64_t s_row,
+                                     int64_t s_group, const int32_t* first, const int32_t* last, unsigned* status,
+                                     void* stream)
 {
     MB_REQUIRE(x_type == MB_T_F32 || x_type == MB_T_BF16 || x_type == MB_T_F16, "mb_operand_rows: x type %d", x_type);
     MB_REQUIRE(type == MB_T_E4M3 || type == MB_T_BF16 || type == MB_T_F16, "mb_operand_rows: operand type %d", type);
     MB_REQUIRE(n >= 0 && n < (1ll << 31) && n_src >= 0 && d > 0 && d <= (1 << 24), "mb_operand_rows: n=%lld n_src=%lld d=%d",
                (long long)n, (long long)n_src, d);
     MB_REQUIRE(rows || n <= n_src, "mb_operand_rows: %lld rows of %lld", (long long)n, (long long)n_src);
+    MB_REQUIRE(!first == !last, "mb_operand_rows: first without last");
     MB_REQUIRE(ldx >= d && ldq >= d, "mb_operand_rows: rows closer (%lld, %lld) than their width %d", (long long)ldx,
                (long long)ldq, d);
     if (n == 0) return MB_OK;
     MB_REQUIRE(q && (x || n_src == 0) && (type != MB_T_E4M3 || scales), "mb_operand_rows: null pointer");
     const cudaStream_t st = mb_stream(stream);
     if (x_type == MB_T_F32)
-        return launch_as((const float*)x, ldx, n_src, rows, n, d, type, q, ldq, scales, s_row, s_group, status, st);
+        return launch_as((const float*)x, ldx, n_src, rows, n, d, type, q, ldq, scales, s_row, s_group, first, last, status,
+                         st);
     if (x_type == MB_T_BF16)
-        return launch_as((const __nv_bfloat16*)x, ldx, n_src, rows, n, d, type, q, ldq, scales, s_row, s_group, status,
-                      st);
-    return launch_as((const __half*)x, ldx, n_src, rows, n, d, type, q, ldq, scales, s_row, s_group, status, st);
+        return launch_as((const __nv_bfloat16*)x, ldx, n_src, rows, n, d, type, q, ldq, scales, s_row, s_group, first, last,
+                         status, st);
+    return launch_as((const __half*)x, ldx, n_src, rows, n, d, type, q, ldq, scales, s_row, s_group, first, last, status,
+                     st);
+}
+
+extern "C" int mb_operand_rows(const void* x, int x_type, int64_t ldx, int64_t n_src, const int32_t* rows, int64_t n,
+                               int d, int type, void* q, int64_t ldq, float* scales, int64_t s_row, int64_t s_group,
+                               unsigned* status, void* stream)
+{
+    return mb_operand_rows_slice(x, x_type, ldx, n_src, rows, n, d, type, q, ldq, scales, s_row, s_group, nullptr, nullptr,
+                                 status, stream);
 }

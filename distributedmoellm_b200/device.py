@@ -421,6 +421,13 @@ def _new_scales(like: torch.Tensor, n: int, groups: int):
     return torch.empty_strided((n, groups), (1, n), dtype=torch.float32, device=like.device)
 
 
+def _picks(picks, P):
+    """How many of P rows a slice's offsets span, as far as the caller knows."""
+    if not 0 <= picks <= P:
+        raise ValueError(f"{picks} picks of {P} rows")
+    return picks
+
+
 def _new_operand(like: torch.Tensor, n: int, d: int, dtype):
     """Operand rows (n, d) that the products take: a multiple of 16 bytes apart."""
     step = 16 // dtype.itemsize
@@ -430,7 +437,8 @@ def _new_operand(like: torch.Tensor, n: int, d: int, dtype):
 
 
 def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None = None, q: torch.Tensor | None = None,
-                 scales: torch.Tensor | None = None, status: torch.Tensor | None = None):
+                 scales: torch.Tensor | None = None, status: torch.Tensor | None = None,
+                 offsets: torch.Tensor | None = None):
     """Rows of x (T, d) f32 / bf16 / f16 in the form the grouped products take:
     x[rows] (all of x when rows is None; rows int32, as Routing.sorted_rows)
     rounded to ``dtype``.  torch.float8_e4m3fn: each group of 128 columns over
@@ -438,11 +446,16 @@ def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None 
     or None); rows of q and the scales may have any strides, columns of x and q
     must be adjacent.  A new q has rows a multiple of 16 bytes apart, as the
     products take them.  An index outside x sets bit 2 of ``status`` and gives a row
-    of zeros."""
+    of zeros.  ``offsets`` (those of a slice of the experts, int32 on the
+    device): only the rows offsets[0] <= p < offsets[-1] are made."""
     if x.dim() != 2 or x.dtype not in RESULT_TYPES:
         raise ValueError(f"operand_rows takes (rows, columns) of f32, bf16 or f16, got {tuple(x.shape)} {x.dtype}")
     if dtype not in OPERAND_TYPES:
         raise ValueError(f"operand type {dtype}, expected one of {', '.join(str(d) for d in OPERAND_TYPES)}")
+    if offsets is not None:
+        if offsets.dim() != 1 or offsets.dtype is not torch.int32 or not offsets.is_contiguous() or not offsets.shape[0]:
+            raise ValueError("offsets must be a contiguous vector of int32")
+        _on(x, offsets)
     if rows is not None and (rows.dim() != 1 or rows.dtype is not torch.int32 or not rows.is_contiguous()):
         raise ValueError("rows must be a contiguous vector of int32")
     T, d = x.shape
@@ -456,14 +469,25 @@ def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None 
     ldx = _rows_of(x, "x")
     st = _status_ptr(status)
     dev = _on(x, rows, q, scales, status)
-    if q is None:
+    if q is not None:
+        ldq = _rows_of(q, "q")
+    elif d & 15:
         q = _new_operand(x, n, d, dtype)
+        ldq = q.stride(0)
+    else:
+        q, ldq = x.new_empty((n, d), dtype=dtype), d
     s, sr, sg = None, 0, 0
     if dtype is _E4M3:
         scales = _new_scales(x, n, _blocks(d)) if scales is None else scales
         s, (sr, sg) = scales.data_ptr(), scales.stride()
-    _call("mb_operand_rows", dev, x.data_ptr(), _TYPES[x.dtype], ldx, T, None if rows is None else rows.data_ptr(), n, d,
-          _TYPES[dtype], q.data_ptr(), _rows_of(q, "q"), s, sr, sg, st)
+    rp = None if rows is None else rows.data_ptr()
+    if offsets is None:
+        _call("mb_operand_rows", dev, x.data_ptr(), _TYPES[x.dtype], ldx, T, rp, n, d, _TYPES[dtype], q.data_ptr(), ldq, s,
+              sr, sg, st)
+    else:
+        first = offsets.data_ptr()
+        _call("mb_operand_rows_slice", dev, x.data_ptr(), _TYPES[x.dtype], ldx, T, rp, n, d, _TYPES[dtype], q.data_ptr(),
+              ldq, s, sr, sg, first, first + 4 * (offsets.shape[0] - 1), st)
     return q, scales
 
 
@@ -533,14 +557,16 @@ def matmul_t_e4m3(x: torch.Tensor, xs: torch.Tensor, w: torch.Tensor, ws: torch.
 
 def grouped_matmul_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs: torch.Tensor | None = None,
                      ws: torch.Tensor | None = None, y: torch.Tensor | None = None, dtype: torch.dtype | None = None,
-                     status: torch.Tensor | None = None):
+                     status: torch.Tensor | None = None, picks: int | None = None):
     """y[p] = x[p] @ w[e].T for the rows offsets[e] <= p < offsets[e+1] of every
     expert (offsets: Routing.offsets).  x (P, K) and w (E, O, K) both bf16,
     both f16, or both e4m3 with xs (P, ceil(K/128)) and ws (E, ceil(O/128),
     ceil(K/128)).  y (P, O) of ``dtype`` (f32 unless said otherwise, bf16 or
     f16); f32 sums.  Rows of y outside every expert's range are not written.
     Rows and matrices of x and w must lie a multiple of 16 bytes apart.
-    Offsets that decrease or pass P set bit 2 of ``status``."""
+    Offsets that decrease or pass P set bit 2 of ``status``.  ``picks`` (a slice
+    of the experts, whose offsets span some of the rows): about how many rows
+    they span, P unless said otherwise; kernels and splits are chosen by it."""
     _groups(w, offsets)
     E, O, K = w.shape
     xsp, xr, xg, wsp = _operands(x, w, xs, ws, (E, _blocks(O), _blocks(K)))
@@ -548,15 +574,15 @@ def grouped_matmul_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs
     y = _result(x, y, (P, O), dtype)
     ldx, ldw = _operand_stride(x, "x"), _operand_stride(w, "w")
     dev = _on(x, w, offsets, xs, ws, y, status)
-    _call("mb_grouped_matmul_t", dev, x.data_ptr(), _TYPES[x.dtype], ldx, xsp, xr, xg, P,
+    _call("mb_grouped_matmul_t_slice", dev, x.data_ptr(), _TYPES[x.dtype], ldx, xsp, xr, xg, P,
           w.data_ptr(), w.stride(0), ldw, wsp, E, O, K, offsets.data_ptr(), y.data_ptr(),
-          _TYPES[y.dtype], _rows_of(y, "y"), _status_ptr(status))
+          _TYPES[y.dtype], _rows_of(y, "y"), P if picks is None else _picks(picks, P), _status_ptr(status))
     return y
 
 
 def grouped_swiglu_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs: torch.Tensor | None = None,
                      ws: torch.Tensor | None = None, q: torch.Tensor | None = None, scales: torch.Tensor | None = None,
-                     status: torch.Tensor | None = None):
+                     status: torch.Tensor | None = None, picks: int | None = None):
     """The grouped product with gate|up matrices w (E, 2I, K) (I gate rows, then
     I up rows; ws (E, 2, ceil(I/128), ceil(K/128)) for e4m3), SiLU(gate) * up
     in f32, and its rows in operand form of x's type: returns (q (P, I), scales
@@ -578,14 +604,14 @@ def grouped_swiglu_t(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, xs
     ldx, ldw = _operand_stride(x, "x"), _operand_stride(w, "w")
     dev = _on(x, w, offsets, xs, ws, q, scales, status)
     if q is None:
-        q = _new_operand(x, P, I, x.dtype)
+        q = _new_operand(x, P, I, x.dtype) if I & 15 else x.new_empty((P, I))
     s, sr, sg = None, 0, 0
     if x.dtype is _E4M3:
         scales = _new_scales(x, P, _blocks(I)) if scales is None else scales
         s, (sr, sg) = scales.data_ptr(), scales.stride()
-    _call("mb_grouped_swiglu_t", dev, x.data_ptr(), _TYPES[x.dtype], ldx, xsp, xr, xg, P,
+    _call("mb_grouped_swiglu_t_slice", dev, x.data_ptr(), _TYPES[x.dtype], ldx, xsp, xr, xg, P,
           w.data_ptr(), w.stride(0), ldw, wsp, E, I, K, offsets.data_ptr(), q.data_ptr(),
-          _rows_of(q, "q"), s, sr, sg, _status_ptr(status))
+          _rows_of(q, "q"), s, sr, sg, P if picks is None else _picks(picks, P), _status_ptr(status))
     return q, scales
 
 

@@ -68,18 +68,21 @@ def _float_buffers(ex: FloatExperts, P: int, workspace):
 
 
 def run_float_experts(ex: FloatExperts, x: torch.Tensor, routing, y: torch.Tensor, workspace,
-                      status: torch.Tensor) -> None:
+                      status: torch.Tensor, picks: int | None = None) -> None:
     """Every expert's picks through its float matrices into y (one row per
     pick, in routing order): the picks' rows in operand form, the grouped
     gate|up product with SiLU(gate) * up back in operand form, the grouped down
-    product with f32 results."""
+    product with f32 results.  ``picks``: as for :func:`run_experts`; then only
+    the picks within routing.offsets are put into operand form."""
     P = routing.P
     if P == 0:
         return
     q, qs, a, as_ = _float_buffers(ex, P, workspace)
-    D.operand_rows(x, ex.dtype, routing.sorted_rows[:P], q, qs, status)
-    D.grouped_swiglu_t(q, ex.gu, routing.offsets, qs, ex.gu_s, a, as_, status)
-    D.grouped_matmul_t(a, ex.down, routing.offsets, as_, ex.dn_s, y[:P], status=status)
+    part = {} if picks is None or picks == P else dict(picks=picks)
+    D.operand_rows(x, ex.dtype, routing.sorted_rows[:P], q, qs, status,
+                   **(dict(offsets=routing.offsets) if part else {}))
+    D.grouped_swiglu_t(q, ex.gu, routing.offsets, qs, ex.gu_s, a, as_, status, **part)
+    D.grouped_matmul_t(a, ex.down, routing.offsets, as_, ex.dn_s, y[:P], status=status, **part)
 
 
 def run_experts(experts: LayerExperts, x: torch.Tensor, row_exp: torch.Tensor, routing, y: torch.Tensor,
@@ -91,7 +94,7 @@ def run_experts(experts: LayerExperts, x: torch.Tensor, row_exp: torch.Tensor, r
     the picks these experts get (default routing.P; smaller when routing
     covers other ranks' experts too), for the choice of kernels."""
     if isinstance(experts, FloatExperts):
-        return run_float_experts(experts, x, routing, y, workspace, status)
+        return run_float_experts(experts, x, routing, y, workspace, status, picks)
     ex, P = experts, routing.P
     plan = kernel_plan(ex, P if picks is None else picks, gemm_min_rows)
     for kind, rows in plan:

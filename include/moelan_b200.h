@@ -419,6 +419,26 @@ int mb_grouped_swiglu_t(const void *x, int type, int64_t ldx, const float *xs, i
                         const int32_t *offsets, void *q, int64_t ldq, float *qs, int64_t qs_row, int64_t qs_group,
                         unsigned *status, void *stream);
 
+/* The three for a slice of the experts (expert parallelism: w, ws and offsets
+ * of E local experts, while rows, x and y hold every rank's P picks).  `picks`,
+ * 0 .. P: how many rows lie within offsets[0] .. offsets[E] as far as the host
+ * knows (P / ranks, say); kernels and splits are chosen by it, and any value
+ * gives right results (in another order of f32 sums).  mb_operand_rows_slice
+ * makes the rows *first <= p < *last only (device addresses, offsets and
+ * offsets + E; both NULL for every row) and leaves the others.  mb_operand_rows
+ * and the grouped products are these with every row. */
+int mb_operand_rows_slice(const void *x, int x_type, int64_t ldx, int64_t n_src, const int32_t *rows, int64_t n, int d,
+                          int type, void *q, int64_t ldq, float *scales, int64_t s_row, int64_t s_group,
+                          const int32_t *first, const int32_t *last, unsigned *status, void *stream);
+int mb_grouped_matmul_t_slice(const void *x, int type, int64_t ldx, const float *xs, int64_t xs_row, int64_t xs_group,
+                              int64_t P, const void *w, int64_t w_expert, int64_t ldw, const float *ws, int E, int O,
+                              int K, const int32_t *offsets, void *y, int y_type, int64_t ldy, int64_t picks,
+                              unsigned *status, void *stream);
+int mb_grouped_swiglu_t_slice(const void *x, int type, int64_t ldx, const float *xs, int64_t xs_row, int64_t xs_group,
+                              int64_t P, const void *w, int64_t w_expert, int64_t ldw, const float *ws, int E, int I,
+                              int K, const int32_t *offsets, void *q, int64_t ldq, float *qs, int64_t qs_row,
+                              int64_t qs_group, int64_t picks, unsigned *status, void *stream);
+
 /* x @ w.T for one e4m3 matrix w (O, K) with block scales ws (ceil(O/128),
  * ceil(K/128)) and e4m3 rows x (n, K) with scales xs (beside mb_matmul_t):
  * mb_grouped_matmul_t of one expert with every row. */

@@ -6,8 +6,8 @@ whose helpers these tests use; each is derived beside its test where it differs.
 import pytest
 import torch
 
-from test_gpu_float import (BF16, E4M3, F16, F32, G, ceil, check_grouped, close, gen, offsets_of, plain_e4m3, rand_rows,
-                            rand_weights, round_tol, same_bits, sum_tol, want_grouped, want_swiglu)
+from test_gpu_float import (BF16, E4M3, F16, F32, G, ceil, close, float_layer, gen, layer_reference, offsets_of,
+                            plain_e4m3, rand_rows, rand_weights, round_tol, same_bits, sum_tol, want_grouped, want_swiglu)
 from test_gpu_float import D  # noqa: F401  (fixture)
 
 pytestmark = pytest.mark.gpu
@@ -210,3 +210,155 @@ def test_operators_take_each_others_rows_at_any_width(D, dtype, H, I):
         m, ms, mw = rand_weights((I, H), E4M3, g)
         want, S = wide(q, s) @ mw.t(), wide(q, s).abs() @ mw.abs().t()
         close(D.matmul_t_e4m3(q, s, m, ms), want, sum_tol(H, S) + round_tol(want, F32))
+
+
+# ---- slices of the experts (expert parallelism) ------------------------------------------------------
+
+@pytest.mark.parametrize("picks", [0, 1, 40, 300, 700])
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+def test_products_are_right_whatever_picks_says(D, dtype, picks):
+    """A slice's offsets within many rows: passes and splits follow `picks`, results do not depend on it beyond the order of
+    sums; rows outside stay."""
+    g = gen(picks)
+    P, K, O, E = 700, 272, 256, 4
+    off = offsets_of([33, 0, 150, 5], 100)
+    x, xs, xw = rand_rows((P, K), dtype, g)
+    w, ws, ww = rand_weights((E, O, K), dtype, g)
+    y = torch.full((P, O), 7.0, device="cuda")
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    D.grouped_matmul_t(x, w, off, xs, ws, y=y, status=st, picks=picks)
+    want, S, real = want_grouped(xw, ww, off)
+    close(y[real], want[real], (sum_tol(K, S) + round_tol(want, F32))[real])
+    assert (y[~real] == 7.0).all() and int(st) == 0
+    g2, gs2, gw2 = rand_weights((E, 2, 128, K), dtype, g, scale=3.0 / K ** 0.5)
+    q = torch.full((P, 128), 7.0, device="cuda").to(dtype)
+    s = torch.full((P, 1), 7.0, device="cuda") if dtype == E4M3 else None
+    D.grouped_swiglu_t(x, g2.reshape(E, 256, K), off, xs, gs2, q=q, scales=s, status=st, picks=picks)
+    a, tol, _ = want_swiglu(xw, gw2.reshape(E, 256, K), off, 128, K)
+    assert (q[~real].float() == 7.0).all() and int(st) == 0
+    if dtype != E4M3:
+        close(q[real], a[real], (tol + round_tol(a, dtype))[real])
+        return
+    assert (s[~real] == 7.0).all()
+    sw = s.double().expand(P, 128)
+    close(q[real].double() * sw[real], a[real],
+          (tol * 17 / 16 + 2.0 ** -4 * a.abs() * (1 + 2.0 ** -20) + 2.0 ** -10 * sw)[real])
+
+
+@pytest.mark.parametrize("dst", [E4M3, BF16])
+@pytest.mark.parametrize("blocks,k", [(0, 8), (1, 8)], ids=["few rows", "many rows"])
+@pytest.mark.parametrize("first,last", [(0, -1), (100, 3000), (3, 4), (700, 700), (2047, 10 ** 9), (-5, 60), (900, 20)])
+def test_operand_rows_of_a_slice_only(D, dst, blocks, k, first, last):
+    """Only the rows within the offsets are made (and only their indices looked at); the others keep what they held."""
+    T = 16 * torch.cuda.get_device_properties(0).multi_processor_count if blocks else 500
+    d = 512
+    g = gen(T + first)
+    x = torch.randn((T, d), generator=g, device="cuda")
+    n = T * k
+    rows = torch.randint(0, T, (n,), generator=g, device="cuda", dtype=torch.int32)
+    last = n if last == -1 else last
+    lo, hi = max(first, 0), max(min(last, n), max(first, 0))
+    rows[:lo], rows[hi:] = 2 ** 31 - 1, -7                       # nothing looks at these
+    q = torch.full((n, d), 3.0, device="cuda").to(dst)
+    s = torch.full((n, d // G), 3.0, device="cuda") if dst == E4M3 else None
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    off = torch.tensor([first, lo, last], dtype=torch.int32, device="cuda")
+    D.operand_rows(x, dst, rows=rows, q=q, scales=s, status=st, offsets=off)
+    assert int(st) == 0
+    assert (q[:lo].float() == 3).all() and (q[hi:].float() == 3).all()
+    assert s is None or ((s[:lo] == 3).all() and (s[hi:] == 3).all())
+    if hi > lo:
+        want = x[rows[lo:hi].long()]
+        wq, ws = plain_e4m3(want) if dst == E4M3 else (want.to(dst), None)
+        assert same_bits(q[lo:hi], wq) and (s is None or torch.equal(s[lo:hi], ws))
+
+
+class OneProcess:
+    """torch.distributed for the ranks of a group that run one after the other in this process: a first pass of every rank
+    records what it gathers, a second one hands all ranks' parts out."""
+
+    def __init__(self, world):
+        self.world, self.rank, self.sent, self.play, self.at = world, 0, {}, False, 0
+
+    def start(self, rank, play):
+        self.rank, self.play, self.at = rank, play, 0
+
+    def get_world_size(self, group=None):
+        return self.world
+
+    def get_rank(self, group=None):
+        return self.rank
+
+    def _coalescing_manager(self, group=None, device=None):
+        import contextlib
+        return contextlib.nullcontext()
+
+    def all_gather_into_tensor(self, out, inp, group=None):
+        if not self.play:
+            self.sent[self.rank, self.at] = inp.clone()
+        parts = [self.sent[r, self.at] if self.play else inp for r in range(self.world)]
+        out.copy_(torch.cat([p.reshape(inp.shape) for p in parts]).view(out.shape))
+        self.at += 1
+
+    def all_to_all_single(self, out, inp, out_rows, in_rows, group=None):
+        assert self.world == 1
+        out.copy_(inp)
+
+    def reduce_scatter_tensor(self, out, inp, group=None):
+        T = out.shape[0]
+        out.copy_(inp[self.rank * T:(self.rank + 1) * T])
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("world", [1, 2, 4])
+def test_gather_layer_of_float_experts(D, monkeypatch, dtype, T, world):
+    """EPGatherLayer with a slice of the float experts on each of `world` ranks, run one after the other: the ranks' partial
+    sums add up to the layer (tolerance as in test_layer_of_float_experts, and an addition for each rank)."""
+    from distributedmoellm_b200 import ep
+    from distributedmoellm_b200.store import FloatExperts
+    E, H, I, k = 8, 272, 208, 3
+    layer, wide = float_layer(dtype, E, H, I, k, 97)
+    x = torch.randn((world * T, H), generator=gen(T), device="cuda")
+    layer(x)
+    want, mag = layer_reference(D, layer, wide, x, dtype, layer.buffers(world * T))
+    fake = OneProcess(world)
+    monkeypatch.setattr(ep, "dist", fake)
+    ranks = []
+    El = E // world
+    for r in range(world):
+        fake.start(r, False)
+        ex = FloatExperts(El, H, I, dtype, "cuda")
+        for j in range(El):
+            e = r * El + j
+            ex.put(j, layer.experts.gu[e], layer.experts.down[e], None if dtype != E4M3 else layer.experts.gu_s[e],
+                   None if dtype != E4M3 else layer.experts.dn_s[e])
+        ranks.append(ep.EPGatherLayer(layer.router, ex, E, k))
+    for play in (False, True):
+        for r, l in enumerate(ranks):
+            fake.start(r, play)
+            if l._bufs:                     # whatever earlier calls left in workspaces and results is not seen
+                b = l.buffers(T)
+                b.y.fill_(float("nan"))
+                for w in b.ws.values():
+                    w.fill_(0x7F)
+            l(x[r * T:(r + 1) * T])
+            assert l.status(T) == 0
+    got = sum(l.buffers(T).partial.double() for l in ranks)
+    half = {E4M3: 2.0 ** -4, BF16: 2.0 ** -8}[dtype]
+    close(got, want, half * mag * 1.01 + 1e-4 * mag.amax(1, keepdim=True), f"{world} ranks")
+
+
+@pytest.mark.parametrize("dtype", [E4M3, F16])
+@pytest.mark.parametrize("T", [1, 50])
+def test_exchange_layer_of_float_experts(D, monkeypatch, dtype, T):
+    """EPLayer (rows exchanged and regrouped by local expert) over float experts, as a single rank: the layer's results."""
+    from distributedmoellm_b200 import ep
+    E, H, I, k = 8, 272, 208, 3
+    layer, wide = float_layer(dtype, E, H, I, k, 98)
+    x = torch.randn((T, H), generator=gen(T), device="cuda")
+    whole = layer(x).clone()
+    monkeypatch.setattr(ep, "dist", OneProcess(1))
+    ops = ep.DeviceOps(layer.router, layer.experts, E, k)
+    got = ep.EPLayer(ops, E, k, H)(x)
+    assert torch.equal(got, whole) and int(ops._ws["status"]) == 0
