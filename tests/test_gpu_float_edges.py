@@ -6,6 +6,7 @@ whose helpers these tests use; each is derived beside its test where it differs.
 import pytest
 import torch
 
+import test_gpu_float as base
 from test_gpu_float import (BF16, E4M3, F16, F32, G, ceil, close, float_layer, gen, layer_reference, offsets_of,
                             plain_e4m3, rand_rows, rand_weights, round_tol, same_bits, sum_tol, want_grouped, want_swiglu)
 from test_gpu_float import D  # noqa: F401  (fixture)
@@ -362,3 +363,52 @@ def test_exchange_layer_of_float_experts(D, monkeypatch, dtype, T):
     ops = ep.DeviceOps(layer.router, layer.experts, E, k)
     got = ep.EPLayer(ops, E, k, H)(x)
     assert torch.equal(got, whole) and int(ops._ws["status"]) == 0
+
+
+# ---- accuracy of f32 results -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16, F16])
+@pytest.mark.parametrize("K", [2048, 7168])
+@pytest.mark.parametrize("counts", [[3], [40], [300, 0, 130], [5] * 40], ids=["3", "40", "300+130", "40x5"])
+def test_f32_results_over_long_columns(D, dtype, K, counts):
+    """Few rows (split over K), ordinary ones and many, against 64 bits, relative in norm.
+
+    The tensor cores cut an f32 sum at each step of 32 bytes of columns: by 0.36 of 2^-23 of the sum so far on average, and
+    over n steps of random products the sums so far add up to 2 n / 3 of the last.  16-bit types: n = 16 steps between two
+    f32 additions (256 columns): 4.6e-7; the additions behind them, rounded, come to 2.5e-8 sqrt(K / 512) <= 1e-7, added as
+    squares: below 5e-7.  (Sums over all of K, n = 128 from 2048 columns, would be at 3.7e-6.)  e4m3: n = 4 steps a group:
+    1.15e-7, the scaled additions 2.5e-8 sqrt(K / 256) <= 1.35e-7 and the scales' products 3e-8: 1.8e-7, and a bound of 3e-7
+    for what chance adds."""
+    g = gen(K + len(counts))
+    off = offsets_of(counts)
+    x, xs, xw = rand_rows((int(off[-1]), K), dtype, g)
+    w, ws, ww = rand_weights((len(counts), 384, K), dtype, g)
+    y = D.grouped_matmul_t(x, w, off, xs, ws)
+    want, _, _ = want_grouped(xw, ww, off)
+    error = float((y.double() - want).norm() / want.norm())
+    assert error < (3e-7 if dtype == E4M3 else 5e-7), error
+
+
+# ---- rows made once and copied, wherever that way begins ---------------------------------------------
+
+def rows_for_every_sm():
+    return 16 * torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.parametrize("more", [-1, 0, 3, 100])
+@pytest.mark.parametrize("src,dst,k,d", [(F32, E4M3, 8, 512), (F32, E4M3, 5, 400), (BF16, E4M3, 4, 2048), (F32, BF16, 6, 768),
+                                         (F16, F16, 4, 1032)])
+def test_operand_rows_of_many_picks_around_the_rule(D, src, dst, k, d, more):
+    """From sixteen rows of x for every SM on, each row is made once; one row fewer, for every pick."""
+    base.test_operand_rows_of_many_picks(D, src, dst, rows_for_every_sm() + more, k, d)
+
+
+@pytest.mark.parametrize("d", [2736, 2752, 2768, 2776, 2784])
+def test_operand_rows_made_once_at_the_shared_memory_limit(D, d):
+    """bf16 rows of up to 2768 columns fit sixteen at a time (2 d bytes and a scale's place per 128 columns each, 88 KB in
+    all); wider ones are made for every pick."""
+    T = rows_for_every_sm()
+    x = torch.randn((T, d), generator=gen(d), device="cuda")
+    rows = torch.arange(T, device="cuda", dtype=torch.int32).repeat(4)
+    q, _ = D.operand_rows(x, BF16, rows=rows)
+    assert torch.equal(q, x[rows.long()].to(BF16))
