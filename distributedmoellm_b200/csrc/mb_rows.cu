@@ -8,12 +8,11 @@
 // A warp takes four groups of a row (512 columns): lane l holds columns 4l .. 4l+3 of each, loaded at once; the four
 // maxima are reduced together, and each group's scale is worked out by the eight lanes that end with its maximum.
 //
-// Two kernels.  operand_rows_kernel makes each row of the result from its row of x; bound by instructions (about 200 a
-// warp) when tokens have many picks, since every pick of a token repeats the work.  spread_rows_kernel makes each row
-// of x once, into shared memory, looks through `rows` for its picks and copies the row to them.  Looking costs
-// n * 4 bytes per sixteen rows of x, which pays for many picks of not too many rows.  us, first way / second, rows of
-// 2048 columns from f32: 32768 from 4096 44.9 / 31 (3.3 TB/s), 16384 from 4096 23.8 / 19, 18944 from 2368 26.1 / 19.2,
-// 9472 from 2368 13.7 / 11.8.
+// Two kernels.  operand_rows_kernel makes each row of the result from its row of x; e4m3 rows are bound by instructions
+// (about 200 a warp) when tokens have many picks, since every pick of a token repeats the work.  spread_rows_kernel, for
+// e4m3, makes each row of x once, into shared memory, looks through `rows` for its picks and copies the row to them.
+// Looking costs n * 4 bytes per sixteen rows of x, which pays for long rows.  us in graphs, made once / for each pick, from
+// f32: 32768 rows of 2048 from 4096 30.0 / 46.2 (3.4 TB/s), 18944 from 2368 16.7 / 25.7, 9472 from 2368 10.4 / 13.9.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -177,22 +176,21 @@ constexpr int kSpreadThreads = 32 * kSpreadRows;
 constexpr int kSegment = 4 * kSpreadThreads;   // picks looked through at a time
 constexpr int kSpreadSmem = 88 << 10;     // for the rows, at most: two blocks per SM
 
-// Sixteen rows of x, each put into operand form once and copied to its picks.  Block 0 takes the picks of no row of x.
-// Needs 16 bytes at a time to be aligned in q, four columns in x, and d * bytes a multiple of 16.
-template <typename SRC, int TYPE>
+// Sixteen rows of x, each put into e4m3 form once and copied to its picks.  Block 0 takes the picks of no row of x.
+// Needs 16 bytes at a time to be aligned in q, four columns in x, and d a multiple of 16.
+template <typename SRC>
 __global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const SRC* __restrict__ x, int64_t ldx, int n_src,
                                                           const int32_t* __restrict__ rows, int n, int d,
-                                                          uint8_t* __restrict__ q, int64_t ldq_bytes,
+                                                          uint8_t* __restrict__ q, int64_t ldq,
                                                           float* __restrict__ scales, int64_t s_row, int64_t s_group,
                                                           unsigned* status)
 {
-    constexpr int B = TYPE == MB_T_E4M3 ? 1 : 2;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint16_t found[kSegment], slots[kSegment];
     __shared__ int count;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int ng = (d + kScaleBlock - 1) / kScaleBlock, bytes = d * B;
-    float* sc = reinterpret_cast<float*>(smem + kSpreadRows * bytes);      // [kSpreadRows][ng]
+    const int ng = (d + kScaleBlock - 1) / kScaleBlock;
+    float* sc = reinterpret_cast<float*>(smem + kSpreadRows * d);      // [kSpreadRows][ng]
     const int r0 = blockIdx.x * kSpreadRows;
     mb_pdl_trigger();
     mb_pdl_wait();
@@ -209,24 +207,18 @@ __global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const SRC* 
     load(0);
     if (r0 + warp < n_src) {
         const SRC* from = x + (int64_t)(r0 + warp) * ldx;
-        uint8_t* row = smem + warp * bytes;
+        uint8_t* row = smem + warp * d;
         for (int g0 = 0; g0 < ng; g0 += kGroups) {
             const int c0 = g0 * kScaleBlock + 4 * lane;
             float v[kGroups][4];
             load_groups<SRC, true>(v, from, c0, d, true);
             uint32_t u[kGroups];
-            if constexpr (TYPE == MB_T_E4M3) {
-                const float s = encode_groups(v, u, lane);
-                if ((lane & 7) == 0 && g0 + lane / 8 < ng) sc[warp * ng + g0 + lane / 8] = s;
-            }
+            const float s = encode_groups(v, u, lane);
+            if ((lane & 7) == 0 && g0 + lane / 8 < ng) sc[warp * ng + g0 + lane / 8] = s;
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
                 const int c = c0 + g * kScaleBlock;
-                if (c >= d) continue;
-                if constexpr (TYPE == MB_T_E4M3)
-                    *reinterpret_cast<uint32_t*>(row + c) = u[g];
-                else
-                    *reinterpret_cast<uint2*>(row + 2 * c) = round4<TYPE>(v[g]);
+                if (c < d) *reinterpret_cast<uint32_t*>(row + c) = u[g];
             }
         }
     }
@@ -252,12 +244,11 @@ __global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const SRC* 
             const int64_t p = base + found[k];
             const bool real = slot < kSpreadRows;
             if (!real && lane == 0 && status) atomicOr(status, MB_STATUS_BADARG);
-            uint8_t* dst = q + p * ldq_bytes;
-            for (int i = 16 * lane; i < bytes; i += 512)
+            uint8_t* dst = q + p * ldq;
+            for (int i = 16 * lane; i < d; i += 512)
                 *reinterpret_cast<uint4*>(dst + i) =
-                    real ? *reinterpret_cast<const uint4*>(smem + slot * bytes + i) : make_uint4(0u, 0u, 0u, 0u);
-            if (TYPE == MB_T_E4M3)
-                for (int g = lane; g < ng; g += 32) scales[p * s_row + g * s_group] = real ? sc[slot * ng + g] : 1.0f;
+                    real ? *reinterpret_cast<const uint4*>(smem + slot * d + i) : make_uint4(0u, 0u, 0u, 0u);
+            for (int g = lane; g < ng; g += 32) scales[p * s_row + g * s_group] = real ? sc[slot * ng + g] : 1.0f;
         }
         __syncthreads();
     }
@@ -271,29 +262,33 @@ int launch(const SRC* x, int64_t ldx, int64_t n_src, const int32_t* rows, int64_
     constexpr int B = TYPE == MB_T_E4M3 ? 1 : 2;
     const bool vec = d % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 && (uintptr_t)x % (4 * sizeof(SRC)) == 0 &&
                      (uintptr_t)q % (4 * B) == 0;
-    // Worth it from four picks a row on, with a block of rows for every SM (16384 from 2048 rows: 23.7 us, made for each
-    // pick 22.5; 9600 from 1200: 19.1 and 13.2), and few enough rows that looking through the picks (4 n bytes for each
-    // 16 rows) stays below reading x for each pick.  A slice of the experts is made for each pick: it has 1 / ranks of them
-    // (the bounds of its rows in the kernel cost every call 1.1 of 29.4 us at 32768 from 4096).
-    const int ng = (d + kScaleBlock - 1) / kScaleBlock;
-    const int64_t smem = (int64_t)kSpreadRows * (d * B + ng * 4);
-    if (rows && !first && vec && n >= 4 * n_src && n_src >= kSpreadRows * mb_num_sms() && n_src <= 8 * (int64_t)d &&
-        smem <= kSpreadSmem && d * B % 16 == 0 && ldq * B % 16 == 0 && (uintptr_t)q % 16 == 0) {
-        static thread_local uint64_t ready = 0;            // devices whose attribute is set
-        int dev = 0;
-        cudaGetDevice(&dev);
-        cudaError_t e = cudaSuccess;
-        if (!(ready >> (dev & 63) & 1))
-            e = cudaFuncSetAttribute(spread_rows_kernel<SRC, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     kSpreadSmem);
-        if (e == cudaSuccess) {
-            ready |= 1ull << (dev & 63);
-            e = mb_launch_pdl(spread_rows_kernel<SRC, TYPE>, dim3((unsigned)((n_src + kSpreadRows - 1) / kSpreadRows)),
-                              dim3(kSpreadThreads), (size_t)smem, st, x, ldx, (int)n_src, rows, (int)n, d, (uint8_t*)q,
-                              ldq * B, scales, s_row, s_group, status);
+    // Made once: e4m3, from four picks a row on, with a block of rows for every SM (16384 from 2048 rows of 2048: 23.7 us,
+    // made for each pick 22.5; 9600 from 1200: 19.1 and 13.2), and at most four rows of x a column, since looking through
+    // the picks (4 n bytes for each 16 rows) has to stay below the work it saves (us, once / each: 2368 rows x 8 of 1024
+    // columns 13.0 / 13.9, of 512 11.7 / 8.0; 4096 x 8 of 1024 22.0 / 22.5, of 512 19.9 / 12.3; 8192 x 8 of 2048 83.9 /
+    // 92.7, of 1024 71.3 / 46.5).  Rows of 16 bits cost little to make again, and the copies lose at every size (4096 x 8 of
+    // 2048 columns 34.8 / 29.9, from bf16 41.5 / 25.3).  A slice of the experts has a part of the picks and is
+    // made for each (its bounds in the other kernel cost every call 1.1 of 29.4 us at 32768 from 4096).
+    if constexpr (TYPE == MB_T_E4M3) {
+        const int ng = (d + kScaleBlock - 1) / kScaleBlock;
+        const int64_t smem = (int64_t)kSpreadRows * (d + ng * 4);
+        if (rows && !first && vec && n >= 4 * n_src && n_src >= kSpreadRows * mb_num_sms() && n_src <= 4 * (int64_t)d &&
+            smem <= kSpreadSmem && d % 16 == 0 && ldq % 16 == 0 && (uintptr_t)q % 16 == 0) {
+            static thread_local uint64_t ready = 0;        // devices whose attribute is set
+            int dev = 0;
+            cudaGetDevice(&dev);
+            cudaError_t e = cudaSuccess;
+            if (!(ready >> (dev & 63) & 1))
+                e = cudaFuncSetAttribute(spread_rows_kernel<SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSpreadSmem);
+            if (e == cudaSuccess) {
+                ready |= 1ull << (dev & 63);
+                e = mb_launch_pdl(spread_rows_kernel<SRC>, dim3((unsigned)((n_src + kSpreadRows - 1) / kSpreadRows)),
+                                  dim3(kSpreadThreads), (size_t)smem, st, x, ldx, (int)n_src, rows, (int)n, d, (uint8_t*)q,
+                                  ldq, scales, s_row, s_group, status);
+            }
+            if (e != cudaSuccess) return mb_fail(MB_ECUDA, "mb_operand_rows: %s", cudaGetErrorString(e));
+            return MB_OK;
         }
-        if (e != cudaSuccess) return mb_fail(MB_ECUDA, "mb_operand_rows: %s", cudaGetErrorString(e));
-        return MB_OK;
     }
     const int cols = kGroups * kScaleBlock;
     const dim3 grid((unsigned)((n + kRowsPerBlock - 1) / kRowsPerBlock), (unsigned)((d + cols - 1) / cols));

@@ -102,7 +102,7 @@ def test_operand_rows_groups_of_nothing_but_nan_have_scale_one(D, T, k, d):
     rows and picks that each row is made once."""
     if k:
         T = 16 * torch.cuda.get_device_properties(0).multi_processor_count
-        d = ceil(d, 16) * 16
+        d = 512 + ceil(d, 16) * 16
     g = gen(d)
     x = torch.randn((T, d), generator=g, device="cuda")
     x[0] = float("nan")
@@ -252,7 +252,7 @@ def test_products_are_right_whatever_picks_says(D, dtype, picks):
 def test_operand_rows_of_a_slice_only(D, dst, blocks, k, first, last):
     """Only the rows within the offsets are made (and only their indices looked at); the others keep what they held."""
     T = 16 * torch.cuda.get_device_properties(0).multi_processor_count if blocks else 500
-    d = 512
+    d = 1024
     g = gen(T + first)
     x = torch.randn((T, d), generator=g, device="cuda")
     n = T * k
@@ -396,19 +396,30 @@ def rows_for_every_sm():
 
 
 @pytest.mark.parametrize("more", [-1, 0, 3, 100])
-@pytest.mark.parametrize("src,dst,k,d", [(F32, E4M3, 8, 512), (F32, E4M3, 5, 400), (BF16, E4M3, 4, 2048), (F32, BF16, 6, 768),
-                                         (F16, F16, 4, 1032)])
+@pytest.mark.parametrize("src,dst,k,d", [(F32, E4M3, 8, 1024), (F32, E4M3, 5, 656), (BF16, E4M3, 4, 2048), (F16, E4M3, 6, 784),
+                                         (F32, BF16, 6, 768), (F16, F16, 4, 1032)])
 def test_operand_rows_of_many_picks_around_the_rule(D, src, dst, k, d, more):
-    """From sixteen rows of x for every SM on, each row is made once; one row fewer, for every pick."""
+    """From sixteen rows of x for every SM on, each e4m3 row of enough columns is made once; one row fewer, for every pick."""
     base.test_operand_rows_of_many_picks(D, src, dst, rows_for_every_sm() + more, k, d)
 
 
-@pytest.mark.parametrize("d", [2736, 2752, 2768, 2776, 2784])
+@pytest.mark.parametrize("d", [5440, 5456, 5472, 5488])
 def test_operand_rows_made_once_at_the_shared_memory_limit(D, d):
-    """bf16 rows of up to 2768 columns fit sixteen at a time (2 d bytes and a scale's place per 128 columns each, 88 KB in
-    all); wider ones are made for every pick."""
+    """Rows of up to 5456 columns fit sixteen at a time (d bytes and a scale per 128 columns each, 88 KB in all); wider ones
+    are made for every pick."""
     T = rows_for_every_sm()
     x = torch.randn((T, d), generator=gen(d), device="cuda")
     rows = torch.arange(T, device="cuda", dtype=torch.int32).repeat(4)
-    q, _ = D.operand_rows(x, BF16, rows=rows)
-    assert torch.equal(q, x[rows.long()].to(BF16))
+    q, s = D.operand_rows(x, E4M3, rows=rows)
+    wq, ws = plain_e4m3(x)
+    assert same_bits(q, wq[rows.long()]) and torch.equal(s, ws[rows.long()])
+
+
+def test_operand_rows_made_once_with_the_most_rows_a_column(D):
+    """Four rows of x a column, and one more, which is made for every pick."""
+    for T in (4096, 4097):
+        x = torch.randn((T, 1024), generator=gen(T), device="cuda")
+        rows = torch.randint(0, T, (4 * T,), generator=gen(1), device="cuda", dtype=torch.int32)
+        q, s = D.operand_rows(x, E4M3, rows=rows)
+        wq, ws = plain_e4m3(x)
+        assert same_bits(q, wq[rows.long()]) and torch.equal(s, ws[rows.long()])
