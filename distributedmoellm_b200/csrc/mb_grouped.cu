@@ -38,11 +38,11 @@
 // Every wait of a role is bounded (status word + abort flag), so each reaches the
 // CTA's (and cluster's) barriers at the end, which have no limit of their own.
 //
-// Few rows an expert: bound by memory (512 picks of 128 e4m3 experts of 2048 x
-// 768: 33-34 us, operands and results at 5.9-6.1 TB/s).  Many: products and epilogue each take 160-180 us of
-// the 250 of 4096 x 14336 x 4096 (e4m3, 1.92 PFLOP/s in bursts, 1.68 in a row
-// under the power limit); 16384 picks of f16 experts of 1536 x 2048 take 167-178
-// us (5.2-5.5 TB/s), of e4m3 experts of 2048 x 768 78 (4.5 TB/s).
+// Measured in bursts of a graph / in a row, where large calls meet the power limit.  Few rows an expert: 512 picks of 128
+// e4m3 experts of 2048 x 768, of which they meet about 105, take 34 / 38 us (170 MB of operands and results, 5.0 TB/s; DRAM
+// is busy half of the cycles, the rest goes to items of six steps and their hand-overs).  Many: products and epilogue each
+// take 160-180 us of the 247 / 288 of 4096 x 14336 x 4096 (e4m3, 1.95 / 1.67 PFLOP/s); 16384 picks of f16 experts of 1536 x
+// 2048 take 173 / 210 us (837 MB, 4.8 TB/s), of e4m3 experts of 2048 x 768 80 / 92 (4.3 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 

@@ -160,8 +160,9 @@ class FloatExperts:
     dtype float8_e4m3fn (with one f32 scale per block of 128 x 128 weights),
     bfloat16 or float16.  gu (E, 2I, H): each expert's gate rows, then its up
     rows; down (E, H, I); for e4m3 gu_s (E, 2, ceil(I/128), ceil(H/128)) and
-    dn_s (E, ceil(H/128), ceil(I/128)).  moelan keeps such experts dense in
-    host memory (moelan/experts.py:72-122)."""
+    dn_s (E, ceil(H/128), ceil(I/128)).  An expert that was never put is zeros,
+    and so are its picks' results (``present`` holds those that were).  moelan
+    keeps 16-bit experts dense in host memory (moelan/experts.py:72-122)."""
 
     def __init__(self, E: int, H: int, I: int, dtype: torch.dtype, device):
         from . import device as D

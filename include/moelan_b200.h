@@ -393,14 +393,16 @@ int mb_operand_rows(const void *x, int x_type, int64_t ldx, int64_t n_src, const
  * device, non-decreasing within 0 .. P (else MB_STATUS_BADARG is set and the
  * offending experts are left out: those whose range decreases or leaves 0 .. P,
  * and those whose range starts before the end of an earlier one that counts);
- * rows of y before offsets[0] and from offsets[E] on are left as they are.
+ * rows of y before offsets[0] and from offsets[E] on are left as they are.  y
+ * overlaps no operand.
  *   x (P, K) and w (E, O, K) of one type: MB_T_E4M3, MB_T_BF16 or MB_T_F16.
  *   ldx, ldw: elements between rows; w_expert: between experts' matrices.  x,
  *   w and these distances in bytes must be multiples of 16.  y rows are ldy
  *   elements apart (no alignment beyond the element's).
  *   MB_T_E4M3: xs[p, g] at xs[p * xs_row + g * xs_group], ws (E, ceil(O/128),
  *   ceil(K/128)) contiguous:
- *     y[p, o] = sum_g xs[p, g] * ws[e, o/128, g] * sum_{k in g} x[p, k] w[e, o, k].
+ *     y[p, o] = sum_g xs[p, g] * ws[e, o/128, g] * sum_{k in g} x[p, k] w[e, o, k]
+ *   with xs * ws first, in f32 (so it has to be a normal number, or 0).
  * 1 <= E <= 1024, P < 2^31. */
 int mb_grouped_matmul_t(const void *x, int type, int64_t ldx, const float *xs, int64_t xs_row, int64_t xs_group,
                         int64_t P, const void *w, int64_t w_expert, int64_t ldw, const float *ws, int E, int O, int K,
@@ -410,10 +412,11 @@ int mb_grouped_matmul_t(const void *x, int type, int64_t ldx, const float *xs, i
  * then the I up rows (moelan/experts.py:247-263 Expert), with the activation:
  *   a[p, j] = g / (1 + exp(-g)) * u,  g = x[p] @ w[e][j], u = x[p] @ w[e][I + j]
  * in f32, the exponential and the quotient by the device's fast functions (off
- * by at most (|g| + 8) 2^-22 of a, and by |g u| 2^-149), then put into operand form of x's type as mb_operand_rows does: q
- * (P, I) of `type`, and for MB_T_E4M3 its scales qs[p, g] at
- * qs[p * qs_row + g * qs_group].  ws (E, 2, ceil(I/128), ceil(K/128)): the gate
- * rows' blocks and the up rows' blocks, each half with its own grid. */
+ * by at most (|g| + 8) 2^-22 of a, and by |g u| 2^-149), then put into operand
+ * form of x's type as mb_operand_rows does: q (P, I) of `type`, and for
+ * MB_T_E4M3 its scales qs[p, g] at qs[p * qs_row + g * qs_group].
+ * ws (E, 2, ceil(I/128), ceil(K/128)): the gate rows' blocks and the up rows'
+ * blocks, each half with its own grid. */
 int mb_grouped_swiglu_t(const void *x, int type, int64_t ldx, const float *xs, int64_t xs_row, int64_t xs_group,
                         int64_t P, const void *w, int64_t w_expert, int64_t ldw, const float *ws, int E, int I, int K,
                         const int32_t *offsets, void *q, int64_t ldq, float *qs, int64_t qs_row, int64_t qs_group,
