@@ -431,9 +431,7 @@ def _picks(picks, P):
 def _new_operand(like: torch.Tensor, n: int, d: int, dtype):
     """Operand rows (n, d) that the products take: a multiple of 16 bytes apart."""
     step = 16 // dtype.itemsize
-    if d % step == 0:
-        return like.new_empty((n, d), dtype=dtype)
-    return like.new_empty((n, -(-d // step) * step), dtype=dtype)[:, :d]
+    return like.new_empty_strided((n, d), (-(-d // step) * step, 1), dtype=dtype)
 
 
 def operand_rows(x: torch.Tensor, dtype: torch.dtype, rows: torch.Tensor | None = None, q: torch.Tensor | None = None,
