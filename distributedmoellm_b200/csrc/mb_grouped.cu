@@ -501,6 +501,23 @@ __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.
 template <int R>
 __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
+// The items of experts whose offsets were not all in order: a range that starts before the end of an earlier one is left out,
+// so that no row has two writers and the items stay within the count that the launch allowed for.  (A call, which keeps its
+// code out of the way of launches whose offsets are in order: 0.06 us of the 6.9 of 120 picks of 16 e4m3 experts.)
+__device__ __noinline__ int disjoint_items(int2* meta, int* pstart, int E, int Nb, int MT)
+{
+    int total = 0;
+    for (int e = 0, end = 0; e < E; ++e) {
+        const int2 m = meta[e];
+        const int n = m.x < end ? 0 : m.y;
+        if (n < m.y) meta[e].y = 0;
+        if (n > 0) end = m.x + n;
+        pstart[e] = total;
+        total += Nb * ((n + MT - 1) / MT);
+    }
+    return total;
+}
+
 template <int TYPE, bool DUAL, bool WIDE, bool SMALL, int OUT>
 __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Roles<SMALL, TYPE == MB_T_E4M3>::kCtas)
     grouped_kernel(const __grid_constant__ GroupedArgs a, const __grid_constant__ Maps maps)
@@ -601,9 +618,7 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
             if (lane >= o) run += t;
         }
         if (lane == 31) wsum[warp] = run;
-        // Where no pair of offsets decreases, the ranges are disjoint.  Else what is left of them may overlap: a range that
-        // starts before the end of an earlier one is left out too, so that no row has two writers and the items stay within
-        // the count that the launch allowed for.
+        // Where no pair of offsets decreases, the ranges are disjoint.  Else what is left of them may overlap.
         bad = __syncthreads_or(bad);
         int before = run - mine, total = 0;
         for (int w = 0; w < kWarps; ++w) {
@@ -612,17 +627,7 @@ __global__ void __launch_bounds__(Roles<SMALL, TYPE == MB_T_E4M3>::kThreads, Rol
             total += s;
         }
         if (bad) {
-            if (threadIdx.x == 0) {
-                total = 0;
-                for (int e = 0, end = 0; e < a.E; ++e) {
-                    const int2 m = meta[e];
-                    const int n = m.x < end ? 0 : m.y;
-                    if (n < m.y) meta[e].y = 0;
-                    if (n > 0) end = m.x + n;
-                    pstart[e] = total;
-                    total += a.Nb * ((n + a.MT - 1) / a.MT);
-                }
-            }
+            if (threadIdx.x == 0) total = disjoint_items(meta, pstart, a.E, a.Nb, a.MT);
         } else {
             for (int e = e0; e < e1; ++e) pstart[e] += before;
         }
