@@ -423,3 +423,49 @@ def test_operand_rows_made_once_with_the_most_rows_a_column(D):
         q, s = D.operand_rows(x, E4M3, rows=rows)
         wq, ws = plain_e4m3(x)
         assert same_bits(q, wq[rows.long()]) and torch.equal(s, ws[rows.long()])
+
+
+@pytest.mark.parametrize("dtype", [E4M3, F16])
+def test_captured_slice_follows_its_offsets(D, dtype):
+    """run_experts over a slice, captured: replays on new picks, whose range begins and ends elsewhere, equal eager calls,
+    and rows outside the range stay."""
+    from distributedmoellm_b200 import layer as Lyr
+    from distributedmoellm_b200.store import FloatExperts
+    E, H, I, k, T, e0, El = 8, 272, 144, 2, 60, 2, 3
+    layer, _ = float_layer(dtype, E, H, I, k, 99)
+    ex = FloatExperts(El, H, I, dtype, "cuda")
+    for j in range(El):
+        e = e0 + j
+        ex.put(j, layer.experts.gu[e], layer.experts.down[e], None if dtype != E4M3 else layer.experts.gu_s[e],
+               None if dtype != E4M3 else layer.experts.dn_s[e])
+    P = T * k
+    x = torch.randn((T, H), generator=gen(1), device="cuda")
+    idx = torch.zeros((T, k), dtype=torch.int32, device="cuda")
+    w = torch.ones((T, k), device="cuda")
+    r = D.Routing(T, k, E, "cuda")
+    local = D.Routing.from_plan(r.counts[e0:e0 + El], r.offsets[e0:e0 + El + 1], r.sorted_rows[:P])
+    bufs, st = {}, torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def step(y):
+        D.permute(idx, w, E, r)
+        Lyr.run_experts(ex, x, None, local, y, lambda n, b: bufs.setdefault(n, torch.empty(b, dtype=torch.uint8, device="cuda")),
+                        st, 12, picks=P // 2)
+
+    def route(seed):
+        idx.copy_(torch.rand((T, E), generator=gen(seed), device="cuda").topk(k, dim=1).indices)
+    route(1)
+    got, want = torch.empty((P, H), device="cuda"), torch.empty((P, H), device="cuda")
+    step(got)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(got)
+    for seed in (2, 3):
+        route(seed)
+        got.fill_(5.0)
+        want.fill_(5.0)
+        g.replay()
+        step(want)
+        assert torch.equal(got, want) and int(st) == 0
+        lo, hi = int(local.offsets[0]), int(local.offsets[-1])
+        assert 0 < lo < hi < P and (got[:lo] == 5).all() and (got[hi:] == 5).all() and (got[lo:hi] != 5).any()
